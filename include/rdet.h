@@ -229,6 +229,89 @@ int32_t rdet_det_attention_decode_noalloc(const int32_t* q, const int32_t* k_cac
                                           uint32_t head_dim, uint32_t position, uint32_t window, int32_t* out,
                                           void* stream);
 
+/* ---- verification of drafted tokens ------------------------------------------
+ * A draft is a tree: node i of a sequence has a parent that comes before it
+ * (parents[i] < i, -1: the last committed token) and stands at position
+ * context + depth(i).  The operators below take caller-owned memory, launch on
+ * `stream` (a cudaStream_t or NULL), allocate nothing and keep nothing from one
+ * call for the next, so calls on different streams may overlap as long as
+ * their outputs and workspaces do not.  Their descriptor arrays are host
+ * memory that is read before the call returns.  No counterpart in the
+ * reference, which decodes one token at a time; the arithmetic is det_num v1's. */
+#define RDET_MAX_TREE_NODES 64
+typedef struct rdet_tree_seq {
+  const int32_t* k_cache; /* device, [num_kv_heads, cap, head_dim]: rows [0, context) are attended */
+  const int32_t* v_cache;
+  const int32_t* k_tree;  /* device, [num_kv_heads, tree_cap, head_dim]: row i is node i.  May be the */
+  const int32_t* v_tree;  /*   cache itself from row `context` on (k_cache + context * head_dim, tree_cap = cap) */
+  const int32_t* parents; /* host, [n_nodes] */
+  uint32_t cap, context, tree_cap, n_nodes; /* 1 <= n_nodes <= RDET_MAX_TREE_NODES */
+} rdet_tree_seq;
+
+/* det attention of every node of every sequence's tree: q and out are
+ * [nodes of all sequences, num_heads, head_dim], the sequences in order.  Node
+ * i attends, in the order of their positions, to the cache rows
+ * [max(0, p + 1 - window), context) with p its position, to its ancestors at
+ * positions >= p + 1 - window and to itself (window 0: no limit): the result is
+ * attention_output_into (det_kernels.rs:340-367) over those rows, bit for bit
+ * what rdet_det_attention_decode gives when the ancestors are committed.
+ * num_heads a multiple of num_kv_heads, 1 <= head_dim <= 512; context, and the
+ * attended rows, below 2^24.  workspace: at least
+ * rdet_det_attention_tree_workspace bytes, 256-byte aligned. */
+int32_t rdet_det_attention_tree_workspace(const rdet_tree_seq* seqs, uint32_t n_seqs, uint32_t num_heads,
+                                          uint32_t num_kv_heads, uint32_t head_dim, uint32_t window,
+                                          size_t* bytes_out);
+int32_t rdet_det_attention_tree(const rdet_tree_seq* seqs, uint32_t n_seqs, const int32_t* q, uint32_t num_heads,
+                                uint32_t num_kv_heads, uint32_t head_dim, uint32_t window, int32_t* out,
+                                void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rules on logits rows and the greedy token under them.  For token t of a row
+ * with logit l (Q16.16), count c (how often t occurs in history[0,
+ * history_len), plus in the row's own token and those of its ancestor rows):
+ *   c > 0:  l = l > 0 ? div_act(l, repetition) : mul_sat(l, repetition)
+ *           l = sub_sat(sub_sat(l, frequency * c), presence)
+ *           (frequency * c exact, then clamped to i32)
+ *   biased: l = add_sat(l, sum of t's entries in the bias list, exact, clamped to i32)
+ *   bit t of allow (word t / 32, bit t % 32) clear: the processed value is
+ *           INT32_MIN and t is not selected
+ * out (may be NULL, may be the logits row itself) receives the processed row;
+ * the row's token is the lowest index of the largest value among the allowed
+ * tokens, RDET_NO_TOKEN when none is allowed.  repetition > 0 (65536: none);
+ * history and bias ids outside the vocabulary are ignored.  parent: the row of
+ * this call that holds the parent node (below the row's own index), -1: none;
+ * token: the row's own drafted token, RDET_NO_TOKEN: none. */
+#define RDET_NO_TOKEN 0xffffffffu
+typedef struct rdet_logit_row {
+  const int32_t* logits;       /* device, [vocab] */
+  int32_t* out;                /* device, [vocab], or NULL */
+  const uint32_t* allow;       /* device, [(vocab + 31) / 32] words, or NULL: every token */
+  const uint32_t* history;     /* device, [history_len] */
+  const uint32_t* bias_ids;    /* device, [n_bias] */
+  const int32_t* bias_values;  /* device, [n_bias] Q16.16 */
+  uint32_t history_len, n_bias;
+  int32_t repetition, frequency, presence; /* Q16.16 */
+  int32_t parent;
+  uint32_t token;
+} rdet_logit_row;
+/* tokens_out: device, [n_rows].  Rows linked by `parent` lie within 192
+ * consecutive rows. */
+int32_t rdet_det_logits_rules(const rdet_logit_row* rows, uint32_t n_rows, uint32_t vocab, uint32_t* tokens_out,
+                              void* stream);
+
+/* Moves the drafted rows of an accepted path into the caches: for every move
+ * and KV head, cache row context + i becomes draft row path[i].  A move is one
+ * K or V cache of one layer; moves of a sequence share its path.  Path p is
+ * nodes[path_off[p] .. path_off[p + 1]), strictly increasing, at most
+ * RDET_MAX_TREE_NODES long (path_off and nodes: host memory).  draft may be the cache itself from row
+ * `context` on (cache + context * head_dim, draft_cap = cap). */
+typedef struct rdet_tree_move {
+  int32_t* cache;        /* device, [kv_heads, cap, head_dim] */
+  const int32_t* draft;  /* device, [kv_heads, draft_cap, head_dim] */
+  uint32_t cap, draft_cap, kv_heads, head_dim, context, path;
+} rdet_tree_move;
+int32_t rdet_det_tree_commit(const rdet_tree_move* moves, uint32_t n_moves, const uint32_t* nodes,
+                             const uint32_t* path_off, uint32_t n_paths, void* stream);
+
 /* Tensor-parallel batched decode (no counterpart in the reference, which runs
  * one process on the CPU).  Every rank
  * opens the same model on its own GPU; rank 0 creates an id with

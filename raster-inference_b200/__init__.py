@@ -38,9 +38,15 @@ SYMBOLS = [
     "rdet_prefill_finalize", "rdet_select", "rdet_select_batch", "rdet_decode", "rdet_decode_begin", "rdet_decode_range",
     "rdet_decode_finalize", "rdet_generate", "rdet_read", "rdet_commitment", "rdet_kv_prefix_commitments",
     "rdet_det_gemv", "rdet_det_linear",
-    "rdet_det_attention_decode", "rdet_det_attention_decode_noalloc", "rdet_det_attention_prefill", "rdet_convert_to_wgt", "rdet_get_stream", "rdet_tensor_core_prefill", "rdet_nccl_unique_id", "rdet_tp_init", "rdet_tp_world", "rdet_tp_shard_logits", "rdet_tp_ipc_export", "rdet_tp_ipc_connect", "rdet_seq_kernels_per_step", "rdet_last_error",
+    "rdet_det_attention_decode", "rdet_det_attention_decode_noalloc", "rdet_det_attention_prefill", "rdet_convert_to_wgt",
+    "rdet_det_attention_tree_workspace", "rdet_det_attention_tree", "rdet_det_logits_rules", "rdet_det_tree_commit",
+    "rdet_get_stream", "rdet_tensor_core_prefill", "rdet_nccl_unique_id", "rdet_tp_init", "rdet_tp_world", "rdet_tp_shard_logits", "rdet_tp_ipc_export", "rdet_tp_ipc_connect", "rdet_seq_kernels_per_step", "rdet_last_error",
     "rdet_version",
 ]
+
+
+NO_TOKEN = 0xFFFFFFFF
+MAX_TREE_NODES = 64
 
 
 class RdetError(RuntimeError):
@@ -58,6 +64,24 @@ class ModelInfo(C.Structure):
     _fields_ = [("hidden_size", C.c_uint32), ("vocab_size", C.c_uint32), ("num_layers", C.c_uint32),
                 ("num_heads", C.c_uint32), ("ple_dim", C.c_uint32), ("intermediate_size", C.c_uint32),
                 ("weight_bytes", C.c_uint64)]
+
+
+class TreeSeq(C.Structure):
+    _fields_ = [("k_cache", C.c_void_p), ("v_cache", C.c_void_p), ("k_tree", C.c_void_p), ("v_tree", C.c_void_p),
+                ("parents", C.c_void_p), ("cap", C.c_uint32), ("context", C.c_uint32), ("tree_cap", C.c_uint32),
+                ("n_nodes", C.c_uint32)]
+
+
+class LogitRow(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("out", C.c_void_p), ("allow", C.c_void_p), ("history", C.c_void_p),
+                ("bias_ids", C.c_void_p), ("bias_values", C.c_void_p), ("history_len", C.c_uint32),
+                ("n_bias", C.c_uint32), ("repetition", C.c_int32), ("frequency", C.c_int32),
+                ("presence", C.c_int32), ("parent", C.c_int32), ("token", C.c_uint32)]
+
+
+class TreeMove(C.Structure):
+    _fields_ = [("cache", C.c_void_p), ("draft", C.c_void_p), ("cap", C.c_uint32), ("draft_cap", C.c_uint32),
+                ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("context", C.c_uint32), ("path", C.c_uint32)]
 
 
 _lib = None
@@ -102,6 +126,10 @@ def lib() -> C.CDLL:
         "rdet_det_attention_decode_noalloc": [p, p, p, u32, u32, u32, u32, u32, u32, p, p],
         "rdet_det_attention_prefill": [p, p, p, u32, u32, u32, u32, u32, u32, u32, p, p],
         "rdet_convert_to_wgt": [p, i32, C.c_uint64, C.c_uint64, p, p, p, p],
+        "rdet_det_attention_tree_workspace": [p, u32, u32, u32, u32, u32, p],
+        "rdet_det_attention_tree": [p, u32, p, u32, u32, u32, u32, p, p, sz, p],
+        "rdet_det_logits_rules": [p, u32, u32, p, p],
+        "rdet_det_tree_commit": [p, u32, p, p, u32, p],
         "rdet_get_stream": [p, p],
         "rdet_tensor_core_prefill": [p],
         "rdet_nccl_unique_id": [p, sz],
@@ -437,3 +465,70 @@ def det_attention_decode_noalloc(q_ptr: int, k_ptr: int, v_ptr: int, cap: int, n
     _check(lib().rdet_det_attention_decode_noalloc(C.c_void_p(q_ptr), C.c_void_p(k_ptr), C.c_void_p(v_ptr), cap,
                                                    num_heads, num_kv_heads, head_dim, position, window,
                                                    C.c_void_p(out_ptr), C.c_void_p(stream) if stream else None))
+
+
+# ---- verification of drafted tokens ---------------------------------------------------
+class Descriptors:
+    """A host descriptor array of the draft-verification operators with the
+    host memory it points into; device pointers stay the caller's."""
+
+    def __init__(self, ctype, items, keep=()):
+        self.n = len(items)
+        self.array = (ctype * max(self.n, 1))(*[ctype(**it) for it in items])
+        self.keep = keep
+
+
+def tree_seqs(seqs) -> Descriptors:
+    """rdet_tree_seq array from dicts of k_cache, v_cache, cap, context,
+    k_tree, v_tree, tree_cap (device pointers as integers) and parents (list)."""
+    keep, items = [], []
+    for s in seqs:
+        par = np.ascontiguousarray(s["parents"], dtype=np.int32)
+        keep.append(par)
+        items.append({**s, "parents": par.ctypes.data, "n_nodes": par.size})
+    return Descriptors(TreeSeq, items, keep)
+
+
+def det_attention_tree_workspace(seqs: Descriptors, num_heads: int, num_kv_heads: int, head_dim: int,
+                                 window: int) -> int:
+    """Bytes of device workspace that det_attention_tree needs for these trees."""
+    n = C.c_size_t(0)
+    _check(lib().rdet_det_attention_tree_workspace(seqs.array, seqs.n, num_heads, num_kv_heads, head_dim, window,
+                                                   C.byref(n)))
+    return n.value
+
+
+def det_attention_tree(seqs: Descriptors, q_ptr: int, num_heads: int, num_kv_heads: int, head_dim: int, window: int,
+                       out_ptr: int, ws_ptr: int, ws_bytes: int, stream: int = 0):
+    """Attention of every node of a tree of drafted tokens over its sequence's
+    cache rows, its ancestors and itself (rdet_det_attention_tree)."""
+    _check(lib().rdet_det_attention_tree(seqs.array, seqs.n, q_ptr, num_heads, num_kv_heads, head_dim, window,
+                                         out_ptr, ws_ptr, ws_bytes, stream))
+
+
+def logit_rows(rows) -> Descriptors:
+    """rdet_logit_row array from dicts; every field but `logits` may be left
+    out (no rule of that kind)."""
+    base = {"repetition": 1 << 16, "parent": -1, "token": NO_TOKEN}
+    return Descriptors(LogitRow, [{**base, **r} for r in rows])
+
+
+def det_logits_rules(rows: Descriptors, vocab: int, tokens_ptr: int, stream: int = 0):
+    """Penalties, biases and the mask of allowed tokens on logits rows, and the
+    greedy token of each (rdet_det_logits_rules)."""
+    _check(lib().rdet_det_logits_rules(rows.array, rows.n, vocab, tokens_ptr, stream))
+
+
+def tree_moves(moves, paths) -> Descriptors:
+    """rdet_tree_move array from dicts of cache, draft, cap, draft_cap,
+    kv_heads, head_dim, context and path (an index into `paths`, lists of nodes)."""
+    nodes = np.ascontiguousarray([n for p in paths for n in p], dtype=np.uint32)
+    off = np.ascontiguousarray(np.cumsum([0] + [len(p) for p in paths]), dtype=np.uint32)
+    d = Descriptors(TreeMove, list(moves), (nodes, off))
+    d.nodes, d.path_off, d.n_paths = nodes.ctypes.data, off.ctypes.data, len(paths)
+    return d
+
+
+def det_tree_commit(moves: Descriptors, stream: int = 0):
+    """The drafted K/V rows of accepted paths into the caches (rdet_det_tree_commit)."""
+    _check(lib().rdet_det_tree_commit(moves.array, moves.n, moves.nodes, moves.path_off, moves.n_paths, stream))

@@ -552,6 +552,7 @@ void kernels_init() {
   attn_cluster_init();
   tc_init();
   tc_attn_init();
+  draft_ops_init();
   if ((size_t)dev >= done.size()) done.resize(dev + 1, 0);
   done[dev] = 1;
 }

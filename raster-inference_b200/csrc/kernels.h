@@ -374,7 +374,69 @@ struct TpPeerFlags {
   uint32_t* f[8] = {};
 };
 void launch_tp_signal(const TpPeerFlags& peers, int32_t world, int32_t rank, uint32_t value, cudaStream_t s);
-// vocab-sharded logits: src [world][rows][vl] -> dst[r][w * vl + j]
+// ---- verification of drafted tokens (tree_attn.cu, draft_ops.cu) --------------------
+// One launch group of the tree attention: sequences and the nodes of their
+// trees by value (kernel parameters), so a call copies nothing to the device.
+constexpr int kTreeNodes = 64;        // nodes of one tree at most (ancestor masks are 64 bits)
+constexpr int kTreeGroupSeqs = 32, kTreeGroupNodes = 512;
+struct TreeSeq {
+  const int32_t *k = nullptr, *v = nullptr;    // [Hkv, cap, d]
+  const int32_t *kt = nullptr, *vt = nullptr;  // [Hkv, tcap, d], row i = node i
+  int64_t kstride = 0, tstride = 0;            // ints from one KV head to the next: cap * d, tcap * d
+  int32_t ctx = 0, n = 0;                      // committed rows, nodes
+  int32_t node0 = 0;                           // first node within the group
+  int32_t lo = 0, len = 0;                     // keys [lo, lo + len): cache rows, then nodes (key ctx + i)
+  int32_t pad = 0;                             // row stride of the scores (len rounded up)
+  int64_t soff = 0;                            // first score of the sequence, in elements
+};
+struct TreeGroup {
+  TreeSeq seq[kTreeGroupSeqs];
+  uint64_t mask[kTreeGroupNodes];              // node's ancestors and itself, bit = node of the same tree
+  int32_t nseq = 0, nnode = 0;
+  int32_t Hq = 0, Hkv = 0, d = 0, window = 0;
+  const int32_t* q = nullptr;                  // [nnode, Hq, d]
+  int32_t* out = nullptr;
+  void* ws = nullptr;
+};
+size_t tree_attn_plan(TreeGroup& g);           // fills lo, len, pad, soff; returns workspace bytes
+void launch_tree_attn(const TreeGroup& g, cudaStream_t s);
+
+// Rules on logits rows (rdet_det_logits_rules): rows by value.
+constexpr int kRuleRows = 192;
+struct RuleRow {
+  const int32_t* logits;
+  int32_t* out;
+  const uint32_t* allow;
+  const uint32_t* history;
+  const uint32_t* bias_ids;
+  const int32_t* bias_values;
+  uint32_t history_len, n_bias;
+  int32_t repetition, frequency, presence;
+  int32_t parent;  // row of the same launch, -1: none
+  uint32_t token;
+};
+struct RuleRows {
+  RuleRow row[kRuleRows];
+};
+void launch_logit_rules(const RuleRows& r, int rows, uint32_t vocab, uint32_t* tokens, cudaStream_t s);
+
+// Accepted rows into the caches (rdet_det_tree_commit): moves by value.
+constexpr int kCommitMoves = 512, kCommitPaths = 64;
+struct CommitMove {
+  int32_t* cache;
+  const int32_t* draft;
+  uint32_t cap, draft_cap, context;
+  uint16_t head_dim, path;
+  uint32_t kv_heads;
+};
+struct CommitMoves {
+  CommitMove mv[kCommitMoves];
+  uint8_t len[kCommitPaths];
+  uint8_t node[kCommitPaths][kTreeNodes];
+};
+void launch_tree_commit(const CommitMoves& m, int moves, cudaStream_t s);
+void draft_ops_init();  // per-device kernel attributes (called by kernels_init)
+
 // ---- model ingestion: safetensors values -> Q16.16 weights (convert.cu) --------------
 enum SrcDtype : int32_t { kSrcF32 = 0, kSrcBF16 = 1, kSrcF16 = 2 };
 // out[r * row_len + k] = f32_to_wgt(src value), row_mass[r] = sum_k |out|;
@@ -383,6 +445,7 @@ enum SrcDtype : int32_t { kSrcF32 = 0, kSrcBF16 = 1, kSrcF16 = 2 };
 void launch_convert_wgt(const void* src, int dtype, uint64_t rows, uint64_t row_len, int32_t* out,
                         uint64_t* row_mass, uint32_t* stats, cudaStream_t s);
 
+// vocab-sharded logits: src [world][rows][vl] -> dst[r][w * vl + j]
 void launch_gather_vocab(const int32_t* src, int32_t world, int32_t rows, int32_t vl, int32_t* const* dst,
                          cudaStream_t s);
 // dst[r] + off <- src row r (n ints), for r < rows; cap > 0 applies the

@@ -2439,6 +2439,62 @@ static unsigned char* noalloc_scratch_current_device() {
   return static_cast<unsigned char*>(p);
 }
 
+// ---------------------------------------------------------------------------
+// Draft verification, host side of the kernel-level entry points: argument
+// checks, ancestor masks and the launch groups of the by-value descriptors.
+// ---------------------------------------------------------------------------
+constexpr uint32_t kTreeMaxRows = 1u << 24;  // attended rows of one sequence
+
+// Calls f(group) for every launch group of the trees (at most kTreeGroupSeqs
+// sequences and kTreeGroupNodes nodes each, a sequence's tree in one group).
+template <typename F>
+static void tree_groups(const rdet_tree_seq* seqs, uint32_t n_seqs, uint32_t num_heads, uint32_t num_kv_heads,
+                        uint32_t head_dim, uint32_t window, F&& f) {
+  REQUIRE(n_seqs == 0 || seqs, RDET_E_INVALID, "null argument");
+  REQUIRE(num_kv_heads > 0 && num_heads > 0 && num_heads % num_kv_heads == 0, RDET_E_INVALID,
+          "num_heads must be a multiple of num_kv_heads");
+  REQUIRE(num_heads <= 1024, RDET_E_RANGE, "at most 1024 query heads");
+  REQUIRE(head_dim > 0 && head_dim <= 512, RDET_E_RANGE, "head_dim must be in [1, 512]");
+  auto g = std::make_unique<TreeGroup>();
+  auto flush = [&] {
+    if (g->nseq == 0) return;
+    g->Hq = (int)num_heads;
+    g->Hkv = (int)num_kv_heads;
+    g->d = (int)head_dim;
+    g->window = (int)std::min<uint32_t>(window, 1u << 30);
+    f(*g);
+    g->nseq = g->nnode = 0;
+  };
+  for (uint32_t i = 0; i < n_seqs; ++i) {
+    const rdet_tree_seq& t = seqs[i];
+    REQUIRE(t.n_nodes >= 1 && t.n_nodes <= RDET_MAX_TREE_NODES, RDET_E_RANGE, "a tree has between 1 and 64 nodes");
+    REQUIRE(t.parents && t.k_tree && t.v_tree && (t.context == 0 || (t.k_cache && t.v_cache)), RDET_E_INVALID,
+            "null argument");
+    REQUIRE(t.context <= t.cap || t.context == 0, RDET_E_RANGE, "context must not exceed the cache capacity");
+    REQUIRE(t.n_nodes <= t.tree_cap, RDET_E_RANGE, "n_nodes must not exceed tree_cap");
+    REQUIRE(t.context < kTreeMaxRows, RDET_E_RANGE, "context must be below 2^24");
+    if (g->nseq == kTreeGroupSeqs || g->nnode + (int)t.n_nodes > kTreeGroupNodes) flush();
+    TreeSeq& d = g->seq[g->nseq++];
+    d.k = t.k_cache;
+    d.v = t.v_cache;
+    d.kt = t.k_tree;
+    d.vt = t.v_tree;
+    d.kstride = (int64_t)t.cap * head_dim;
+    d.tstride = (int64_t)t.tree_cap * head_dim;
+    d.ctx = (int)t.context;
+    d.n = (int)t.n_nodes;
+    d.node0 = g->nnode;
+    uint64_t* mask = g->mask + g->nnode;
+    for (uint32_t j = 0; j < t.n_nodes; ++j) {
+      const int32_t p = t.parents[j];
+      REQUIRE(p >= -1 && p < (int32_t)j, RDET_E_INVALID, "a node's parent must come before it (-1: none)");
+      mask[j] = (p >= 0 ? mask[p] : 0) | 1ull << j;
+    }
+    g->nnode += (int)t.n_nodes;
+  }
+  flush();
+}
+
 }  // namespace rdet
 
 // ===========================================================================
@@ -3337,6 +3393,136 @@ int32_t rdet_det_linear(const int32_t* x, uint32_t n_rows_x, const void* w, int3
       launch_tc_linear(ta, tw, o, s);
     } else {
       launch_linear(x, (int)n_rows_x, m, y, kEpiPlain, nullptr, s);
+    }
+    CK(cudaGetLastError());
+  });
+}
+
+int32_t rdet_det_attention_tree_workspace(const rdet_tree_seq* seqs, uint32_t n_seqs, uint32_t num_heads,
+                                          uint32_t num_kv_heads, uint32_t head_dim, uint32_t window,
+                                          size_t* bytes_out) {
+  return guard([&] {
+    REQUIRE(bytes_out, RDET_E_INVALID, "null argument");
+    size_t need = 0;
+    tree_groups(seqs, n_seqs, num_heads, num_kv_heads, head_dim, window,
+                [&](TreeGroup& g) { need = std::max(need, tree_attn_plan(g)); });
+    *bytes_out = need;
+  });
+}
+
+int32_t rdet_det_attention_tree(const rdet_tree_seq* seqs, uint32_t n_seqs, const int32_t* q, uint32_t num_heads,
+                                uint32_t num_kv_heads, uint32_t head_dim, uint32_t window, int32_t* out,
+                                void* workspace, size_t workspace_bytes, void* stream) {
+  return guard([&] {
+    REQUIRE(n_seqs == 0 || (q && out && workspace), RDET_E_INVALID, "null argument");
+    REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, RDET_E_INVALID, "workspace must be 256-byte aligned");
+    // nothing is launched unless every group can be
+    tree_groups(seqs, n_seqs, num_heads, num_kv_heads, head_dim, window, [&](TreeGroup& g) {
+      REQUIRE(tree_attn_plan(g) <= workspace_bytes, RDET_E_RANGE,
+              "workspace is smaller than rdet_det_attention_tree_workspace asks for");
+    });
+    kernels_init();
+    size_t node = 0;
+    const size_t row = (size_t)num_heads * head_dim;
+    tree_groups(seqs, n_seqs, num_heads, num_kv_heads, head_dim, window, [&](TreeGroup& g) {
+      tree_attn_plan(g);
+      g.q = q + node * row;
+      g.out = out + node * row;
+      g.ws = workspace;
+      launch_tree_attn(g, static_cast<cudaStream_t>(stream));
+      node += (size_t)g.nnode;
+    });
+    CK(cudaGetLastError());
+  });
+}
+
+int32_t rdet_det_logits_rules(const rdet_logit_row* rows, uint32_t n_rows, uint32_t vocab, uint32_t* tokens_out,
+                              void* stream) {
+  return guard([&] {
+    REQUIRE(n_rows == 0 || (rows && tokens_out), RDET_E_INVALID, "null argument");
+    REQUIRE(vocab > 0 && vocab <= (1u << 30), RDET_E_RANGE, "vocab must be in [1, 2^30]");
+    REQUIRE(n_rows <= (1u << 20), RDET_E_RANGE, "at most 2^20 rows per call");
+    // the first row of every row's tree: rows linked by `parent` go into one launch
+    std::vector<uint32_t> root(n_rows);
+    for (uint32_t i = 0; i < n_rows; ++i) {
+      const rdet_logit_row& r = rows[i];
+      REQUIRE(r.logits, RDET_E_INVALID, "null argument");
+      REQUIRE((r.history_len == 0 || r.history) && (r.n_bias == 0 || (r.bias_ids && r.bias_values)), RDET_E_INVALID,
+              "null argument");
+      REQUIRE(r.repetition > 0, RDET_E_INVALID, "the repetition penalty must be positive");
+      REQUIRE(r.parent >= -1 && (r.parent < 0 || (uint32_t)r.parent < i), RDET_E_INVALID,
+              "a row's parent must come before it (-1: none)");
+      root[i] = r.parent >= 0 ? root[r.parent] : i;
+    }
+    // a launch may start at row i when no row from i on hangs on an earlier one
+    std::vector<uint32_t> reach(n_rows + 1, n_rows);  // lowest root of the rows from i on
+    for (uint32_t i = n_rows; i-- > 0;) reach[i] = std::min(reach[i + 1], root[i]);
+    std::vector<uint32_t> cut{0};  // the launches' first rows; nothing is launched unless all can be
+    while (cut.back() < n_rows) {
+      uint32_t i1 = std::min<uint32_t>(n_rows, cut.back() + kRuleRows);
+      while (i1 < n_rows && i1 > cut.back() && reach[i1] < i1) --i1;
+      REQUIRE(i1 > cut.back(), RDET_E_RANGE, "rows linked by parent must lie within 192 consecutive rows");
+      cut.push_back(i1);
+    }
+    kernels_init();
+    auto part = std::make_unique<RuleRows>();
+    for (size_t c = 0; c + 1 < cut.size(); ++c) {
+      const uint32_t i0 = cut[c], i1 = cut[c + 1];
+      for (uint32_t i = i0; i < i1; ++i) {
+        const rdet_logit_row& r = rows[i];
+        part->row[i - i0] = RuleRow{r.logits, r.out, r.allow, r.history, r.bias_ids, r.bias_values, r.history_len,
+                                    r.n_bias, r.repetition, r.frequency, r.presence,
+                                    r.parent >= 0 ? r.parent - (int32_t)i0 : -1, r.token};
+      }
+      launch_logit_rules(*part, (int)(i1 - i0), vocab, tokens_out + i0, static_cast<cudaStream_t>(stream));
+    }
+    CK(cudaGetLastError());
+  });
+}
+
+int32_t rdet_det_tree_commit(const rdet_tree_move* moves, uint32_t n_moves, const uint32_t* nodes,
+                             const uint32_t* path_off, uint32_t n_paths, void* stream) {
+  return guard([&] {
+    REQUIRE(n_moves == 0 || (moves && path_off && n_paths > 0), RDET_E_INVALID, "null argument");
+    for (uint32_t p = 0; n_moves > 0 && p < n_paths; ++p) {
+      REQUIRE(path_off[p] <= path_off[p + 1] && path_off[p + 1] - path_off[p] <= RDET_MAX_TREE_NODES, RDET_E_RANGE,
+              "a path has at most 64 nodes");
+      REQUIRE(path_off[p] == path_off[p + 1] || nodes, RDET_E_INVALID, "null argument");
+      for (uint32_t j = path_off[p]; j < path_off[p + 1]; ++j)
+        REQUIRE(nodes[j] < RDET_MAX_TREE_NODES && (j == path_off[p] || nodes[j] > nodes[j - 1]), RDET_E_INVALID,
+                "a path's nodes must increase and be below 64");
+    }
+    for (uint32_t i = 0; i < n_moves; ++i) {
+      const rdet_tree_move& m = moves[i];
+      REQUIRE(m.cache && m.draft, RDET_E_INVALID, "null argument");
+      REQUIRE(m.path < n_paths, RDET_E_INVALID, "path out of range");
+      REQUIRE(m.kv_heads > 0 && m.kv_heads <= 1024 && m.head_dim > 0 && m.head_dim <= 1024, RDET_E_RANGE,
+              "kv_heads and head_dim must be in [1, 1024]");
+      const uint32_t len = path_off[m.path + 1] - path_off[m.path];
+      REQUIRE((uint64_t)m.context + len <= m.cap, RDET_E_RANGE, "the accepted rows would overflow the cache");
+      REQUIRE(len == 0 || nodes[path_off[m.path + 1] - 1] < m.draft_cap, RDET_E_RANGE,
+              "a path's node lies past the drafted rows");
+    }
+    auto part = std::make_unique<CommitMoves>();
+    for (uint32_t i0 = 0; i0 < n_moves;) {
+      uint32_t i = i0, paths = 0;
+      uint32_t local[kCommitPaths];  // the call's path of each path of this launch
+      for (; i < n_moves && i - i0 < (uint32_t)kCommitMoves; ++i) {
+        const rdet_tree_move& m = moves[i];
+        uint32_t p = 0;
+        while (p < paths && local[p] != m.path) ++p;
+        if (p == paths) {
+          if (paths == (uint32_t)kCommitPaths) break;
+          local[paths++] = m.path;
+          const uint32_t o = path_off[m.path];
+          part->len[p] = (uint8_t)(path_off[m.path + 1] - o);
+          for (uint32_t j = 0; j < part->len[p]; ++j) part->node[p][j] = (uint8_t)nodes[o + j];
+        }
+        part->mv[i - i0] = CommitMove{m.cache, m.draft, m.cap, m.draft_cap, m.context, (uint16_t)m.head_dim,
+                                      (uint16_t)p, m.kv_heads};
+      }
+      launch_tree_commit(*part, (int)(i - i0), static_cast<cudaStream_t>(stream));
+      i0 = i;
     }
     CK(cudaGetLastError());
   });
