@@ -552,6 +552,7 @@ void kernels_init() {
   attn_cluster_init();
   tc_init();
   tc_attn_init();
+  tree_attn_init();
   draft_ops_init();
   if ((size_t)dev >= done.size()) done.resize(dev + 1, 0);
   done[dev] = 1;
@@ -564,7 +565,8 @@ int stream_error_flag(bool reset) {
     int z = 0;
     cudaMemcpyToSymbol(g_stream_err, &z, sizeof(int));
   }
-  return v | tc_error_flag(reset) | tc_attn_error_flag(reset) | tc_attn_dec_error_flag(reset);
+  return v | tc_error_flag(reset) | tc_attn_error_flag(reset) | tc_attn_dec_error_flag(reset) |
+         tree_attn_error_flag(reset);
 }
 
 // Plans and launches the streamed GEMV; returns false when the launch does not

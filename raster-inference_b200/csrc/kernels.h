@@ -386,8 +386,11 @@ struct TreeSeq {
   int32_t ctx = 0, n = 0;                      // committed rows, nodes
   int32_t node0 = 0;                           // first node within the group
   int32_t lo = 0, len = 0;                     // keys [lo, lo + len): cache rows, then nodes (key ctx + i)
-  int32_t pad = 0;                             // row stride of the scores (len rounded up)
+  int32_t pad = 0;                             // row stride of the scores: len rounded up to 64
+  int32_t splits = 1;                          // value items over the keys
+  int32_t blk0 = 0;                            // first (KV head, row block) of the sequence
   int64_t soff = 0;                            // first score of the sequence, in elements
+  int64_t woff = 0;                            // its weight digits, in bytes from the workspace
 };
 struct TreeGroup {
   TreeSeq seq[kTreeGroupSeqs];
@@ -397,9 +400,16 @@ struct TreeGroup {
   const int32_t* q = nullptr;                  // [nnode, Hq, d]
   int32_t* out = nullptr;
   void* ws = nullptr;
+  // filled by tree_attn_plan: rows per block, items and rows of the
+  // sequences before each one, key tiles per score item, workspace sections
+  int32_t nr = 0, qk_tiles = 1, qk_items = 0, pv_items = 0, rows = 0;
+  int32_t qk_first[kTreeGroupSeqs], pv_first[kTreeGroupSeqs], row_first[kTreeGroupSeqs];
+  int64_t acc_off = 0, cnt_off = 0;
 };
-size_t tree_attn_plan(TreeGroup& g);           // fills lo, len, pad, soff; returns workspace bytes
+size_t tree_attn_plan(TreeGroup& g);           // returns the workspace bytes
 void launch_tree_attn(const TreeGroup& g, cudaStream_t s);
+void tree_attn_init();                         // per-device kernel attributes (called by kernels_init)
+int tree_attn_error_flag(bool reset);          // nonzero when one of its pipeline waits gave up
 
 // Rules on logits rows (rdet_det_logits_rules): rows by value.
 constexpr int kRuleRows = 192;
