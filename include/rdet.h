@@ -255,8 +255,8 @@ typedef struct rdet_tree_seq {
  * positions >= p + 1 - window and to itself (window 0: no limit): the result is
  * attention_output_into (det_kernels.rs:340-367) over those rows, bit for bit
  * what rdet_det_attention_decode gives when the ancestors are committed.
- * num_heads a multiple of num_kv_heads, 1 <= head_dim <= 512; context, and the
- * attended rows, below 2^24.  workspace: at least
+ * num_heads a multiple of num_kv_heads, 1 <= head_dim <= 512; context below 2^24,
+ * at most 523264 attended rows (context within the window and nodes).  workspace: at least
  * rdet_det_attention_tree_workspace bytes, 256-byte aligned. */
 int32_t rdet_det_attention_tree_workspace(const rdet_tree_seq* seqs, uint32_t n_seqs, uint32_t num_heads,
                                           uint32_t num_kv_heads, uint32_t head_dim, uint32_t window,

@@ -274,6 +274,52 @@ RDET_HD int32_t softmax_weight(int64_t e, int64_t sum) {
   return requantize((int64_t)q);
 }
 
+// a * b / 2^32 for a, b < 2^32, ties to even (acc_mul_u32 with the rounding as
+// one carry: half less one, plus one when the quotient is odd)
+RDET_HD uint32_t acc_mul_rte(uint32_t a, uint32_t b) {
+  const uint64_t p = (uint64_t)a * b;
+  return (uint32_t)((p + 0x7fffffffull + ((p >> 32) & 1)) >> 32);
+}
+// v / d for a constant even d, ties to even: up iff 2 r + (q odd) > d
+RDET_HD uint32_t div_rte(uint32_t v, uint32_t d) {
+  const uint32_t q = v / d, r = v - q * d;
+  return q + (2 * r + (q & 1) > d ? 1u : 0u);
+}
+// exp_term(max - D, max) for 0 <= D < 16 * 2^16 in 32-bit pieces.  The number
+// of halvings floor(D 2^16 / ln2) is one multiply by 2^62 / ln2 rounded down
+// (the host test compares every D with exp_term).
+RDET_HD uint64_t exp_term_below(uint32_t D) {
+  const uint32_t LN2 = 2977044472u;
+  uint32_t shift = (uint32_t)(((uint64_t)D * 1549082004u) >> 46);  // <= 23
+  uint32_t r = (D << 16) - shift * LN2;                             // exact mod 2^32, below ln2
+  const uint32_t r2 = acc_mul_rte(r, r), r3 = acc_mul_rte(r2, r), r4 = acc_mul_rte(r3, r), r5 = acc_mul_rte(r4, r);
+  // the terms after 1 - r sum to a value in [0, 2^31): one 32-bit sum
+  const uint32_t tail = ((r2 >> 1) + (r2 & (r2 >> 1) & 1)) - div_rte(r3, 6) + div_rte(r4, 24) - div_rte(r5, 120);
+  const uint64_t e = kOneAcc - (uint64_t)r + tail;  // > 0: at least 2^32 (1 - ln2)
+  if (shift == 0) return e;
+  const uint64_t half = (1ull << (shift - 1)) - 1 + ((e >> shift) & 1);
+  return (e + half) >> shift;
+}
+
+// Softmax weights against one sum without a division each.  inv is 2^64 / sum
+// (sum >= 2^32) cut to 32 bits, off by at most 2 with the rounding of the
+// double quotient.  e * inv is then e 2^64 / sum within 3 * 2^32 (e is below
+// 2^32, or 2^32 coded 2^32 - 1), so e * inv / 2^48 is the weight in Q16.16
+// within 3 * 2^-16; cutting the product to its high word costs 2^-16 more, and
+// the reference's first rounding (to 2^-32) moves the weight by at most 2^-17.
+// Where that is nearer than 6 * 2^-16 to a half, the exact division decides.
+RDET_HD uint32_t softmax_inverse(uint64_t sum) {
+  const double q = 18446744073709551616.0 / (double)sum;
+  return q >= 4294967295.0 ? 0xffffffffu : (uint32_t)q;
+}
+RDET_HD int32_t softmax_weight_coded(uint32_t e, uint32_t inv, uint64_t sum) {
+  const uint32_t hi = (uint32_t)(((uint64_t)e * inv) >> 32);
+  // near a half, or near 2^16 (where the rounding add would wrap)
+  if (((hi + 0x8006u) & 0xffffu) < 12 || hi > 0xffff7ff0u)
+    return softmax_weight(e == 0xffffffffu ? kOneAcc : (int64_t)e, (int64_t)sum);
+  return (int32_t)((hi + 0x8000u) >> 16);
+}
+
 // ops.rs:354 tanh_act
 RDET_HD int32_t tanh_act(int32_t x) {
   if (x >= (3 << 16)) return kOneAct;

@@ -378,6 +378,7 @@ void launch_tp_signal(const TpPeerFlags& peers, int32_t world, int32_t rank, uin
 // One launch group of the tree attention: sequences and the nodes of their
 // trees by value (kernel parameters), so a call copies nothing to the device.
 constexpr int kTreeNodes = 64;        // nodes of one tree at most (ancestor masks are 64 bits)
+constexpr int kTreeMaxKeys = 16 * 32704;  // attended rows of one sequence: 16 value CTAs' s32 accumulators
 constexpr int kTreeGroupSeqs = 32, kTreeGroupNodes = 512;
 struct TreeSeq {
   const int32_t *k = nullptr, *v = nullptr;    // [Hkv, cap, d]
@@ -387,8 +388,7 @@ struct TreeSeq {
   int32_t node0 = 0;                           // first node within the group
   int32_t lo = 0, len = 0;                     // keys [lo, lo + len): cache rows, then nodes (key ctx + i)
   int32_t pad = 0;                             // row stride of the scores: len rounded up to 64
-  int32_t splits = 1;                          // value items over the keys
-  int32_t blk0 = 0;                            // first (KV head, row block) of the sequence
+  int32_t qk_per = 1;                          // score items of one row block
   int64_t soff = 0;                            // first score of the sequence, in elements
   int64_t woff = 0;                            // its weight digits, in bytes from the workspace
 };
@@ -400,11 +400,10 @@ struct TreeGroup {
   const int32_t* q = nullptr;                  // [nnode, Hq, d]
   int32_t* out = nullptr;
   void* ws = nullptr;
-  // filled by tree_attn_plan: rows per block, items and rows of the
-  // sequences before each one, key tiles per score item, workspace sections
-  int32_t nr = 0, qk_tiles = 1, qk_items = 0, pv_items = 0, rows = 0;
+  // filled by tree_attn_plan: heads per KV head, rows per block, key tiles per score item, CTAs
+  // per value item, items and rows of the sequences before each one
+  int32_t G = 1, nr = 0, qk_tiles = 1, splits = 1, qk_items = 0, pv_items = 0, rows = 0;
   int32_t qk_first[kTreeGroupSeqs], pv_first[kTreeGroupSeqs], row_first[kTreeGroupSeqs];
-  int64_t acc_off = 0, cnt_off = 0;
 };
 size_t tree_attn_plan(TreeGroup& g);           // returns the workspace bytes
 void launch_tree_attn(const TreeGroup& g, cudaStream_t s);

@@ -2443,7 +2443,6 @@ static unsigned char* noalloc_scratch_current_device() {
 // Draft verification, host side of the kernel-level entry points: argument
 // checks, ancestor masks and the launch groups of the by-value descriptors.
 // ---------------------------------------------------------------------------
-constexpr uint32_t kTreeMaxRows = 1u << 24;  // attended rows of one sequence
 
 // Calls f(group) for every launch group of the trees (at most kTreeGroupSeqs
 // sequences and kTreeGroupNodes nodes each, a sequence's tree in one group).
@@ -2472,7 +2471,9 @@ static void tree_groups(const rdet_tree_seq* seqs, uint32_t n_seqs, uint32_t num
             "null argument");
     REQUIRE(t.context <= t.cap || t.context == 0, RDET_E_RANGE, "context must not exceed the cache capacity");
     REQUIRE(t.n_nodes <= t.tree_cap, RDET_E_RANGE, "n_nodes must not exceed tree_cap");
-    REQUIRE(t.context < kTreeMaxRows, RDET_E_RANGE, "context must be below 2^24");
+    REQUIRE(t.context < (1u << 24), RDET_E_RANGE, "context must be below 2^24");
+    const uint32_t rows = (window > 0 ? std::min(t.context, window) : t.context) + t.n_nodes;
+    REQUIRE(rows <= (uint32_t)kTreeMaxKeys, RDET_E_RANGE, "a sequence attends at most 523264 rows");
     if (g->nseq == kTreeGroupSeqs || g->nnode + (int)t.n_nodes > kTreeGroupNodes) flush();
     TreeSeq& d = g->seq[g->nseq++];
     d.k = t.k_cache;

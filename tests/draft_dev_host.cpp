@@ -1,0 +1,75 @@
+// Host build of the softmax helpers of the tree attention (det_dev.cuh),
+// compared here with the general forms; each returns the number of differences.
+#include <cstdint>
+
+#include "det_dev.cuh"
+
+using namespace rdet;
+
+static uint64_t mix(uint64_t z) {
+  z += 0x9E3779B97F4A7C15ull;
+  z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+  z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+  return z ^ (z >> 31);
+}
+
+extern "C" {
+// every distance below the maximum that has a term
+int64_t exp_all(int32_t max_logit) {
+  int64_t bad = 0;
+  for (uint32_t D = 0; D < (16u << 16); ++D)
+    if ((int64_t)max_logit - D >= INT32_MIN)
+      bad += (int64_t)exp_term_below(D) != exp_term((int32_t)((int64_t)max_logit - D), max_logit);
+  return bad;
+}
+// the largest term below 2^32: the code 2^32 - 1 stands for 2^32 alone
+uint64_t exp_second() { return exp_term_below(1); }
+
+static int64_t one(uint64_t e, uint64_t sum) {
+  const uint32_t coded = e >> 32 ? 0xffffffffu : (uint32_t)e;
+  return softmax_weight_coded(coded, softmax_inverse(sum), sum) != softmax_weight((int64_t)e, (int64_t)sum);
+}
+// random sums and terms
+int64_t weights_random(uint64_t seed, int64_t n) {
+  int64_t bad = 0;
+  for (int64_t i = 0; i < n; ++i) {
+    const uint64_t a = mix(seed + 2 * i), b = mix(seed + 2 * i + 1);
+    const uint64_t sum = (1ull << 32) + (a >> (8 + a % 56)) % (1ull << 50);
+    const uint64_t e = b % 3 == 0 ? (1ull << 32) : (b >> (32 + b % 31));
+    bad += one(e, sum);
+  }
+  return bad;
+}
+// terms whose weight lies at k + 1/2, and their neighbours, for sums of every size
+int64_t weights_ties(uint64_t seed, int64_t n) {
+  int64_t bad = 0;
+  for (int64_t i = 0; i < n; ++i) {
+    const uint64_t a = mix(seed + i);
+    const uint64_t sum = (1ull << 32) + (a >> 8) % (1ull << (1 + a % 49));
+    const uint64_t k = mix(a) % 65536;
+    // e 2^16 / sum = k + 1/2  ->  e = (2 k + 1) sum / 2^17
+    const unsigned __int128 p = (unsigned __int128)(2 * k + 1) * sum;
+    const uint64_t e0 = (uint64_t)(p >> 17);
+    for (int64_t d = -3; d <= 4; ++d) {
+      const uint64_t e = e0 + d;
+      // terms are at most 2^32 - 2^15, or 2^32
+      if ((int64_t)e >= 0 && e <= (1ull << 32) - (1ull << 15) && e <= sum) bad += one(e, sum);
+    }
+    // quotients at k + 1/2 exactly: sum a multiple of 2^17
+    const uint64_t s2 = (sum >> 17 << 17) + (1ull << 32), e2 = (2 * k + 1) * (s2 >> 17);
+    for (int64_t d = -2; d <= 2; ++d)
+      if (e2 + d <= (1ull << 32) - (1ull << 15)) bad += one(e2 + d, s2);
+  }
+  return bad;
+}
+// a term equal or almost equal to the sum
+int64_t weights_one(int64_t n) {
+  int64_t bad = 0;
+  for (int64_t i = 0; i < n; ++i) {
+    bad += one(1ull << 32, (1ull << 32) + i);
+    bad += one(1ull << 32, (1ull << 32) + i * 257);
+    bad += one((1ull << 32) - (1ull << 15) - i, (1ull << 32));
+  }
+  return bad;
+}
+}

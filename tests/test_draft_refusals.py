@@ -21,7 +21,7 @@ def tree(s, heads=4, kv=2, d=16, window=0, q=A, out=A, ws=A, ws_bytes=1 << 40, n
 @pytest.mark.parametrize("over,code", [
     (dict(parents=[]), -6), (dict(parents=[-1] * 65, tree_cap=65), -6), (dict(parents=[-1, 1]), -1),
     (dict(parents=[-2]), -1), (dict(context=65), -6), (dict(tree_cap=2), -6), (dict(k_tree=0), -1),
-    (dict(v_cache=0), -1), (dict(context=1 << 24, cap=1 << 25), -6)])
+    (dict(v_cache=0), -1), (dict(context=1 << 24, cap=1 << 25), -6), (dict(context=523262, cap=1 << 20), -6)])
 def test_tree_refuses_sequences(over, code):
     with pytest.raises(rdet.RdetError) as e:
         tree(seq(**over))

@@ -404,3 +404,29 @@ def test_tree_commit_many_moves():
     rdet.det_tree_commit(rdet.tree_moves(moves, paths))
     torch.cuda.synchronize()
     assert np.array_equal(ad.cpu().numpy(), a)
+
+
+def test_tree_attention_many_tiles_back_to_back():
+    # many key tiles per block and calls that overlap at their ends: a block
+    # whose warps drift apart must not miss a barrier's phase (it would wait
+    # out its bound of a second)
+    import time
+    n, ctx, d = 64, 12000, 64
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(1)
+    k = (torch.randn((8, ctx + n, d), generator=gen, device="cuda") * 65536).to(torch.int32)
+    q = (torch.randn((n, 32, d), generator=gen, device="cuda") * 9000).to(torch.int32)
+    s = rdet.tree_seqs([dict(k_cache=k.data_ptr(), v_cache=k.data_ptr(), cap=ctx + n, context=ctx,
+                             k_tree=k.data_ptr() + ctx * d * 4, v_tree=k.data_ptr() + ctx * d * 4, tree_cap=ctx + n,
+                             parents=[i - 1 for i in range(n)])])
+    need = rdet.det_attention_tree_workspace(s, 32, 8, d, 0)
+    ws = torch.zeros(need, dtype=torch.uint8, device="cuda")
+    outs = [torch.zeros((n, 32, d), dtype=torch.int32, device="cuda") for _ in range(2)]
+    rdet.det_attention_tree(s, q.data_ptr(), 32, 8, d, 0, outs[0].data_ptr(), ws.data_ptr(), need)
+    torch.cuda.synchronize()
+    t = time.monotonic()
+    for _ in range(150):
+        rdet.det_attention_tree(s, q.data_ptr(), 32, 8, d, 0, outs[1].data_ptr(), ws.data_ptr(), need)
+    torch.cuda.synchronize()
+    assert time.monotonic() - t < 0.9
+    assert torch.equal(outs[0], outs[1])
