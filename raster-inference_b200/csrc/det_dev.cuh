@@ -307,17 +307,16 @@ RDET_HD uint64_t exp_term_below(uint32_t D) {
 // 2^32, or 2^32 coded 2^32 - 1), so e * inv / 2^48 is the weight in Q16.16
 // within 3 * 2^-16; cutting the product to its high word costs 2^-16 more, and
 // the reference's first rounding (to 2^-32) moves the weight by at most 2^-17.
-// Where that is nearer than 6 * 2^-16 to a half, the exact division decides.
+// False where that is nearer than 6 * 2^-16 to a half: the exact division decides.
 RDET_HD uint32_t softmax_inverse(uint64_t sum) {
   const double q = 18446744073709551616.0 / (double)sum;
   return q >= 4294967295.0 ? 0xffffffffu : (uint32_t)q;
 }
-RDET_HD int32_t softmax_weight_coded(uint32_t e, uint32_t inv, uint64_t sum) {
+RDET_HD bool softmax_weight_near(uint32_t e, uint32_t inv, int32_t* w) {
   const uint32_t hi = (uint32_t)(((uint64_t)e * inv) >> 32);
-  // near a half, or near 2^16 (where the rounding add would wrap)
-  if (((hi + 0x8006u) & 0xffffu) < 12 || hi > 0xffff7ff0u)
-    return softmax_weight(e == 0xffffffffu ? kOneAcc : (int64_t)e, (int64_t)sum);
-  return (int32_t)((hi + 0x8000u) >> 16);
+  *w = (int32_t)((hi + 0x8000u) >> 16);
+  // not near a half, nor near 2^16 (where the rounding add would wrap)
+  return ((hi + 0x8006u) & 0xffffu) >= 12 && hi <= 0xffff7ff0u;
 }
 
 // ops.rs:354 tanh_act

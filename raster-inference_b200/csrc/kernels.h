@@ -378,7 +378,7 @@ void launch_tp_signal(const TpPeerFlags& peers, int32_t world, int32_t rank, uin
 // One launch group of the tree attention: sequences and the nodes of their
 // trees by value (kernel parameters), so a call copies nothing to the device.
 constexpr int kTreeNodes = 64;        // nodes of one tree at most (ancestor masks are 64 bits)
-constexpr int kTreeMaxKeys = 16 * 32704;  // attended rows of one sequence: 16 value CTAs' s32 accumulators
+constexpr int kTreeMaxKeys = 16 * 32704;  // attended rows of one sequence: at most 32 value CTAs' s32 accumulators
 constexpr int kTreeGroupSeqs = 32, kTreeGroupNodes = 512;
 struct TreeSeq {
   const int32_t *k = nullptr, *v = nullptr;    // [Hkv, cap, d]
@@ -388,9 +388,10 @@ struct TreeSeq {
   int32_t node0 = 0;                           // first node within the group
   int32_t lo = 0, len = 0;                     // keys [lo, lo + len): cache rows, then nodes (key ctx + i)
   int32_t pad = 0;                             // row stride of the scores: len rounded up to 64
-  int32_t qk_per = 1;                          // score items of one row block
+  int32_t qk_per = 1;                          // score CTAs of one row block
+  int32_t splits = 1, cfirst = 0;              // value CTAs of one item; its first item
   int64_t soff = 0;                            // first score of the sequence, in elements
-  int64_t woff = 0;                            // its weight digits, in bytes from the workspace
+  int64_t moff = 0;                            // its rows' first partial maximum, qk_per a row
 };
 struct TreeGroup {
   TreeSeq seq[kTreeGroupSeqs];
@@ -400,10 +401,14 @@ struct TreeGroup {
   const int32_t* q = nullptr;                  // [nnode, Hq, d]
   int32_t* out = nullptr;
   void* ws = nullptr;
-  // filled by tree_attn_plan: heads per KV head, rows per block, key tiles per score item, CTAs
-  // per value item, items and rows of the sequences before each one
-  int32_t G = 1, nr = 0, qk_tiles = 1, splits = 1, qk_items = 0, pv_items = 0, rows = 0;
+  // filled by tree_attn_plan: heads per KV head, rows per block, key tiles
+  // per score CTA, keys per term CTA and CTAs per row, CTAs and rows of the
+  // sequences before each one, workspace sections (in
+  // bytes, after the scores): partial maxima, partial sums, first maxima,
+  // value sums, weight sums and arrivals per value item
+  int32_t G = 1, nr = 0, qk_tiles = 1, ex_keys = 0, ex_chunks = 1, qk_items = 0, pv_items = 0, rows = 0;
   int32_t qk_first[kTreeGroupSeqs], pv_first[kTreeGroupSeqs], row_first[kTreeGroupSeqs];
+  int64_t max_off = 0, sum_off = 0, idx_off = 0, acc_off = 0, wt_off = 0, cnt_off = 0;
 };
 size_t tree_attn_plan(TreeGroup& g);           // returns the workspace bytes
 void launch_tree_attn(const TreeGroup& g, cudaStream_t s);

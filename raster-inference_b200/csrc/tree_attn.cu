@@ -9,34 +9,38 @@
 //   out[i] = requantize(sum_j w[j] v[j][i])            (wrapping i64)
 //
 // A weight is rounded against the row's complete maximum and sum, so no
-// running softmax is exact: the scores of all keys come before the first
-// weight.  Three kernels over a scratch, coupled by programmatic dependent
-// launch: scores and weighted values on the tensor cores, the softmax on the
-// CUDA cores between them.  A key is an index into the sequence's
-// [lo, lo + len): cache rows lo .. ctx - 1, then the nodes (key ctx + i).  The
-// order of keys is the order of positions along every node's path, because
-// parents come before their children.
+// running softmax is exact: the scores of all keys come before the first exp
+// term, and all terms before the first weight.  Three kernels over a scratch,
+// coupled by programmatic dependent launch: scores with each block's row
+// maxima (tensor cores), exp terms with partial sums (CUDA cores), weights and
+// weighted values (tensor cores).  The residual 1 - sum w is a term of its
+// own, added with the first maximum's value where the sums are rounded.  A key
+// is an index into the sequence's [lo, lo + len): cache rows lo .. ctx - 1,
+// then the nodes (key ctx + i).  The order of keys is the order of positions
+// along every node's path, because parents come before their children.
 //
-// Digits.  x = sum_b 256^b x_b with x_b in [-128, 127] (balanced base-256
-// digits) holds for every i32 up to 0x7f7f7f7f: the digits are the bytes of
-// (x + 0x80808080) ^ 0x80808080.  Then sum x y = sum_{a,b} 256^(a+b) sum x_b
-// y_a, signed int8 products that need no offset corrections, and digits that
-// are zero throughout (activations after a norm rarely reach 2^23) cost
-// nothing.  A tile that holds a larger value takes the direct wrapping i64
-// sums instead.
+// Digits.  The tensor cores multiply signed bytes.  Queries and weights are
+// split into balanced base-256 digits, x = sum_a 256^a x_a with x_a in
+// [-128, 127]: the bytes of (x + 0x80808080) ^ 0x80808080, for every i32 up to
+// 0x7f7f7f7f (a block with a larger query value takes the direct wrapping i64
+// sums).  Keys and values, of which there are far more, take the cheapest
+// split: their bytes as they are, the three lower ones with the top bit
+// flipped, so that k = sum_b 256^b k_b + 0x808080 for every i32.  Then
+//   sum_i q k = sum_{a,b} 256^(a+b) sum_i q_a k_b + 0x808080 sum_i q
+//   sum_j w v = sum_{a,b} 256^(a+b) sum_j w_a v_b + 0x808080 sum_j w,
+// each correction one number a query row.
 //
 // Scores.  The keys of a 128-key tile are the MMA's M rows, one operand A per
-// key digit b; operand B stacks the digits of NR query rows (rows a * NR + r).
-// The MMA of key digit b accumulates at TMEM column b * NR, so column block g
+// key byte b; operand B stacks the digits of NR query rows (rows a * NR + r).
+// The MMA of key byte b accumulates at TMEM column b * NR, so column block g
 // (columns [g NR, (g + 1) NR)) sums exactly the products of shift 8 g: seven
 // blocks, each at most 4 * 2^14 * 512 = 2^25 in magnitude, exact in s32.
 // A query row is a (node, head of the KV head's group); all of them read a
 // key tile at once, so the cache streams once per NR rows.
 //
 // Weighted values.  M rows are 128 dims of the transposed value tile, B the
-// three digits of the weights (a weight lies in [-2^23, 2^16]): six column
+// three digits of the weights (a weight lies in [0, 2^16]): six column
 // blocks, each at most 3 * 2^14 per key, exact in s32 up to 2^15 keys.
-#include <cooperative_groups.h>
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -54,7 +58,6 @@ __device__ int g_tree_err = 0;
 
 namespace {
 
-namespace cg = cooperative_groups;
 using namespace tcx;
 
 constexpr int kTrKeys = 128;           // keys of a score tile (MMA M)
@@ -63,6 +66,7 @@ constexpr int kTrPlanes = 4 * kTrPlane;
 constexpr int kTrConv = 512;           // converter threads (warps 0-15)
 constexpr int kTrConvWarps = kTrConv / 32;
 constexpr int kQkThreads = 672;        // + warps 16-19 drain the accumulators, warp 20 issues the MMAs
+constexpr int kQkDrainWarps = 20;      // warps 0-19
 constexpr int kPvThreads = 544;        // + warp 16 issues the MMAs
 constexpr int kTrMaxDigit = 0x7f7f7f7f;
 constexpr int kTrSplitKeys = 32704;    // keys of one value CTA at most: 3 * 2^14 each in s32
@@ -115,7 +119,7 @@ __device__ __forceinline__ bool ta_mbar_wait(uint64_t* b, uint32_t parity) {
 // 2^18, so the address field does not carry)
 __device__ __forceinline__ uint64_t ta_adv(uint64_t desc, int bytes) { return desc + (uint64_t)(bytes >> 4); }
 
-// digits of x as four signed bytes
+// balanced digits of x as four signed bytes
 __device__ __forceinline__ uint32_t ta_digits(int32_t x) { return ((uint32_t)x + 0x80808080u) ^ 0x80808080u; }
 // 4 x 4 byte transpose: o[b] = byte b of w0..w3 (w0 in the low byte)
 __device__ __forceinline__ void ta_t4(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, uint32_t (&o)[4]) {
@@ -168,52 +172,152 @@ __device__ __forceinline__ int seq_of(const int32_t* first, int nseq, int it) {
   return 31 - __clz((int)m);
 }
 
-// four dims from `dim` on of a row (zero past the head): 16-byte loads where
-// every row is 16-byte aligned, else one value at a time
+// Loads into registers that keep their values where `on` is false.  Written
+// as predicated instructions: a load under a branch or a select makes the
+// compiler wait for it where the paths meet, which costs the prefetch its
+// point (a stage took a memory latency longer).  Not .nc: a grid may be
+// resident already while the grid before it writes what it reads.
+__device__ __forceinline__ void ld16(uint4& v, const void* p, bool on) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %5, 0;\n @p ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n}"
+      : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
+      : "l"(p), "r"((int)on));
+}
+__device__ __forceinline__ void ld4(uint32_t& v, const void* p, bool on) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %2, 0;\n @p ld.global.L1::no_allocate.u32 %0, [%1];\n}"
+               : "+r"(v)
+               : "l"(p), "r"((int)on));
+}
+// four dims from `dim` on of a row of d: 16 bytes where every row is 16-byte
+// aligned, else one value at a time; what lies past the head is left alone
 template <bool VEC>
-__device__ __forceinline__ uint4 load4(const int32_t* row, int dim, int d) {
-  if (VEC) return dim < d ? __ldg(reinterpret_cast<const uint4*>(row + dim)) : make_uint4(0, 0, 0, 0);
-  uint4 v = make_uint4(0, 0, 0, 0);
-  if (dim < d) v.x = (uint32_t)row[dim];
-  if (dim + 1 < d) v.y = (uint32_t)row[dim + 1];
-  if (dim + 2 < d) v.z = (uint32_t)row[dim + 2];
-  if (dim + 3 < d) v.w = (uint32_t)row[dim + 3];
-  return v;
+__device__ __forceinline__ void load4(uint4& v, const int32_t* row, int dim, int d, bool on) {
+  if (VEC) {
+    ld16(v, row + dim, on && dim < d);
+  } else {
+    ld4(v.x, row + dim, on && dim < d);
+    ld4(v.y, row + dim + 1, on && dim + 1 < d);
+    ld4(v.z, row + dim + 2, on && dim + 2 < d);
+    ld4(v.w, row + dim + 3, on && dim + 3 < d);
+  }
 }
 __device__ __forceinline__ int32_t max4(int32_t m, const uint4& v) {
   return max(max(max(m, (int32_t)v.x), max((int32_t)v.y, (int32_t)v.z)), (int32_t)v.w);
 }
 
-// sum of seven column blocks: sum_g 256^g c[g], wrapping
-__device__ __forceinline__ int64_t shift_sum(const int32_t (&c)[7]) {
-  const int64_t p0 = mac_wide(c[0], c[1], 256), p1 = mac_wide(c[2], c[3], 256), p2 = mac_wide(c[4], c[5], 256);
-  return (int64_t)((uint64_t)p0 + ((uint64_t)p1 << 16) + ((uint64_t)p2 << 32) + ((uint64_t)(int64_t)c[6] << 48));
+// the bytes of four keys' or values' words as four operand words
+__device__ __forceinline__ void ta_bytes(uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3, uint32_t (&o)[4]) {
+  ta_t4(w0, w1, w2, w3, o);
+  o[0] ^= 0x80808080u;
+  o[1] ^= 0x80808080u;
+  o[2] ^= 0x80808080u;
+}
+constexpr int64_t kTrBias = 0x808080;
+
+// the rare weights that the reciprocal leaves open, out of line
+__device__ __noinline__ int32_t ta_weight_exact(uint32_t e, uint64_t sum) {
+  return softmax_weight(e == 0xffffffffu ? kOneAcc : (int64_t)e, (int64_t)sum);
+}
+__device__ __forceinline__ int32_t ta_weight(uint32_t e, uint32_t inv, uint64_t sum) {
+  int32_t w;
+  return softmax_weight_near(e, inv, &w) ? w : ta_weight_exact(e, sum);
+}
+
+// add + sum over g of 256^g c_g, wrapping: widening multiply-adds below 2^32,
+// the rest in the high word
+__device__ __forceinline__ int64_t shift_sum(int64_t add, int32_t c0, int32_t c1, int32_t c2, int32_t c3, int32_t c4,
+                                             int32_t c5, int32_t c6) {
+  int64_t v = mac_wide(add, c0, 1);
+  v = mac_wide(v, c1, 1 << 8);
+  v = mac_wide(v, c2, 1 << 16);
+  v = mac_wide(v, c3, 1 << 24);
+  const uint32_t hi = (uint32_t)((uint64_t)v >> 32) + (uint32_t)c4 + ((uint32_t)c5 << 8) + ((uint32_t)c6 << 16);
+  return (int64_t)((uint64_t)hi << 32 | (uint32_t)v);
 }
 
 // ---------------------------------------------------------------------------
 // scores
 // ---------------------------------------------------------------------------
+// plane buffers between the converters and the MMAs
 template <int NR>
-__host__ __device__ constexpr int qk_smem(int ns) { return 2 * kTrPlanes + ns * 4 * NR * 64 + 1024; }
+__host__ __device__ constexpr int qk_stages() { return NR == 64 ? 3 : 4; }
+template <int NR>
+__host__ __device__ constexpr int qk_smem(int ns) { return qk_stages<NR>() * kTrPlanes + ns * 4 * NR * 64 + 1024; }
+
+// what draining a tile needs, per row of the block
+template <int NR>
+struct QkRows {
+  int64_t corr[NR];        // 0x808080 times the sum of the query row
+  uint64_t mask[NR];       // the node's ancestors and itself
+  int32_t start[NR];       // the first position it attends
+  uint32_t top[NR];        // its largest score so far, order-preserving as u32
+  int32_t npos[kTreeNodes];  // positions of the tree's nodes
+  int32_t* sc;             // scores of the block's row 0
+  int32_t pad, nr, ctx, lo, len, maxstart;
+};
+// Scores of the row quads quad, quad + step, .. of a tile from TMEM (this
+// lane's key is j, the tile's first one j0), and each row's largest one.
+template <int NR>
+__device__ __noinline__ void qk_drain(QkRows<NR>& c, uint32_t taddr, int j0, int quad, int step) {
+  const int lane = threadIdx.x & 31, j = j0 + 32 * ((threadIdx.x >> 5) & 3) + lane, key = c.lo + j;
+  const bool in = j < c.len, all = c.lo + j0 >= c.maxstart && c.lo + j0 + kTrKeys <= c.ctx;  // every row attends every key
+  int32_t* out = c.sc + (int64_t)(4 * quad) * c.pad + j;
+  for (int r = 4 * quad; r < c.nr; r += 4 * step, out += 4 * (int64_t)step * c.pad) {
+    int32_t v[7][4];
+#pragma unroll
+    for (int b = 0; b < 7; ++b) ta_ld4(taddr + b * NR + r, v[b]);
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int32_t s = requantize(shift_sum(c.corr[r + i], v[0][i], v[1][i], v[2][i], v[3][i], v[4][i], v[5][i], v[6][i]));
+      bool vis = in && r + i < c.nr;
+      if (vis) out[(int64_t)i * c.pad] = s;
+      if (!all) {
+        const int n = key - c.ctx;
+        vis = vis && (n < 0 ? key >= c.start[r + i] : (c.mask[r + i] >> n & 1) && c.npos[n] >= c.start[r + i]);
+      }
+      const uint32_t top = __reduce_max_sync(0xffffffffu, vis ? (uint32_t)s ^ 0x80000000u : 0u);
+      if (lane == 0) atomicMax(&c.top[r + i], top);
+    }
+  }
+}
+// The same by direct wrapping sums, for a block with a query value outside
+// the digits' range.
+template <int NR>
+__device__ __noinline__ void qk_drain_direct(QkRows<NR>& c, const int32_t* k, const int32_t* qb, int r0, int G, int Hq,
+                                             int d, int j0, int quad, int step) {
+  const int lane = threadIdx.x & 31, j = j0 + 32 * ((threadIdx.x >> 5) & 3) + lane, key = c.lo + j;
+  for (int r4 = 4 * quad; r4 < c.nr; r4 += 4 * step)
+    for (int r = r4; r < min(c.nr, r4 + 4); ++r) {
+      const int node = (r0 + r) / G;
+      const int32_t* q = qb + ((int64_t)node * Hq + (r0 + r - node * G)) * d;
+      int64_t acc = 0;
+      bool vis = j < c.len;
+      if (vis) {
+        for (int e = 0; e < d; ++e) acc = mac_wide(acc, q[e], k[e]);
+        c.sc[(int64_t)r * c.pad + j] = requantize(acc);
+        const int n = key - c.ctx;
+        vis = n < 0 ? key >= c.start[r] : (c.mask[r] >> n & 1) && c.npos[n] >= c.start[r];
+      }
+      const uint32_t top = __reduce_max_sync(0xffffffffu, vis ? (uint32_t)requantize(acc) ^ 0x80000000u : 0u);
+      if (lane == 0) atomicMax(&c.top[r], top);
+    }
+}
 
 template <int NR, bool VEC>
 __global__ void __launch_bounds__(kQkThreads, 1) tree_qk(const __grid_constant__ TreeGroup g) {
   constexpr int kCols = 7 * NR, kTmem = NR == 16 ? 256 : 512;
-  constexpr int kSets = 2;                      // stages a converter holds in registers
+  constexpr int kBuf = NR == 64 ? 1 : 2;        // accumulator buffers in TMEM
   constexpr int na = 4;                         // query digits
   extern __shared__ __align__(16) unsigned char tr_raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(tr_raw) + 1023) & ~(uintptr_t)1023);
-  unsigned char* planes = sm;                   // [2][4 digits][128 keys][64 B]
-  unsigned char* qpl = sm + 2 * kTrPlanes;      // [chunk][4 NR rows][64 B]
-  __shared__ __align__(8) uint64_t planes_full[2], mma_done[2], acc_full[2], acc_empty[2], last_full;
+  constexpr int kSt = qk_stages<NR>();
+  unsigned char* planes = sm;                   // [kSt][4 bytes][128 keys][64 B]
+  unsigned char* qpl = sm + kSt * kTrPlanes;    // [chunk][4 NR rows][64 B]
+  __shared__ __align__(8) uint64_t planes_full[kSt], mma_done[kSt], acc_full[2], acc_empty[2], last_full;
   __shared__ uint32_t tmem_holder;
   __shared__ int s_fail;
-  // last stage (plus 1) of each plane buffer that uses digit 3
-  __shared__ int s_top[2];
-  // last tile (plus 1) with a value outside the digits' range.  Four slots: a
-  // converter runs at most two stages, so at most two tiles, ahead of the MMAs,
-  // and those at most two tiles ahead of the drain that reads the slot.
-  __shared__ int s_over[4];
+  __shared__ QkRows<NR> s_rows;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   // item -> sequence, KV head, row block, key tiles [t0, t1)
@@ -222,192 +326,199 @@ __global__ void __launch_bounds__(kQkThreads, 1) tree_qk(const __grid_constant__
   const int d = g.d, ns = (d + 63) / 64, G = g.G, Hq = g.Hq;
   const int rows = t.n * G, nrb = (rows + NR - 1) / NR, tiles = (t.len + kTrKeys - 1) / kTrKeys, qt = g.qk_tiles;
   const int it = blockIdx.x - g.qk_first[si];
-  const int blk = it / t.qk_per, t0 = (it - blk * t.qk_per) * qt, t1 = min(tiles, t0 + qt);
+  const int blk = it / t.qk_per, part = it - blk * t.qk_per, t0 = part * qt, t1 = min(tiles, t0 + qt);
   const int kvh = blk / nrb, rb = blk - kvh * nrb;
   const int r0 = rb * NR, nr = min(NR, rows - r0);
   const int total = (t1 - t0) * ns;
   const int32_t* const kc = t.k + (int64_t)kvh * t.kstride;
   const int32_t* const kt = t.kt + (int64_t)kvh * t.tstride;
   const int32_t* const qb = g.q + ((int64_t)t.node0 * Hq + kvh * G) * d;
-  int32_t* const sc = static_cast<int32_t*>(g.ws) + t.soff + ((int64_t)kvh * rows + r0) * t.pad;
   ta_wait();
   ta_go();
 
-  // a converter thread's part of stage (tile, s): keys 8 warp + 2 i + lane / 16, dims 64 s + 4 (lane % 16) ..
+  // a converter thread's part of stage (tile, s): keys 8 warp + 2 i + lane / 16,
+  // dims 64 s + 4 (lane % 16) ..  Keys past the sequence read its last key and
+  // dims past the head keep what the registers held: the first give scores
+  // that nothing reads, the second meet zero query digits.
   const uint32_t lkey = 8 * warp + (lane >> 4), off0 = (lkey * (uint32_t)d + 4 * (lane & 15)) * 4, step = 8 * (uint32_t)d;
-  auto load = [&](uint4 (&x)[4], int tile, int s) {
-    const int key0 = t.lo + (t0 + tile) * kTrKeys;
-    if (VEC && key0 + kTrKeys <= t.ctx && s * 64 + 64 <= d) {  // cache rows and dims only
-      const unsigned char* base = reinterpret_cast<const unsigned char*>(kc + (int64_t)key0 * d + s * 64);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = __ldg(reinterpret_cast<const uint4*>(base + (off0 + i * step)));
-      return;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int key = key0 + (int)lkey + 2 * i;
-      const int32_t* p = key < t.ctx ? kc + (int64_t)key * d : kt + (int64_t)(key - t.ctx) * d;
-      x[i] = key < t.lo + t.len ? load4<VEC>(p, s * 64 + 4 * (lane & 15), d) : make_uint4(0, 0, 0, 0);
-    }
-  };
-  uint4 x[kSets][4];
+  const int last_key = t.lo + t.len - 1;
+  uint4 x[2][4] = {};  // two stages in flight
   int lt = 0, ls = 0;  // next stage to load
   auto next = [&](uint4 (&y)[4]) {
-    if (lt < t1 - t0) load(y, lt, ls);
+    const int key0 = t.lo + (t0 + lt) * kTrKeys;
+    const unsigned char* p[4];
+    if (key0 + kTrKeys <= t.ctx) {  // cache rows only
+      const unsigned char* base = reinterpret_cast<const unsigned char*>(kc + (int64_t)key0 * d + ls * 64);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = base + (off0 + i * step);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = min(key0 + (int)lkey + 2 * i, last_key);
+        p[i] = reinterpret_cast<const unsigned char*>((key < t.ctx ? kc + (int64_t)key * d : kt + (int64_t)(key - t.ctx) * d) +
+                                                      ls * 64 + 4 * (lane & 15));
+      }
+    }
+    const int dim = ls * 64 + 4 * (lane & 15);
+    const bool on = lt < t1 - t0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) load4<VEC>(y[i], reinterpret_cast<const int32_t*>(p[i]) - dim, dim, d, on);
     if (++ls == ns) { ls = 0; ++lt; }
   };
   if (warp < kTrConvWarps) {
-#pragma unroll
-    for (int i = 0; i < kSets; ++i) next(x[i]);
+    next(x[0]);
+    next(x[1]);
   }
 
   if (tid == 0) {
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kSt; ++i) {
       mbar_init(&planes_full[i], kTrConvWarps);
       mbar_init(&mma_done[i], 1);
-      mbar_init(&acc_full[i], 2);
-      mbar_init(&acc_empty[i], 4);
     }
-    mbar_init(&last_full, 2);
-    s_top[0] = s_top[1] = s_over[0] = s_over[1] = s_over[2] = s_over[3] = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], kBuf == 1 ? kQkDrainWarps : 4);
+    }
+    mbar_init(&last_full, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     s_fail = 0;
+    s_rows.sc = static_cast<int32_t*>(g.ws) + t.soff + ((int64_t)kvh * rows + r0) * t.pad;
+    s_rows.pad = t.pad;
+    s_rows.nr = nr;
+    s_rows.ctx = t.ctx;
+    s_rows.lo = t.lo;
+    s_rows.len = t.len;
+    // (no row's window begins later than that of a node at the tree's greatest possible depth)
+    s_rows.maxstart = g.window > 0 ? max(0, t.ctx + t.n - g.window) : 0;
   }
+  if (tid < t.n) s_rows.npos[tid] = t.ctx + __popcll(g.mask[t.node0 + tid]) - 1;
   if (warp == 20) ta_alloc<kTmem>(&tmem_holder);
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (!ta_mbar_wait(bar, parity)) s_fail = 1;
   };
-  // query row r (node * G + head of the group) of this block
-  auto qrow = [&](int r) {
-    const int rr = r0 + r, node = rr / G;
+  if (tid < NR) {
+    const uint64_t m = tid < nr ? g.mask[t.node0 + (r0 + tid) / G] : 0;
+    s_rows.mask[tid] = m;
+    s_rows.start[tid] = tid < nr ? first_pos(g, t, m) : 0;
+    s_rows.top[tid] = 0;
+  }
+  // query digits: chunk s holds dims [64 s, 64 s + 64) of rows a * NR + r; two
+  // rows per warp and step, 16-byte pieces lane + 32 i of each
+  int32_t qmax = INT32_MIN;
+  auto qrow = [&](int r) {  // node * G + head of the group
+    const int rr = r0 + min(r, nr - 1), node = rr / G;
     return qb + ((int64_t)node * Hq + (rr - node * G)) * d;
   };
-  // query digits: chunk s holds dims [64 s, 64 s + 64) of rows a * NR + r.
-  // One row per warp and step, 16-byte pieces lane + 32 i of the row.
-  int32_t qmax = INT32_MIN;
-  for (int r = warp; r < NR; r += kQkThreads / 32) {
-    const int32_t* q = r < nr ? qrow(r) : qb;
-    uint4 v[4];
+#pragma unroll 1
+  for (int rp = 2 * warp; rp < NR; rp += kQkThreads / 16) {
+    uint4 v[2][4] = {};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      v[i] = r < nr && lane + 32 * i < ns * 16 ? load4<VEC>(q, 4 * (lane + 32 * i), d) : make_uint4(0, 0, 0, 0);
+    for (int h = 0; h < 2; ++h) {
+      const int32_t* q = qrow(rp + h);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int dg = lane + 32 * i;
-      if (dg >= ns * 16) break;
-      uint32_t o[4];
-      ta_t4(ta_digits((int32_t)v[i].x), ta_digits((int32_t)v[i].y), ta_digits((int32_t)v[i].z),
-            ta_digits((int32_t)v[i].w), o);
-      qmax = max4(qmax, v[i]);
+      for (int i = 0; i < 4; ++i) load4<VEC>(v[h][i], q, 4 * (lane + 32 * i), d, rp + h < nr);
+    }
 #pragma unroll
-      for (int a = 0; a < 4; ++a)
-        *reinterpret_cast<uint32_t*>(qpl + (dg >> 4) * (4 * NR * 64) + ta_sw(a * NR + r, (dg & 15) >> 2) +
-                                     4 * (dg & 3)) = o[a];
+    for (int h = 0; h < 2; ++h) {
+      int64_t sum = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int dg = lane + 32 * i;
+        sum += (int64_t)(int32_t)v[h][i].x + (int32_t)v[h][i].y + (int32_t)v[h][i].z + (int32_t)v[h][i].w;
+        if (dg >= ns * 16) continue;
+        uint32_t o[4];
+        ta_t4(ta_digits((int32_t)v[h][i].x), ta_digits((int32_t)v[h][i].y), ta_digits((int32_t)v[h][i].z),
+              ta_digits((int32_t)v[h][i].w), o);
+        qmax = max4(qmax, v[h][i]);
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+          *reinterpret_cast<uint32_t*>(qpl + (dg >> 4) * (4 * NR * 64) + ta_sw(a * NR + rp + h, (dg & 15) >> 2) +
+                                       4 * (dg & 3)) = o[a];
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) s_rows.corr[rp + h] = sum * kTrBias;
     }
   }
   ta_fence_async();
   fence_before();
+  // a query value outside the digits' range: the block's scores are taken directly
   const bool qover = __syncthreads_or(qmax > kTrMaxDigit);
   fence_after();
   const uint32_t tmem = tmem_holder;
-
-  // scores of rows [ra, re) of a drained tile, this thread's key
-  const int lk = 32 * (warp & 3) + lane;
-  auto drain = [&](int tile, int ra, int re) {
-    const int j = (t0 + tile) * kTrKeys + lk;
-    const bool slow = qover || *reinterpret_cast<volatile int*>(&s_over[tile & 3]) == tile + 1;
-    const uint32_t taddr = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)((tile & 1) * kCols);
-    int32_t* out = sc + (int64_t)ra * t.pad + j;
-    if (!slow) {
-      for (int r = ra; r < re; r += 4) {
-        int32_t c[7][4];
-#pragma unroll
-        for (int b = 0; b < 7; ++b) ta_ld4(taddr + b * NR + r, c[b]);
-        tmem_wait_ld();
-        int32_t sv[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int32_t cc[7] = {c[0][i], c[1][i], c[2][i], c[3][i], c[4][i], c[5][i], c[6][i]};
-          sv[i] = requantize(shift_sum(cc));
-        }
-        if (j < t.len) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (r + i < re) out[(int64_t)i * t.pad] = sv[i];
-        }
-        out += 4 * (int64_t)t.pad;
-      }
-    } else if (j < t.len) {
-      const int key = t.lo + j;
-      const int32_t* k = key < t.ctx ? kc + (int64_t)key * d : kt + (int64_t)(key - t.ctx) * d;
-      for (int r = ra; r < re; ++r, out += t.pad) {
-        const int32_t* q = qrow(r);
-        int64_t acc = 0;
-        for (int i = 0; i < d; ++i) acc = mac_wide(acc, q[i], k[i]);
-        *out = requantize(acc);
-      }
+  auto drain = [&](int tile, int quad, int step) {
+    const int j0 = (t0 + tile) * kTrKeys;
+    if (!qover) {
+      qk_drain<NR>(s_rows, tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)((kBuf == 1 ? 0 : tile & 1) * kCols), j0,
+                   quad, step);
+    } else {
+      const int key = t.lo + j0 + 32 * (warp & 3) + lane;
+      qk_drain_direct<NR>(s_rows, key < t.ctx ? kc + (int64_t)key * d : kt + (int64_t)(key - t.ctx) * d, qb, r0, G, Hq, d,
+                          j0, quad, step);
     }
   };
-  // The last tile is drained by all five groups of four warps, a fifth of the
-  // rows each (the converters are done by then).
-  const int last_tile = t1 - t0 - 1, fifth = ((nr + 19) / 20) * 4;
+  const int last_tile = t1 - t0 - 1;
 
   if (warp < kTrConvWarps) {
-    int tile = 0, s = 0;
     // rows 8 warp + 2 i + lane / 16 of the planes: bits 1-2 of the row are i
     const int ch = (lane & 15) >> 2;
     unsigned char* const pl0 = planes + lkey * 64 + 4 * (lane & 3);
-    unsigned char* const plx[4] = {pl0 + (ch << 4), pl0 + 128 + ((ch ^ 1) << 4), pl0 + 256 + ((ch ^ 2) << 4),
-                                   pl0 + 384 + ((ch ^ 3) << 4)};
-    for (int u = 0; u < total; u += kSets) {
+    const int plx[4] = {ch << 4, 128 + ((ch ^ 1) << 4), 256 + ((ch ^ 2) << 4), 384 + ((ch ^ 3) << 4)};
+    int tile = 0, s = 0, pb = 0, ph = 1;  // plane buffer, parity of its last use's end
+    for (int u = 0; u < total; u += 2) {
 #pragma unroll
-      for (int p = 0; p < kSets; ++p) {
+      for (int p = 0; p < 2; ++p) {
         if (u + p < total) {
-          if (u + p >= 2) wait(&mma_done[p], ((u + p - 2) >> 1) & 1);
-          uint32_t top = 0;
-          int32_t mx = INT32_MIN;
+          if (u + p >= kSt) wait(&mma_done[pb], ph);
+          unsigned char* const pl = pl0 + pb * kTrPlanes;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint32_t o[4];
-            ta_t4(ta_digits((int32_t)x[p][i].x), ta_digits((int32_t)x[p][i].y), ta_digits((int32_t)x[p][i].z),
-                  ta_digits((int32_t)x[p][i].w), o);
-            mx = max4(mx, x[p][i]);
-            top |= o[3];
+            ta_bytes(x[p][i].x, x[p][i].y, x[p][i].z, x[p][i].w, o);
 #pragma unroll
-            for (int b = 0; b < 4; ++b) *reinterpret_cast<uint32_t*>(plx[i] + p * kTrPlanes + b * kTrPlane) = o[b];
+            for (int b = 0; b < 4; ++b) *reinterpret_cast<uint32_t*>(pl + plx[i] + b * kTrPlane) = o[b];
           }
-          if (top) s_top[p] = u + p + 1;
-          if (mx > kTrMaxDigit) s_over[tile & 3] = tile + 1;
           ta_fence_async();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&planes_full[p]);
+          if (lane == 0) mbar_arrive(&planes_full[pb]);
+          if (++pb == kSt) { pb = 0; ph ^= 1; }
           next(x[p]);
-          if (++s == ns) { s = 0; ++tile; }
+          if (kBuf == 1 && ++s == ns) {  // the one accumulator is drained by everyone
+            wait(&acc_full[0], tile & 1);
+            fence_after();
+            drain(tile, 1 + (warp >> 2), 5);
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[0]);
+            s = 0;
+            ++tile;
+          }
         }
       }
     }
-    // a barrier of its own: a converter does not follow acc_full's phases, and
-    // a parity tells neighbouring phases apart only
-    wait(&last_full, 0);
-    fence_after();
-    const int ra = fifth * (1 + (warp >> 2));
-    if (ra < nr) drain(last_tile, ra, min(nr, ra + fifth));
+    if (kBuf == 2) {
+      // the last tile is drained by all five groups of four warps.  A barrier
+      // of its own: a converter does not follow acc_full's phases, and a parity
+      // tells neighbouring phases apart only
+      wait(&last_full, 0);
+      fence_after();
+      drain(last_tile, 1 + (warp >> 2), 5);
+    }
   } else if (warp == 20) {
     if (lane == 0) {
       const uint32_t full = ta_idesc(na * NR), low = ta_idesc((na - 1) * NR), one = ta_idesc(NR);
       const uint64_t pdesc = smem_desc_sw64(su32(planes)), qdesc = smem_desc_sw64(su32(qpl));
-      int tile = 0, s = 0;
+      int tile = 0, s = 0, pb = 0, ph = 0;
       for (int u = 0; u < total; ++u) {
-        const int pb = u & 1;
-        if (s == 0 && tile >= 2) wait(&acc_empty[tile & 1], ((tile - 2) >> 1) & 1);
-        wait(&planes_full[pb], (u >> 1) & 1);
+        const int ab = kBuf == 1 ? 0 : tile & 1;
+        if (s == 0 && tile >= kBuf) wait(&acc_empty[ab], ((tile - kBuf) / kBuf) & 1);
+        wait(&planes_full[pb], ph);
         fence_after();
         const uint64_t pd = ta_adv(pdesc, pb * kTrPlanes), qd = ta_adv(qdesc, s * (4 * NR * 64));
-        const uint32_t dcol = tmem + (uint32_t)((tile & 1) * kCols);
-        const bool top = *reinterpret_cast<volatile int*>(&s_top[pb]) == u + 1;
+        const uint32_t dcol = tmem + (uint32_t)(ab * kCols);
         if (s == 0) {
-          // the first products of a tile open its column blocks: digit b adds
-          // to the blocks that the digits before it opened and opens block
+          // the first products of a tile open its column blocks: byte b adds
+          // to the blocks that the bytes before it opened and opens block
           // b + na - 1
           mma_i8(dcol, pd, qd, full, 0);
 #pragma unroll
@@ -417,20 +528,15 @@ __global__ void __launch_bounds__(kQkThreads, 1) tree_qk(const __grid_constant__
           }
         } else {
 #pragma unroll
-          for (int b = 0; b < 3; ++b) mma_i8(dcol + b * NR, ta_adv(pd, b * kTrPlane), qd, full, 1);
-          if (top) mma_i8(dcol + 3 * NR, ta_adv(pd, 3 * kTrPlane), qd, full, 1);
+          for (int b = 0; b < 4; ++b) mma_i8(dcol + b * NR, ta_adv(pd, b * kTrPlane), qd, full, 1);
         }
 #pragma unroll
-        for (int b = 0; b < 3; ++b) mma_i8(dcol + b * NR, ta_adv(pd, b * kTrPlane + 32), ta_adv(qd, 32), full, 1);
-        if (top) mma_i8(dcol + 3 * NR, ta_adv(pd, 3 * kTrPlane + 32), ta_adv(qd, 32), full, 1);
+        for (int b = 0; b < 4; ++b) mma_i8(dcol + b * NR, ta_adv(pd, b * kTrPlane + 32), ta_adv(qd, 32), full, 1);
         mma_commit(&mma_done[pb]);
+        if (++pb == kSt) { pb = 0; ph ^= 1; }
         if (s == ns - 1) {
-          mma_commit(&acc_full[tile & 1]);
-          mbar_arrive(&acc_full[tile & 1]);  // hands the converters' s_over on
-          if (u == total - 1) {
-            mma_commit(&last_full);
-            mbar_arrive(&last_full);
-          }
+          mma_commit(&acc_full[ab]);
+          if (u == total - 1) mma_commit(&last_full);
           s = 0;
           ++tile;
         } else {
@@ -441,298 +547,227 @@ __global__ void __launch_bounds__(kQkThreads, 1) tree_qk(const __grid_constant__
   } else {
     // warps 16-19: accumulator lane (key) 32 (warp % 4) + lane
     for (int tile = 0; tile <= last_tile; ++tile) {
-      wait(&acc_full[tile & 1], (tile >> 1) & 1);
+      const int ab = kBuf == 1 ? 0 : tile & 1;
+      wait(&acc_full[ab], (tile / kBuf) & 1);
       fence_after();
-      drain(tile, 0, tile == last_tile ? min(nr, fifth) : nr);
+      if (kBuf == 1 || tile == last_tile) drain(tile, 0, 5);
+      else drain(tile, 0, 1);
       fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[tile & 1]);
+      if (lane == 0) mbar_arrive(&acc_empty[ab]);
     }
   }
   fence_before();
   __syncthreads();
+  if (tid < nr) {
+    uint32_t* tmax = reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(g.ws) + g.max_off) + t.moff;
+    tmax[((int64_t)kvh * rows + r0 + tid) * t.qk_per + part] = s_rows.top[tid];
+  }
   if (s_fail && tid == 0) atomicExch(&g_tree_err, 1);
   fence_after();
   if (warp == 20) ta_dealloc<kTmem>(tmem);
 }
 
 // ---------------------------------------------------------------------------
-// softmax: one cluster per row, its keys split over the CTAs in spans of 64
+// exp terms: a CTA takes one chunk of keys of one row.  Terms replace the
+// scores, as u32: the one value of 2^32 (a score equal to the maximum) is
+// coded 2^32 - 1, which no other score gives (the next lower score's term is
+// below 2^32 - 2^15).
 // ---------------------------------------------------------------------------
-constexpr int kSmThreads = 256;
-constexpr int kSmVec = 4;                                  // keys per thread and step
-constexpr int kSmRegs = 4;                                 // steps whose terms stay in registers
-constexpr int kSmRegKeys = kSmThreads * kSmVec * kSmRegs;  // keys per CTA of the register form
+constexpr int kExThreads = 256;
 
-__device__ __forceinline__ uint64_t sm_warp_max(uint64_t v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
-__device__ __forceinline__ int64_t sm_warp_sum(int64_t v) {
+__device__ __forceinline__ uint64_t ta_warp_sum(uint64_t v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
-// REG: every thread keeps its keys' scores, terms and weights in registers;
-// else they stay in the score scratch between the passes (longer rows).
-template <int NR, bool REG>
-__global__ void __launch_bounds__(kSmThreads) tree_softmax(const __grid_constant__ TreeGroup g) {
-  cg::cluster_group cl = cg::this_cluster();
-  const int CL = (int)cl.num_blocks(), rank = (int)cl.block_rank();
-  __shared__ uint64_t red[3][kSmThreads / 32], part[3];
+__global__ void __launch_bounds__(kExThreads) tree_exp(const __grid_constant__ TreeGroup g) {
+  __shared__ uint64_t red[kExThreads / 32];
+  __shared__ int32_t redi[kExThreads / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int G = g.G;
   // row of the group: (sequence, KV head, node, head of the KV head's group)
-  const int grow = blockIdx.x / CL, si = seq_of(g.row_first, g.nseq, grow);
+  const int grow = blockIdx.x / g.ex_chunks, chunk = blockIdx.x - grow * g.ex_chunks;
+  const int si = seq_of(g.row_first, g.nseq, grow);
   const TreeSeq t = g.seq[si];
-  const int rows = t.n * G, lrow = grow - g.row_first[si], kvh = lrow / rows, rr = lrow - kvh * rows;
-  const uint64_t mask = g.mask[t.node0 + rr / G];
+  const int rows = t.n * g.G, lrow = grow - g.row_first[si], rr = lrow % rows;
+  const uint64_t mask = g.mask[t.node0 + rr / g.G];
   const int start = first_pos(g, t, mask);
-  const int nrb = (rows + NR - 1) / NR, rb = rr / NR, r = rr % NR;
   unsigned char* const ws = static_cast<unsigned char*>(g.ws);
   int32_t* const sc = reinterpret_cast<int32_t*>(ws) + t.soff + (int64_t)lrow * t.pad;
-  const int chunks = t.pad / 64;  // the CTA's span: chunks [c0, c1) of 64 keys
-  const int c0 = (int)((int64_t)chunks * rank / CL), c1 = (int)((int64_t)chunks * (rank + 1) / CL);
-  const int k0 = c0 * 64, k1 = c1 * 64;
-
-  // block and cluster reduction number `i` of the row
-  auto reduce = [&](uint64_t v, int i, bool mx) {
-    v = mx ? sm_warp_max(v) : (uint64_t)sm_warp_sum((int64_t)v);
-    if (lane == 0) red[i][warp] = v;
-    __syncthreads();
-    v = red[i][lane & (kSmThreads / 32 - 1)];
-#pragma unroll
-    for (int o = kSmThreads / 64; o > 0; o >>= 1) {
-      const uint64_t u = __shfl_xor_sync(0xffffffffu, v, o);
-      v = mx ? max(v, u) : v + u;
-    }
-    if (CL > 1) {
-      if (tid == 0) part[i] = v;
-      cl.sync();
-      v = *cl.map_shared_rank(&part[i], lane < CL ? lane : 0);
-      if (lane >= CL) v = 0;
-      v = mx ? sm_warp_max(v) : (uint64_t)sm_warp_sum((int64_t)v);
-    }
-    return v;
-  };
-  auto key_of = [&](int step) { return k0 + (step * kSmThreads + tid) * kSmVec; };
-  // which of the keys j .. j + 3 the row attends
-  auto seen = [&](int j) -> uint32_t {
-    const int key = t.lo + j;
-    if (key >= start && key + 3 < t.ctx) return 15u;
-    uint32_t m = 0;
-    for (int i = 0; i < 4; ++i) m |= sees(g, t, mask, start, key + i) ? 1u << i : 0u;
-    return m;
-  };
-  // weight digits of four keys into the value kernel's operand tiles
-  unsigned char* const wpl = ws + t.woff + (int64_t)(kvh * nrb + rb) * chunks * (3 * NR * 64);
-  auto put = [&](int j, const int32_t (&w)[4]) {
-    uint32_t o[4];
-    ta_t4(ta_digits(w[0]), ta_digits(w[1]), ta_digits(w[2]), ta_digits(w[3]), o);
-    unsigned char* tile = wpl + (int64_t)(j >> 6) * (3 * NR * 64);
-#pragma unroll
-    for (int a = 0; a < 3; ++a)
-      *reinterpret_cast<uint32_t*>(tile + ta_sw(a * NR + r, (j & 63) >> 4) + (j & 15)) = o[a];
-  };
-
-  int32_t v[REG ? kSmRegs : 1][4];
-  uint32_t vis[REG ? kSmRegs : 1];
-  if (REG) {
-#pragma unroll
-    for (int s = 0; s < kSmRegs; ++s) vis[s] = key_of(s) < k1 ? seen(key_of(s)) : 0u;
-  }
+  const uint32_t* tmax = reinterpret_cast<const uint32_t*>(ws + g.max_off) + t.moff + (int64_t)lrow * t.qk_per;
   ta_wait();
   ta_go();
-  const int steps = (k1 - k0 + kSmThreads * kSmVec - 1) / (kSmThreads * kSmVec);
-  if (REG) {
-#pragma unroll
-    for (int s = 0; s < kSmRegs; ++s)
-      if (key_of(s) < k1) *reinterpret_cast<int4*>(v[s]) = *reinterpret_cast<const int4*>(sc + key_of(s));
+  if (chunk == 0 && t.splits > 1) {  // the value kernel's sums and counters
+    uint64_t* acc = reinterpret_cast<uint64_t*>(ws + g.acc_off) + (int64_t)grow * g.d;
+    for (int i = tid; i < g.d; i += kExThreads) acc[i] = 0;
+    const int items = t.cfirst + (lrow / rows * ((rows + g.nr - 1) / g.nr) + rr / g.nr) * ((g.d + 127) / 128);
+    if (tid < (g.d + 127) / 128) reinterpret_cast<int32_t*>(ws + g.wt_off)[(int64_t)tid * g.rows + grow] = 0;
+    if (rr % g.nr == 0 && tid < (g.d + 127) / 128) reinterpret_cast<uint32_t*>(ws + g.cnt_off)[items + tid] = 0;
   }
-  // the thread's first maximum: its keys come in ascending order
-  int32_t bv = INT32_MIN, bj = -1;
-  auto scan = [&](int j, uint32_t m, const int32_t* x) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if ((m >> i & 1) && (x[i] > bv || bj < 0)) { bv = x[i]; bj = j + i; }
-  };
-  if (REG) {
-#pragma unroll
-    for (int s = 0; s < kSmRegs; ++s) scan(key_of(s), vis[s], v[s]);
-  } else {
-    for (int s = 0; s < steps; ++s) {
-      const int j = key_of(s);
-      if (j < k1) {
-        *reinterpret_cast<int4*>(v[0]) = *reinterpret_cast<const int4*>(sc + j);
-        scan(j, seen(j), v[0]);
-      }
-    }
-  }
-  // (value, lowest index): the node itself is always attended, so the row's key is never 0
-  const uint64_t b = reduce(bj >= 0 ? (uint64_t)((uint32_t)bv ^ 0x80000000u) << 32 | (uint32_t)~bj : 0, 0, true);
-  const int32_t m = (int32_t)((uint32_t)(b >> 32) ^ 0x80000000u);
-  const int mi = (int)~(uint32_t)b;
-  // exp terms as u32: the one value of 2^32 (a score equal to the maximum)
-  // is coded 2^32 - 1, which no other score gives (the next lower score's
-  // term is below 2^32 - 2^15)
+  const int k0 = chunk * g.ex_keys, k1 = min(t.pad, k0 + g.ex_keys);
+  if (k0 >= k1 && chunk > 0) return;
+  uint32_t top = 0;
+  for (int i = lane; i < t.qk_per; i += 32) top = max(top, tmax[i]);
+  const uint32_t m = __reduce_max_sync(0xffffffffu, top) ^ 0x80000000u;
   uint64_t sum = 0;
-  auto terms = [&](uint32_t mk, int32_t* x) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t D = (uint32_t)m - (uint32_t)x[i];  // below the maximum by D
+  int32_t first = INT32_MAX;  // the thread's first key at the maximum
+  for (int j = k0 + 4 * tid; j < k1; j += 4 * kExThreads) {
+    uint4 v = *reinterpret_cast<const uint4*>(sc + j);
+    const int key = t.lo + j;
+    uint32_t vis = 15u;
+    if (!(key >= start && key + 3 < t.ctx)) {
+      vis = 0;
+      for (int i = 0; i < 4; ++i) vis |= sees(g, t, mask, start, key + i) ? 1u << i : 0u;
+    }
+    auto term = [&](uint32_t x, int i) -> uint32_t {
+      const uint32_t D = m - x;  // below the maximum by D
       uint64_t e = 0;
-      if ((mk >> i & 1) && D < (16u << 16)) e = exp_term_below(D);
+      if ((vis >> i & 1) && D < (16u << 16)) e = exp_term_below(D);
       sum += e;
-      x[i] = (int32_t)(uint32_t)(e >> 32 ? 0xffffffffu : (uint32_t)e);
-    }
-  };
-  if (REG) {
-#pragma unroll
-    for (int s = 0; s < kSmRegs; ++s)
-      if (key_of(s) < k1) terms(vis[s], v[s]);
-  } else {
-    for (int s = 0; s < steps; ++s) {
-      const int j = key_of(s);
-      if (j < k1) {
-        *reinterpret_cast<int4*>(v[0]) = *reinterpret_cast<const int4*>(sc + j);
-        terms(seen(j), v[0]);
-        *reinterpret_cast<int4*>(sc + j) = *reinterpret_cast<const int4*>(v[0]);
-      }
-    }
+      if (!(e >> 32)) return (uint32_t)e;
+      first = min(first, j + i);
+      return 0xffffffffu;
+    };
+    v = make_uint4(term(v.x, 0), term(v.y, 1), term(v.z, 2), term(v.w, 3));
+    *reinterpret_cast<uint4*>(sc + j) = v;
   }
-  sum = reduce(sum, 1, false);
-  const uint32_t inv = softmax_inverse(sum);
-  uint64_t wsum = 0;
-  auto weights = [&](int32_t* x) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] = softmax_weight_coded((uint32_t)x[i], inv, sum);
-      wsum += (uint32_t)x[i];
-    }
-  };
-  if (REG) {
-#pragma unroll
-    for (int s = 0; s < kSmRegs; ++s)
-      if (key_of(s) < k1) weights(v[s]);
-  } else {
-    for (int s = 0; s < steps; ++s) {
-      const int j = key_of(s);
-      if (j < k1) {
-        *reinterpret_cast<int4*>(v[0]) = *reinterpret_cast<const int4*>(sc + j);
-        weights(v[0]);
-        *reinterpret_cast<int4*>(sc + j) = *reinterpret_cast<const int4*>(v[0]);
-      }
-    }
+  sum = ta_warp_sum(sum);
+  first = __reduce_min_sync(0xffffffffu, first);
+  if (lane == 0) {
+    red[warp] = sum;
+    redi[warp] = first;
   }
-  wsum = reduce(wsum, 2, false);
-  // what the roundings left goes to the first maximum (the sum is below 2^31:
-  // at most 2^16 and half a unit per key)
-  const int32_t left = sub_sat(kOneAct, (int32_t)wsum);
-  auto finish = [&](int j, int32_t* x) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (j + i == mi) x[i] = add_sat(x[i], left);
-    const int32_t w[4] = {x[0], x[1], x[2], x[3]};
-    put(j, w);
-  };
-  if (REG) {
-#pragma unroll
-    for (int s = 0; s < kSmRegs; ++s)
-      if (key_of(s) < k1) finish(key_of(s), v[s]);
-  } else {
-    for (int s = 0; s < steps; ++s) {
-      const int j = key_of(s);
-      if (j < k1) {
-        *reinterpret_cast<int4*>(v[0]) = *reinterpret_cast<const int4*>(sc + j);
-        finish(j, v[0]);
-      }
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < kExThreads / 32; ++w) {
+      sum += red[w];
+      first = min(first, redi[w]);
     }
+    reinterpret_cast<uint64_t*>(ws + g.sum_off)[(int64_t)grow * g.ex_chunks + chunk] = sum;
+    reinterpret_cast<int32_t*>(ws + g.idx_off)[(int64_t)grow * g.ex_chunks + chunk] = first;
   }
-  if (CL > 1) cl.sync();  // every CTA's shared memory stays until it has been read
 }
 
 // ---------------------------------------------------------------------------
-// weighted values: one cluster per (sequence, KV head, row block, block of 128
-// dims), its keys split over the CTAs in chunks of 64; the partial i64 sums
-// meet in distributed shared memory
+// weighted values: an item is a (sequence, KV head, row block, block of 128
+// dims); its keys are split over `splits` CTAs in chunks of 64.  The partial
+// i64 sums meet in global memory (wrapping integer adds: any order gives the
+// same sum) and the item's last CTA to arrive rounds them.  (Clusters with the
+// sums in distributed shared memory measured worse: only about 13 clusters of
+// eight large CTAs fit the GPU at once, so 16 took two waves.)
 // ---------------------------------------------------------------------------
+constexpr int kPvStages = 4;
 template <int NR>
-__host__ __device__ constexpr int pv_smem() { return 2 * kTrPlanes + 2 * 3 * NR * 64 + 1024; }
+__host__ __device__ constexpr int pv_smem() { return kPvStages * (kTrPlanes + 3 * NR * 64) + 1024; }
 
 template <int NR>
 __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__ TreeGroup g) {
-  constexpr int kTmem = NR == 16 ? 128 : 256;
+  constexpr int kTmem = NR == 16 ? 128 : NR == 32 ? 256 : 512;
   constexpr int kW = 3 * NR * 64;               // one stage's weight tile
+  constexpr int kE = (NR * 16 + kTrConv - 1) / kTrConv;  // (row, four keys) pieces of it per converter thread
   extern __shared__ __align__(16) unsigned char tr_raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(tr_raw) + 1023) & ~(uintptr_t)1023);
-  unsigned char* planes = sm;                   // [2][4 digits][128 dims][64 keys]
-  unsigned char* wsm = sm + 2 * kTrPlanes;      // [2][3 NR rows][64 keys]
-  int64_t* const pacc = reinterpret_cast<int64_t*>(sm);  // [NR][128] partial sums, after the last MMA
-  __shared__ __align__(8) uint64_t planes_full[2], mma_done[2], acc_full;
+  unsigned char* planes = sm;                   // [stage][4 bytes][128 dims][64 keys]
+  unsigned char* wsm = sm + kPvStages * kTrPlanes;  // [stage][3 NR rows][64 keys]
+  __shared__ __align__(8) uint64_t planes_full[kPvStages], mma_done[kPvStages], acc_full;
   __shared__ uint32_t tmem_holder;
   __shared__ int s_fail;
-  __shared__ int s_top[2];  // last stage (plus 1) of each plane buffer that uses digit 3
-  cg::cluster_group cl = cg::this_cluster();
-  const int S = (int)cl.num_blocks(), sp = (int)cl.block_rank();
+  __shared__ uint64_t s_sum[NR];                // each row's sum of terms
+  __shared__ int32_t s_first[NR];               // its first maximum
+  __shared__ uint32_t s_inv[NR];
+  __shared__ int32_t s_wsum[NR];                // each row's sum of this CTA's weights
+  __shared__ uint32_t s_last;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  const int item = blockIdx.x / S, si = seq_of(g.pv_first, g.nseq, item);
+  const int si = seq_of(g.pv_first, g.nseq, blockIdx.x);
   const TreeSeq t = g.seq[si];
   const int d = g.d, nd = (d + 127) / 128, G = g.G, Hq = g.Hq;
   const int rows = t.n * G, nrb = (rows + NR - 1) / NR, chunks = t.pad / 64;
-  const int it = item - g.pv_first[si];
+  const int S = t.splits, ic = blockIdx.x - g.pv_first[si], it = ic / S, sp = ic - it * S;
   const int blk = it / nd, db = it - blk * nd, kvh = blk / nrb, rb = blk - kvh * nrb;
   const int c0 = (int)((int64_t)chunks * sp / S), c1 = (int)((int64_t)chunks * (sp + 1) / S);
   const int r0 = rb * NR, nr = min(NR, rows - r0), total = c1 - c0;
-  const unsigned char* const wpl =
-      static_cast<unsigned char*>(g.ws) + t.woff + ((int64_t)blk * chunks + c0) * kW;
+  const int lrow0 = kvh * rows + r0, grow0 = g.row_first[si] + lrow0;
+  unsigned char* const ws = static_cast<unsigned char*>(g.ws);
+  const uint32_t* const ex = reinterpret_cast<const uint32_t*>(ws) + t.soff + (int64_t)lrow0 * t.pad + c0 * 64;
   const int32_t* const vc = t.v + (int64_t)kvh * t.kstride;
   const int32_t* const vt = t.vt + (int64_t)kvh * t.tstride;
 
   // a converter thread's part of a stage: dim tid % 128, keys 16 (tid / 128) .. + 16
   const int dl = tid & 127, quarter = (tid >> 7) & 3, dim = db * 128 + dl;
-  const uint32_t off0 = ((uint32_t)(16 * quarter) * d + dl) * 4, step = 4 * (uint32_t)d;
-  auto load = [&](int32_t (&x)[16], int u) {
+  // keys past the sequence read its last key (their weights are zero), dims
+  // past the head its last dim (their sums are not stored)
+  const int cdim = min(dim, d - 1), last_key = t.lo + t.len - 1;
+  const uint32_t off0 = ((uint32_t)(16 * quarter) * d + cdim) * 4, step = 4 * (uint32_t)d;
+  uint32_t x[2][16] = {};  // two stages in flight
+  auto load = [&](uint32_t (&y)[16], int u) {
     const int key0 = t.lo + (c0 + u) * 64;
-    if (key0 + 64 <= t.ctx && db * 128 + 128 <= d) {  // cache rows and dims only
-      const unsigned char* base = reinterpret_cast<const unsigned char*>(vc + (int64_t)key0 * d + db * 128);
+    const bool on = u < total;
+    if (key0 + 64 <= t.ctx) {  // cache rows only
+      const unsigned char* base = reinterpret_cast<const unsigned char*>(vc + (int64_t)key0 * d);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = __ldg(reinterpret_cast<const int32_t*>(base + (off0 + i * step)));
+      for (int i = 0; i < 16; ++i) ld4(y[i], base + (off0 + i * step), on);
     } else {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int key = key0 + 16 * quarter + i;
-        const int32_t* p = key < t.ctx ? vc + (int64_t)key * d : vt + (int64_t)(key - t.ctx) * d;
-        x[i] = key < t.lo + t.len && dim < d ? p[dim] : 0;
+        const int key = min(key0 + 16 * quarter + i, last_key);
+        ld4(y[i], (key < t.ctx ? vc + (int64_t)key * d : vt + (int64_t)(key - t.ctx) * d) + cdim, on);
       }
     }
   };
-  int32_t x[2][16];  // two stages in flight
-  uint4 wv;
-  auto load_w = [&](int u) {
-    if (tid < kW / 16) wv = reinterpret_cast<const uint4*>(wpl + (int64_t)u * kW)[tid];
+  // its part of the weights: rows tid / 16 + 32 i (at most the block's last),
+  // keys 4 (tid % 16) .. + 4
+  const int wr = tid >> 4, wq = tid & 15;
+  uint4 ev[kE] = {};
+  auto load_e = [&](int u) {
+#pragma unroll
+    for (int i = 0; i < kE; ++i) ld16(ev[i], ex + (int64_t)min(wr + 32 * i, nr - 1) * t.pad + u * 64 + 4 * wq, u < total);
   };
-  static_assert(kW / 16 <= kTrConv, "one 16-byte piece of a weight tile per converter thread");
-  // The values do not depend on the softmax: their first stage loads before
-  // the wait (this grid starts only after the score kernel has completed, and
-  // with it everything before it).
+  // The values do not depend on the terms: their first stages load before the
+  // wait (this grid starts only after the score kernel has completed, and with
+  // it everything before it).
   if (warp < kTrConvWarps) {
-    if (total > 0) load(x[0], 0);
-    if (total > 1) load(x[1], 1);
+    load(x[0], 0);
+    load(x[1], 1);
   }
   if (tid == 0) {
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kPvStages; ++i) {
       mbar_init(&planes_full[i], kTrConvWarps);
       mbar_init(&mma_done[i], 1);
     }
     mbar_init(&acc_full, 1);
-    s_top[0] = s_top[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     s_fail = 0;
   }
   if (warp == kTrConvWarps) ta_alloc<kTmem>(&tmem_holder);
+  ta_wait();
+  ta_go();
+  if (warp < kTrConvWarps) load_e(0);
+  const uint64_t* psum = reinterpret_cast<const uint64_t*>(ws + g.sum_off);
+  const int32_t* pidx = reinterpret_cast<const int32_t*>(ws + g.idx_off);
+  const int nsum = (t.pad + g.ex_keys - 1) / g.ex_keys;  // chunks of this sequence's rows
+  if (tid < 8 * NR) {  // eight lanes a row
+    const int r = tid >> 3;
+    uint64_t v = 0;
+    int32_t f = INT32_MAX;
+    if (r < nr)
+      for (int i = tid & 7; i < nsum; i += 8) {
+        v += psum[(int64_t)(grow0 + r) * g.ex_chunks + i];
+        f = min(f, pidx[(int64_t)(grow0 + r) * g.ex_chunks + i]);
+      }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) {
+      v += __shfl_xor_sync(0xffffffffu, v, o);
+      f = min(f, __shfl_xor_sync(0xffffffffu, f, o));
+    }
+    if ((tid & 7) == 0) {
+      s_sum[r] = v;
+      s_first[r] = f;
+      s_inv[r] = r < nr ? softmax_inverse(v) : 0;
+      s_wsum[r] = 0;
+    }
+  }
   fence_before();
   __syncthreads();
   fence_after();
@@ -741,53 +776,67 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
     if (!ta_mbar_wait(bar, parity)) s_fail = 1;
   };
 
-  int32_t mx = INT32_MIN;  // of the thread's values
   if (warp < kTrConvWarps) {
+    int32_t wsum[kE] = {};
+    int pb = 0, ph = 1;  // plane buffer, parity of its last use's end
     for (int u0 = 0; u0 < total; u0 += 2) {
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         const int u = u0 + p;
         if (u < total) {
-          if (u >= 2) wait(&mma_done[p], ((u - 2) >> 1) & 1);
-          unsigned char* pl = planes + p * kTrPlanes + ta_sw(dl, quarter);
-          uint32_t o[4][4], top = 0;  // one 16-byte piece of each digit plane
+          if (u >= kPvStages) wait(&mma_done[pb], ph);
+#pragma unroll
+          for (int i = 0; i < kE; ++i) {
+            const int r = wr + 32 * i;
+            if (r >= NR) break;
+            const uint32_t inv = s_inv[r];
+            const uint64_t sum = s_sum[r];
+            const int32_t w0 = ta_weight(ev[i].x, inv, sum), w1 = ta_weight(ev[i].y, inv, sum),
+                          w2 = ta_weight(ev[i].z, inv, sum), w3 = ta_weight(ev[i].w, inv, sum);
+            wsum[i] += w0 + w1 + w2 + w3;
+            uint32_t o[4];
+            ta_t4(ta_digits(w0), ta_digits(w1), ta_digits(w2), ta_digits(w3), o);
+#pragma unroll
+            for (int a = 0; a < 3; ++a)
+              *reinterpret_cast<uint32_t*>(wsm + pb * kW + ta_sw(a * NR + r, wq >> 2) + 4 * (wq & 3)) = o[a];
+          }
+          unsigned char* pl = planes + pb * kTrPlanes + ta_sw(dl, quarter);
+          uint32_t o[4][4];  // one 16-byte piece of each byte plane
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            const int32_t x0 = x[p][4 * k], x1 = x[p][4 * k + 1], x2 = x[p][4 * k + 2], x3 = x[p][4 * k + 3];
             uint32_t q[4];
-            ta_t4(ta_digits(x0), ta_digits(x1), ta_digits(x2), ta_digits(x3), q);
-            mx = max(max(max(mx, x0), max(x1, x2)), x3);
-            top |= q[3];
+            ta_bytes(x[p][4 * k], x[p][4 * k + 1], x[p][4 * k + 2], x[p][4 * k + 3], q);
 #pragma unroll
             for (int b = 0; b < 4; ++b) o[b][k] = q[b];
           }
 #pragma unroll
           for (int b = 0; b < 4; ++b)
             *reinterpret_cast<uint4*>(pl + b * kTrPlane) = make_uint4(o[b][0], o[b][1], o[b][2], o[b][3]);
-          if (u == 0) {
-            ta_wait();  // the weights
-            load_w(0);
-          }
-          if (tid < kW / 16) reinterpret_cast<uint4*>(wsm + p * kW)[tid] = wv;
-          if (top) s_top[p] = u + 1;
           ta_fence_async();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&planes_full[p]);
-          if (u + 1 < total) load_w(u + 1);
-          if (u + 2 < total) load(x[p], u + 2);
+          if (lane == 0) mbar_arrive(&planes_full[pb]);
+          if (++pb == kPvStages) { pb = 0; ph ^= 1; }
+          load_e(u + 1);
+          load(x[p], u + 2);
         }
       }
     }
+    // a row's weights lie in the 16 threads of its keys
+#pragma unroll
+    for (int i = 0; i < kE; ++i) {
+      int32_t v = wsum[i];
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if (wq == 0 && wr + 32 * i < NR) s_wsum[wr + 32 * i] = v;
+    }
   } else if (lane == 0 && total > 0) {
-    ta_wait();  // the converters' first stage waits for the weights: not within a bounded wait
     const uint32_t full = ta_idesc(3 * NR), low = ta_idesc(2 * NR), one = ta_idesc(NR);
     const uint64_t pdesc = smem_desc_sw64(su32(planes)), wdesc = smem_desc_sw64(su32(wsm));
+    int pb = 0, ph = 0;
     for (int u = 0; u < total; ++u) {
-      const int pb = u & 1;
-      wait(&planes_full[pb], (u >> 1) & 1);
+      wait(&planes_full[pb], ph);
       fence_after();
       const uint64_t pd = ta_adv(pdesc, pb * kTrPlanes), wd = ta_adv(wdesc, pb * kW);
-      const bool top = *reinterpret_cast<volatile int*>(&s_top[pb]) == u + 1;
       if (u == 0) {  // opens the column blocks, as in the score kernel
         mma_i8(tmem, pd, wd, full, 0);
 #pragma unroll
@@ -797,82 +846,66 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
         }
       } else {
 #pragma unroll
-        for (int b = 0; b < 3; ++b) mma_i8(tmem + b * NR, ta_adv(pd, b * kTrPlane), wd, full, 1);
-        if (top) mma_i8(tmem + 3 * NR, ta_adv(pd, 3 * kTrPlane), wd, full, 1);
+        for (int b = 0; b < 4; ++b) mma_i8(tmem + b * NR, ta_adv(pd, b * kTrPlane), wd, full, 1);
       }
 #pragma unroll
-      for (int b = 0; b < 3; ++b) mma_i8(tmem + b * NR, ta_adv(pd, b * kTrPlane + 32), ta_adv(wd, 32), full, 1);
-      if (top) mma_i8(tmem + 3 * NR, ta_adv(pd, 3 * kTrPlane + 32), ta_adv(wd, 32), full, 1);
+      for (int b = 0; b < 4; ++b) mma_i8(tmem + b * NR, ta_adv(pd, b * kTrPlane + 32), ta_adv(wd, 32), full, 1);
       mma_commit(&mma_done[pb]);
+      if (++pb == kPvStages) { pb = 0; ph ^= 1; }
       if (u == total - 1) mma_commit(&acc_full);
     }
     wait(&acc_full, 0);
   }
-  // a value outside the digits' range: the block's sums are taken directly
-  const bool slow = __syncthreads_or(mx > kTrMaxDigit);
-  ta_wait();
-  ta_go();
+  __syncthreads();
   fence_after();
   // ---- the block's partial sums: lane dl, rows split over the four quarters
   auto orow = [&](int r) {
     const int rr = r0 + r, node = rr / G;
     return g.out + ((int64_t)(t.node0 + node) * Hq + kvh * G + (rr - node * G)) * d;
   };
-  auto give = [&](int r, int64_t v) {
-    if (r >= nr) return;
-    if (S > 1) pacc[r * 128 + dl] = v;
-    else if (dim < d) orow(r)[dim] = requantize(v);
+  // Row r's sum v of digit products and wt of weights to the output: the bytes'
+  // bias, and what the weights' roundings left times the first maximum's value.
+  unsigned long long* const acc = reinterpret_cast<unsigned long long*>(ws + g.acc_off) + (int64_t)grow0 * d;
+  int32_t* const wtot = reinterpret_cast<int32_t*>(ws + g.wt_off) + (int64_t)db * g.rows + grow0;  // sums of weights
+  auto finish = [&](int r, uint64_t v, int32_t wt) {
+    const int key = t.lo + s_first[r];
+    const int32_t* p = key < t.ctx ? vc + (int64_t)key * d : vt + (int64_t)(key - t.ctx) * d;
+    v += (uint64_t)(kTrBias * wt) + (uint64_t)mul_wide(sub_sat(kOneAct, wt), p[dim]);
+    orow(r)[dim] = requantize((int64_t)v);
   };
-  if (warp < kTrConvWarps) {
+  if (warp < kTrConvWarps && total > 0) {
     constexpr int kQ = NR / 4;
-    if (total == 0) {
-      for (int r = quarter; r < nr; r += 4) give(r, 0);
-    } else if (!slow) {
-      const uint32_t taddr = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-      for (int r = quarter * kQ; r < min(nr, (quarter + 1) * kQ); r += 4) {
-        int32_t c[6][4];
+    const uint32_t taddr = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+    for (int r = quarter * kQ; r < min(nr, (quarter + 1) * kQ); r += 4) {
+      int32_t c[6][4];
 #pragma unroll
-        for (int b = 0; b < 6; ++b) ta_ld4(taddr + b * NR + r, c[b]);
-        tmem_wait_ld();
+      for (int b = 0; b < 6; ++b) ta_ld4(taddr + b * NR + r, c[b]);
+      tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int32_t cc[7] = {c[0][i], c[1][i], c[2][i], c[3][i], c[4][i], c[5][i], 0};
-          give(r + i, shift_sum(cc));
+      for (int i = 0; i < 4; ++i) {
+        const int64_t v = shift_sum(0, c[0][i], c[1][i], c[2][i], c[3][i], c[4][i], c[5][i], 0);
+        if (r + i < nr && dim < d) {
+          if (S > 1) atomicAdd(acc + (int64_t)(r + i) * d + dim, (unsigned long long)v);
+          else finish(r + i, (uint64_t)v, s_wsum[r + i]);
         }
       }
-    } else {
-      for (int r = quarter; r < nr; r += 4) {
-        int64_t sum = 0;
-        for (int j = c0 * 64; j < min(c1 * 64, t.len) && dim < d; ++j) {
-          const unsigned char* tile = wpl + (int64_t)((j >> 6) - c0) * kW;
-          int32_t w = 0;
-          for (int a = 2; a >= 0; --a)
-            w = w * 256 + (int8_t)tile[ta_sw(a * NR + r, (j & 63) >> 4) + (j & 15)];
-          const int key = t.lo + j;
-          const int32_t* p = key < t.ctx ? vc + (int64_t)key * d : vt + (int64_t)(key - t.ctx) * d;
-          sum = mac_wide(sum, w, p[dim]);
-        }
-        give(r, sum);
-      }
+    }
+  }
+  if (S > 1) {
+    uint32_t* const cnt = reinterpret_cast<uint32_t*>(ws + g.cnt_off) + t.cfirst + it;
+    if (tid < nr && total > 0) atomicAdd(wtot + tid, s_wsum[tid]);
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) s_last = atomicAdd(cnt, 1u) == (uint32_t)S - 1;
+    __syncthreads();
+    if (s_last && warp < kTrConvWarps && dim < d) {
+      __threadfence();
+      for (int r = quarter; r < nr; r += 4)
+        finish(r, __ldcg(acc + (int64_t)r * d + dim), __ldcg(wtot + r));
     }
   }
   fence_before();
-  if (S > 1) {
-    cl.sync();
-    // rank sp rounds every S-th group of 32 sums of the block
-    for (int e = warp * S + sp; e < nr * 4 && warp < kTrConvWarps; e += kTrConvWarps * S) {
-      const int r = e >> 2, c = (e & 3) * 32 + lane;
-      int64_t v[16];
-#pragma unroll
-      for (int q = 0; q < 16; ++q) v[q] = q < S ? *cl.map_shared_rank(&pacc[r * 128 + c], q) : 0;
-#pragma unroll
-      for (int q = 1; q < 16; ++q) v[0] += v[q];
-      if (db * 128 + c < d) orow(r)[db * 128 + c] = requantize(v[0]);
-    }
-    cl.sync();  // every CTA's shared memory stays until it has been read
-  } else {
-    __syncthreads();
-  }
+  __syncthreads();
   if (s_fail && tid == 0) atomicExch(&g_tree_err, 1);
   fence_after();
   if (warp == kTrConvWarps) ta_dealloc<kTmem>(tmem);
@@ -882,6 +915,10 @@ template <int NR, bool VEC>
 void qk_attr() {
   cudaFuncSetAttribute(tree_qk<NR, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, qk_smem<NR>(8));
 }
+template <int NR>
+void pv_attr() {
+  cudaFuncSetAttribute(tree_pv<NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, pv_smem<NR>());
+}
 
 }  // namespace
 
@@ -890,10 +927,11 @@ void tree_attn_init() {
   qk_attr<16, false>();
   qk_attr<32, true>();
   qk_attr<32, false>();
-  cudaFuncSetAttribute(tree_pv<16>, cudaFuncAttributeMaxDynamicSharedMemorySize, pv_smem<16>());
-  cudaFuncSetAttribute(tree_pv<32>, cudaFuncAttributeMaxDynamicSharedMemorySize, pv_smem<32>());
-  cudaFuncSetAttribute(tree_pv<16>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  cudaFuncSetAttribute(tree_pv<32>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  qk_attr<64, true>();
+  qk_attr<64, false>();
+  pv_attr<16>();
+  pv_attr<32>();
+  pv_attr<64>();
 }
 
 int tree_attn_error_flag(bool reset) {
@@ -909,50 +947,90 @@ int tree_attn_error_flag(bool reset) {
 size_t tree_attn_plan(TreeGroup& g) {
   constexpr int kSms = 148;
   const int G = g.G = g.Hq / g.Hkv, nd = (g.d + 127) / 128;
-  int maxrows = 0;
-  for (int i = 0; i < g.nseq; ++i) maxrows = std::max(maxrows, g.seq[i].n * G);
-  g.nr = maxrows <= 16 ? 16 : 32;
-  int64_t soff = 0, tiles = 0;
-  int rows = 0, pv = 0, maxchunks = 1;
+  int maxrows = 0, maxpad = 0;
   for (int i = 0; i < g.nseq; ++i) {
     TreeSeq& t = g.seq[i];
     // the shallowest node's window is the lowest of the tree
     t.lo = g.window > 0 && t.ctx + 1 > g.window ? std::min(t.ctx, t.ctx + 1 - g.window) : 0;
     t.len = t.ctx - t.lo + t.n;
     t.pad = (t.len + 63) & ~63;
+    maxrows = std::max(maxrows, t.n * G);
+    maxpad = std::max(maxpad, t.pad);
+  }
+  // Rows of a block.  64 rows read each key and value half as often as 32, but
+  // leave half as many items: taken where those still make two waves.
+  int64_t wide = 0;  // score tiles of 64-row blocks
+  for (int i = 0; i < g.nseq; ++i)
+    wide += (int64_t)g.Hkv * ((g.seq[i].n * G + 63) / 64) * ((g.seq[i].len + kTrKeys - 1) / kTrKeys);
+  g.nr = maxrows <= 16 ? 16 : maxrows <= 32 || wide < 2 * kSms ? 32 : 64;
+  int64_t soff = 0, moff = 0;
+  int rows = 0, pv = 0, qk = 0, counters = 0;
+  auto blocks = [&](const TreeSeq& t) { return (int64_t)g.Hkv * ((t.n * G + g.nr - 1) / g.nr); };
+  auto ceil_div = [](int x, int y) { return (x + y - 1) / y; };
+  // Key tiles of a score CTA and 64-key chunks of a value CTA: the size with
+  // the shortest run of work on one SM (CTAs in waves of one per SM; a CTA's
+  // fixed work counted in stages of its loop).
+  auto pick = [&](int most, auto&& ctas, auto&& stages) {
+    int size = 1;
+    int64_t best = INT64_MAX;
+    for (int k = 1; k <= most; k += 1 + k / 8) {
+      const int64_t cost = (ctas(k) + kSms - 1) / kSms * stages(k);
+      if (cost < best) {
+        best = cost;
+        size = k;
+      }
+    }
+    return size;
+  };
+  const int ns = (g.d + 63) / 64;
+  g.qk_tiles = pick(
+      16,
+      [&](int k) {
+        int64_t n = 0;
+        for (int i = 0; i < g.nseq; ++i) n += blocks(g.seq[i]) * ceil_div(ceil_div(g.seq[i].len, kTrKeys), k);
+        return n;
+      },
+      [&](int k) { return k * ns + 4; });
+  const int per = pick(
+      kTrSplitKeys / 64,
+      [&](int k) {
+        int64_t n = 0;
+        for (int i = 0; i < g.nseq; ++i) n += blocks(g.seq[i]) * nd * ceil_div(g.seq[i].pad / 64, k);
+        return n;
+      },
+      [&](int k) { return k + 4; });
+  for (int i = 0; i < g.nseq; ++i) {
+    TreeSeq& t = g.seq[i];
     t.soff = soff;
-    const int nrb = (t.n * G + g.nr - 1) / g.nr;
     soff += (int64_t)t.pad * t.n * g.Hq;
     g.row_first[i] = rows;
     rows += t.n * g.Hq;
-    tiles += (int64_t)g.Hkv * nrb * ((t.len + kTrKeys - 1) / kTrKeys);
-    maxchunks = std::max(maxchunks, t.pad / 64);
+    t.splits = ceil_div(t.pad / 64, per);
     g.pv_first[i] = pv;
-    pv += g.Hkv * nrb * nd;
+    pv += (int)blocks(t) * nd * t.splits;
+    t.cfirst = counters;
+    counters += (int)blocks(t) * nd;
+    t.qk_per = ceil_div(ceil_div(t.len, kTrKeys), g.qk_tiles);
+    g.qk_first[i] = qk;
+    qk += (int)blocks(t) * t.qk_per;
+    t.moff = moff;
+    moff += (int64_t)t.n * g.Hq * t.qk_per;
   }
   g.rows = rows;
   g.pv_items = pv;
-  // key tiles of one score item: enough items for two waves, no more than needed
-  g.qk_tiles = (int)std::max<int64_t>(1, std::min<int64_t>(16, tiles / (2 * kSms)));
-  // CTAs of one value item: while they fit one wave and have two chunks of
-  // their own, and at most kTrSplitKeys keys each
-  g.splits = 1;
-  while (g.splits < 16 && ((int64_t)pv * g.splits * 2 <= kSms && maxchunks >= g.splits * 4)) g.splits *= 2;
-  while (g.splits < 16 && (maxchunks + g.splits - 1) / g.splits * 64 > kTrSplitKeys) g.splits *= 2;
-  int64_t off = soff * 4;
-  int qk = 0;
-  for (int i = 0; i < g.nseq; ++i) {
-    TreeSeq& t = g.seq[i];
-    const int nrb = (t.n * G + g.nr - 1) / g.nr, chunks = t.pad / 64;
-    off = (off + 1023) & ~(int64_t)1023;
-    t.woff = off;
-    off += (int64_t)g.Hkv * nrb * chunks * (3 * g.nr * 64);
-    g.qk_first[i] = qk;
-    t.qk_per = ((t.len + kTrKeys - 1) / kTrKeys + g.qk_tiles - 1) / g.qk_tiles;
-    qk += g.Hkv * nrb * t.qk_per;
-  }
   g.qk_items = qk;
-  return (size_t)((off + 255) & ~(int64_t)255);
+  // keys of one term CTA: four per thread, more where the rows alone fill the GPU
+  g.ex_keys = 4 * kExThreads;
+  while (g.ex_keys < 16 * kExThreads && (int64_t)rows * (maxpad / g.ex_keys) > 32 * kSms) g.ex_keys *= 2;
+  g.ex_chunks = (maxpad + g.ex_keys - 1) / g.ex_keys;
+  auto up = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
+  g.max_off = up(soff * 4);
+  g.sum_off = up(g.max_off + moff * 4);
+  g.idx_off = up(g.sum_off + (int64_t)rows * g.ex_chunks * 8);
+  g.acc_off = up(g.idx_off + (int64_t)rows * g.ex_chunks * 4);
+  g.wt_off = up(g.acc_off + (int64_t)rows * g.d * 8);
+  g.cnt_off = up(g.wt_off + (int64_t)nd * rows * 4);
+  return (size_t)up(g.cnt_off + (int64_t)counters * 4);
 }
 
 template <int NR>
@@ -960,18 +1038,8 @@ static void tree_launch(const TreeGroup& g, bool vec, cudaStream_t s) {
   const int ns = (g.d + 63) / 64;
   if (vec) ta_launch(tree_qk<NR, true>, dim3(g.qk_items), dim3(kQkThreads), qk_smem<NR>(ns), 1, s, g);
   else ta_launch(tree_qk<NR, false>, dim3(g.qk_items), dim3(kQkThreads), qk_smem<NR>(ns), 1, s, g);
-  // CTAs per row: the register form's keys at most, and enough CTAs to fill
-  // the GPU while they have a step of their own
-  int pad = 0;
-  for (int i = 0; i < g.nseq; ++i) pad = std::max(pad, g.seq[i].pad);
-  auto span = [&](int CL) { return (pad / 64 + CL - 1) / CL * 64; };
-  int CL = 1;
-  while (CL < 8 && (span(CL) > kSmRegKeys || ((int64_t)g.rows * CL < 148 && span(CL) > kSmThreads * kSmVec))) CL *= 2;
-  if (span(CL) <= kSmRegKeys)
-    ta_launch(tree_softmax<NR, true>, dim3(CL * g.rows), dim3(kSmThreads), 0, CL, s, g);
-  else
-    ta_launch(tree_softmax<NR, false>, dim3(CL * g.rows), dim3(kSmThreads), 0, CL, s, g);
-  ta_launch(tree_pv<NR>, dim3(g.pv_items * g.splits), dim3(kPvThreads), pv_smem<NR>(), g.splits, s, g);
+  ta_launch(tree_exp, dim3((unsigned)g.rows * g.ex_chunks), dim3(kExThreads), 0, 1, s, g);
+  ta_launch(tree_pv<NR>, dim3(g.pv_items), dim3(kPvThreads), pv_smem<NR>(), 1, s, g);
 }
 
 void launch_tree_attn(const TreeGroup& g, cudaStream_t s) {
@@ -980,7 +1048,8 @@ void launch_tree_attn(const TreeGroup& g, cudaStream_t s) {
     bits |= reinterpret_cast<uintptr_t>(g.seq[i].k) | reinterpret_cast<uintptr_t>(g.seq[i].kt);
   const bool vec = g.d % 4 == 0 && (bits & 15) == 0;
   if (g.nr == 16) tree_launch<16>(g, vec, s);
-  else tree_launch<32>(g, vec, s);
+  else if (g.nr == 32) tree_launch<32>(g, vec, s);
+  else tree_launch<64>(g, vec, s);
 }
 
 }  // namespace rdet

@@ -27,7 +27,18 @@ uint64_t exp_second() { return exp_term_below(1); }
 
 static int64_t one(uint64_t e, uint64_t sum) {
   const uint32_t coded = e >> 32 ? 0xffffffffu : (uint32_t)e;
-  return softmax_weight_coded(coded, softmax_inverse(sum), sum) != softmax_weight((int64_t)e, (int64_t)sum);
+  int32_t w;
+  return softmax_weight_near(coded, softmax_inverse(sum), &w) && w != softmax_weight((int64_t)e, (int64_t)sum);
+}
+// how many of n random weights the reciprocal leaves open
+int64_t weights_open(uint64_t seed, int64_t n) {
+  int64_t open = 0;
+  for (int64_t i = 0; i < n; ++i) {
+    const uint64_t a = mix(seed + 2 * i), b = mix(seed + 2 * i + 1);
+    int32_t w;
+    open += !softmax_weight_near((uint32_t)(b >> (32 + b % 16)), softmax_inverse((1ull << 32) + (a >> 24)), &w);
+  }
+  return open;
 }
 // random sums and terms
 int64_t weights_random(uint64_t seed, int64_t n) {

@@ -22,7 +22,7 @@ def host():
     assert r.returncode == 0, r.stderr
     L = C.CDLL(out)
     for name, args in (("exp_all", [C.c_int32]), ("exp_second", []), ("weights_random", [C.c_uint64, C.c_int64]),
-                       ("weights_ties", [C.c_uint64, C.c_int64]), ("weights_one", [C.c_int64])):
+                       ("weights_ties", [C.c_uint64, C.c_int64]), ("weights_open", [C.c_uint64, C.c_int64]), ("weights_one", [C.c_int64])):
         getattr(L, name).argtypes, getattr(L, name).restype = args, C.c_int64
     return L
 
@@ -44,3 +44,8 @@ def test_weights(host, seed):
 
 def test_weights_of_a_lone_key(host):
     assert host.weights_one(300_000) == 0
+
+
+def test_few_weights_are_left_open(host):
+    # 12 of 2^16 positions between two halves
+    assert host.weights_open(7, 1_000_000) < 400
