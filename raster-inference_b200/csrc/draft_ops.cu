@@ -19,16 +19,20 @@ __device__ __forceinline__ void do_wait() { asm volatile("griddepcontrol.wait;" 
 __device__ __forceinline__ void do_go() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // ---------------------------------------------------------------------------
-// Rules on a logits row.  One thread-block cluster per row: CTA r takes the
-// tiles r, r + CL, ... of the vocabulary and the row's best (value, token) is
-// reduced through distributed shared memory, so a call needs no workspace.
-// A tile's tokens with a history count or a bias ("special" ones, few) are
-// marked in a bit set while the counts are taken; the stream over the tile
-// passes the others through, and the special ones are then computed one per
-// thread, so that the division's long sequence runs on dense warps only.
+// Rules on a logits row.  One thread-block cluster per row: its CTAs take
+// parts of the vocabulary, and the row's best (value, token) is reduced
+// through distributed shared memory, so a call needs no workspace.  A CTA
+//   gathers   the history's ids and the biases that fall into its part in a
+//             hash table (counts, sums of biases) and marks their tokens in a
+//             bit set, reading the history once;
+//   computes  the marked tokens (few), one listed slot per thread, so that their
+//             loads and the division's long sequence are waited for once, on
+//             dense warps;
+//   streams   its part without a barrier: every token is copied, masked ones
+//             as the lowest value, and the maximum of the unmarked ones found;
+//             then the marked tokens' values replace what the stream wrote.
+// Bound by memory: a row streams once.
 // ---------------------------------------------------------------------------
-constexpr int kRuleThreads = 512;
-constexpr int kRuleTile = 16384;  // tokens of one tile: a 64 KB count table
 
 __device__ __forceinline__ int32_t clamp_i32(int64_t v) {
   return v > INT32_MAX ? INT32_MAX : (v < INT32_MIN ? INT32_MIN : (int32_t)v);
@@ -38,106 +42,249 @@ __device__ __forceinline__ uint64_t rule_key(int32_t v, uint32_t t) {
   return (uint64_t)((uint32_t)v ^ 0x80000000u) << 32 | (uint32_t)~t;
 }
 
+// The CTAs of a row take its chunks of 512 tokens in turn, so that the low ids,
+// which tokenizers give the frequent tokens, spread over all of them, in
+// batches of 65536 tokens (li: a token's number within its CTA's batch).  The
+// stream takes four 16-byte pieces per thread and step.  Where a batch marks
+// more tokens than the table holds, it is computed after the stream, block by
+// block of as many tokens as there are slots.
+constexpr int kRuleVec = 4;
+constexpr uint32_t kRuleChunk = 512;
+constexpr uint32_t kRuleBatch = 65536, kRuleSlots = 2048, kRuleProbes = 32, kRuleEmpty = 0xffffffffu;
 struct RuleSmem {
-  uint32_t count[kRuleTile];
-  uint32_t special[kRuleTile / 32];  // tokens with a count or a bias
-  uint32_t biased[kRuleTile / 32];
-  uint16_t list[kRuleTile];          // the special tokens, in any order
+  unsigned long long bias[kRuleSlots];  // sums of the biases, exact
+  uint32_t key[kRuleSlots];             // li, or empty
+  uint32_t count[kRuleSlots];
+  uint32_t marked[kRuleBatch / 32];
+  uint16_t list[kRuleSlots];            // the slots in use, in any order
 };
 
-__global__ void __launch_bounds__(kRuleThreads) logit_rules_kernel(const __grid_constant__ RuleRows rs, uint32_t vocab,
-                                                                  uint32_t* tokens) {
+// loads and stores of rows that are touched once
+__device__ __forceinline__ void ld_stream(int4& v, const int32_t* p, bool on) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %5, 0;\n @p ld.global.L1::no_allocate.v4.s32 {%0, %1, %2, %3}, [%4];\n}"
+      : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
+      : "l"(p), "r"((int)on));
+}
+__device__ __forceinline__ void ld_word(uint32_t& v, const uint32_t* p, bool on) {
+  asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %2, 0;\n @p ld.global.u32 %0, [%1];\n}"
+               : "+r"(v)
+               : "l"(p), "r"((int)on));
+}
+
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) logit_rules_kernel(const __grid_constant__ RuleRows rs,
+                                                                             uint32_t vocab, uint32_t* tokens) {
+  constexpr uint32_t kStep = THREADS * 4 * kRuleVec;
   extern __shared__ __align__(16) unsigned char rule_raw[];
   RuleSmem& sm = *reinterpret_cast<RuleSmem*>(rule_raw);
-  __shared__ uint64_t best[kRuleThreads / 32], cta_best;
-  __shared__ uint32_t nspecial;
+  __shared__ uint64_t best[THREADS / 32], cta_best;
+  __shared__ uint32_t s_over, s_used;
   cg::cluster_group cl = cg::this_cluster();
-  const int CL = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+  const uint32_t CL = cl.num_blocks(), rank = cl.block_rank();  // CL: a power of two
   const int tid = threadIdx.x, row = blockIdx.y;
-  const RuleRow& r = rs.row[row];
+  const int32_t* const logits = rs.row[row].logits;
+  int32_t* const out = rs.row[row].out;
+  const uint32_t* const allow = rs.row[row].allow;
+  const uint32_t* const history = rs.row[row].history;
+  const uint32_t* const bias_ids = rs.row[row].bias_ids;
+  const uint32_t hlen = rs.row[row].history_len, nbias = rs.row[row].n_bias;
   do_wait();
   do_go();
-  const bool hist = r.history_len > 0 || r.token != 0xffffffffu || r.parent >= 0;
-  const bool any = hist || r.n_bias > 0;
+  const bool any = hlen > 0 || nbias > 0 || rs.row[row].has_path;
+  const bool wide = ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+  auto allowed = [&](uint32_t w) { return allow ? __ldg(allow + w) : 0xffffffffu; };
   uint64_t b = 0;
-  for (uint32_t t0 = (uint32_t)rank * kRuleTile; t0 < vocab; t0 += (uint32_t)CL * kRuleTile) {
-    const uint32_t nt = min((uint32_t)kRuleTile, vocab - t0);
-    if (any) {
-      __syncthreads();  // the previous tile's tables are no longer read
-      for (int i = tid; i < kRuleTile / 4; i += kRuleThreads)
-        reinterpret_cast<uint4*>(sm.count)[i] = make_uint4(0, 0, 0, 0);
-      for (int i = tid; i < kRuleTile / 32; i += kRuleThreads) sm.special[i] = sm.biased[i] = 0;
-      if (tid == 0) nspecial = 0;
-      __syncthreads();
-      auto mark = [&](uint32_t i) {
-        if (!(atomicOr(&sm.special[i >> 5], 1u << (i & 31)) & (1u << (i & 31))))
-          sm.list[atomicAdd(&nspecial, 1u)] = (uint16_t)i;
+  // the thread's first maximum of unmarked tokens (they come in ascending
+  // order), and the first of them where all are at the lowest value
+  int32_t bv = INT32_MIN;
+  uint32_t bt = 0xffffffffu, lowest = 0xffffffffu;
+  const uint32_t share = 31 - __clz((int)CL);  // log2 of the row's CTAs
+  const uint32_t chunks = (vocab + kRuleChunk - 1) / kRuleChunk;
+  for (uint32_t c0 = 0; (c0 << share) + rank < chunks; c0 += kRuleBatch / kRuleChunk) {  // the batch's first chunk
+    auto token = [&](uint32_t li) { return (((c0 + li / kRuleChunk) << share) + rank) * kRuleChunk + li % kRuleChunk; };
+    // f(li) for the ids of the row's history and path, g(li, value) for its biases
+    auto each = [&](auto&& f, auto&& g) {
+      auto local = [&](uint32_t id, auto&& h) {
+        const uint32_t c = id / kRuleChunk, li = ((c >> share) - c0) * kRuleChunk + id % kRuleChunk;
+        if (id < vocab && (c & (CL - 1)) == rank && (c >> share) >= c0 && li < kRuleBatch) h(li);
       };
-      for (uint32_t k = tid; k < r.history_len; k += kRuleThreads) {
-        const uint32_t i = r.history[k] - t0;
-        if (i < nt) {
-          atomicAdd(&sm.count[i], 1u);
-          mark(i);
+      // a thread's biases and eight of its ids in flight together
+      uint32_t bi[2] = {kRuleEmpty, kRuleEmpty}, bw[2] = {0, 0};  // (empty: past every vocabulary)
+      const uint32_t* const bias_values = reinterpret_cast<const uint32_t*>(rs.row[row].bias_values);
+      for (uint32_t k0 = 0; k0 < max(hlen, nbias); k0 += 8 * THREADS) {
+        uint32_t id[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          id[k] = kRuleEmpty;
+          ld_word(id[k], history + k0 + tid + k * THREADS, k0 + tid + k * THREADS < hlen);
         }
-      }
-      if (tid == 0)  // the row's own token and its ancestors'
-        for (int p = row; p >= 0; p = rs.row[p].parent) {
-          const uint32_t tok = rs.row[p].token;
-          if (tok != 0xffffffffu && tok - t0 < nt) {
-            atomicAdd(&sm.count[tok - t0], 1u);
-            mark(tok - t0);
+        if (k0 == 0) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            ld_word(bi[k], bias_ids + tid + k * THREADS, tid + k * THREADS < nbias);
+            ld_word(bw[k], bias_values + tid + k * THREADS, tid + k * THREADS < nbias);
           }
         }
-      for (uint32_t k = tid; k < r.n_bias; k += kRuleThreads) {
-        const uint32_t i = r.bias_ids[k] - t0;
-        if (i < nt) {
-          atomicOr(&sm.biased[i >> 5], 1u << (i & 31));
-          mark(i);
-        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) local(id[k], f);
       }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) local(bi[k], [&](uint32_t li) { g(li, (int32_t)bw[k]); });
+      for (uint32_t k = tid + 2 * THREADS; k < nbias; k += THREADS)
+        local(bias_ids[k], [&](uint32_t li) { g(li, (int32_t)bias_values[k]); });
+      if (tid < kRuleRows && (rs.row[row].path[tid >> 6] >> (tid & 63) & 1)) local(rs.row[tid].token, f);
+    };
+    // the slot of li; the table's load is low, so few probes reach it
+    auto slot = [&](uint32_t li) {
+      uint32_t h = (li * 40503u >> 5) % kRuleSlots;
+      for (uint32_t n = 0; n < kRuleProbes; ++n, h = (h + 1) % kRuleSlots) {
+        const uint32_t old = atomicCAS(&sm.key[h], kRuleEmpty, li);
+        if (old == kRuleEmpty) sm.list[atomicAdd(&s_used, 1u)] = (uint16_t)h;
+        if (old == kRuleEmpty || old == li) return h;
+      }
+      s_over = 1;
+      return kRuleSlots;
+    };
+    auto clear = [&] {
+      for (uint32_t i = tid; i < kRuleSlots; i += THREADS) {
+        sm.bias[i] = 0;
+        sm.key[i] = kRuleEmpty;
+        sm.count[i] = 0;
+      }
+    };
+    // token t with the rules that slot h holds; false where it is masked
+    auto compute = [&](uint32_t t, uint32_t h, int32_t& x) {
+      x = logits[t];
+      const uint32_t ok = allowed(t >> 5) >> (t & 31), c = sm.count[h];
+      const int64_t bias = (int64_t)sm.bias[h];
+      if (!(ok & 1)) return false;
+      if (c) {
+        const int32_t rep = rs.row[row].repetition;
+        x = x > 0 ? div_act(x, rep) : mul_sat(x, rep);
+        x = sub_sat(sub_sat(x, clamp_i32((int64_t)rs.row[row].frequency * (int64_t)c)), rs.row[row].presence);
+      }
+      x = add_sat(x, clamp_i32(bias));
+      b = max(b, rule_key(x, t));
+      return true;
+    };
+    if (any) {
+      clear();
+      for (uint32_t i = tid; i < kRuleBatch / 32; i += THREADS) sm.marked[i] = 0;
+      if (tid == 0) s_over = s_used = 0;
+      __syncthreads();
+      auto mark = [&](uint32_t li) { atomicOr(&sm.marked[li >> 5], 1u << (li & 31)); };
+      each(
+          [&](uint32_t li) {
+            mark(li);
+            const uint32_t h = slot(li);
+            if (h < kRuleSlots) atomicAdd(&sm.count[h], 1u);
+          },
+          [&](uint32_t li, int32_t value) {
+            mark(li);
+            const uint32_t h = slot(li);
+            if (h < kRuleSlots) atomicAdd(&sm.bias[h], (unsigned long long)(long long)value);
+          });
       __syncthreads();
     }
-    for (uint32_t i = tid; i < nt; i += kRuleThreads) {
-      int32_t v = r.logits[t0 + i];
-      const bool ok = !r.allow || ((r.allow[(t0 + i) >> 5] >> ((t0 + i) & 31)) & 1);
-      if (!ok) v = INT32_MIN;
-      else if (!any || !((sm.special[i >> 5] >> (i & 31)) & 1)) b = max(b, rule_key(v, t0 + i));
-      if (r.out) r.out[t0 + i] = v;
+    int4 v[kRuleVec] = {};
+    auto load = [&](uint32_t l0) {
+#pragma unroll
+      for (int k = 0; k < kRuleVec; ++k) {
+        const uint32_t li = l0 + 4 * (tid + k * THREADS), t = token(li);
+        ld_stream(v[k], logits + t, wide && li < kRuleBatch && t + 4 <= vocab && t < vocab);
+      }
+    };
+    load(0);
+    if (any && !s_over)
+      for (uint32_t k = tid; k < s_used; k += THREADS) {
+        const uint32_t h = sm.list[k];
+        int32_t x;
+        if (compute(token(sm.key[h]), h, x)) sm.count[h] = (uint32_t)x;
+        else sm.key[h] = kRuleEmpty;  // masked: stays what the stream writes
+      }
+    auto unmarked = [&](uint32_t li) { return any ? ~sm.marked[li >> 5] : 0xffffffffu; };
+    for (uint32_t l0 = 0; l0 < kRuleBatch && token(l0) < vocab; l0 += kStep) {
+#pragma unroll
+      for (int k = 0; k < kRuleVec; ++k) {
+        const uint32_t li = l0 + 4 * (tid + k * THREADS), t = token(li);
+        if (wide && t < vocab && t + 4 <= vocab) {
+          const uint32_t s = t & 31, ok = allowed(t >> 5) >> s, plain = ok & (unmarked(li) >> s) & 15u;
+          if (!(ok & 1)) v[k].x = INT32_MIN;
+          if (!(ok & 2)) v[k].y = INT32_MIN;
+          if (!(ok & 4)) v[k].z = INT32_MIN;
+          if (!(ok & 8)) v[k].w = INT32_MIN;
+          if (out) __stcs(reinterpret_cast<int4*>(out + t), v[k]);
+          const int32_t x = plain & 1 ? v[k].x : INT32_MIN, y = plain & 2 ? v[k].y : INT32_MIN,
+                        z = plain & 4 ? v[k].z : INT32_MIN, u = plain & 8 ? v[k].w : INT32_MIN;
+          const int32_t m = max(max(x, y), max(z, u));
+          if (m > bv) {
+            bv = m;
+            bt = t + (x == m ? 0 : y == m ? 1 : z == m ? 2 : 3);
+          }
+          if (plain && lowest == 0xffffffffu) lowest = t + __ffs(plain) - 1;
+        } else if (t < vocab) {  // the row's last tokens, or a row that is not 16-byte aligned
+          for (uint32_t e = 0; e < 4 && t + e < vocab; ++e) {
+            int32_t x = logits[t + e];
+            const uint32_t s = (t + e) & 31;
+            if (!(allowed((t + e) >> 5) >> s & 1)) x = INT32_MIN;
+            else if (unmarked(li) >> s & 1) b = max(b, rule_key(x, t + e));
+            if (out) out[t + e] = x;
+          }
+        }
+      }
+      load(l0 + kStep);
     }
     if (any) {
-      __syncthreads();  // the special tokens' values replace what the stream wrote
-      for (uint32_t k = tid; k < nspecial; k += kRuleThreads) {
-        const uint32_t i = sm.list[k], t = t0 + i;
-        if (r.allow && !((r.allow[t >> 5] >> (t & 31)) & 1)) continue;
-        int32_t v = r.logits[t];
-        const uint32_t c = sm.count[i];
-        if (c) {
-          v = v > 0 ? div_act(v, r.repetition) : mul_sat(v, r.repetition);
-          v = sub_sat(sub_sat(v, clamp_i32((int64_t)r.frequency * (int64_t)c)), r.presence);
+      __syncthreads();  // the marked tokens' values replace what the stream wrote
+      if (!s_over) {
+        for (uint32_t k = tid; out && k < s_used; k += THREADS) {
+          const uint32_t h = sm.list[k];
+          if (sm.key[h] != kRuleEmpty) out[token(sm.key[h])] = (int32_t)sm.count[h];
         }
-        if ((sm.biased[i >> 5] >> (i & 31)) & 1) {
-          int64_t s = 0;
-          for (uint32_t j = 0; j < r.n_bias; ++j)
-            if (r.bias_ids[j] == t) s += r.bias_values[j];
-          v = add_sat(v, clamp_i32(s));
+        __syncthreads();
+      } else {
+        for (uint32_t block = 0; block < kRuleBatch; block += kRuleSlots) {
+          __syncthreads();
+          clear();
+          __syncthreads();
+          each(
+              [&](uint32_t li) {
+                if (li - block < kRuleSlots) atomicAdd(&sm.count[li - block], 1u);
+              },
+              [&](uint32_t li, int32_t value) {
+                if (li - block < kRuleSlots) atomicAdd(&sm.bias[li - block], (unsigned long long)(long long)value);
+              });
+          __syncthreads();
+          for (uint32_t h = tid; h < kRuleSlots; h += THREADS)
+            if ((sm.marked[(block + h) >> 5] >> (h & 31)) & 1) {
+              int32_t x;
+              const uint32_t t = token(block + h);
+              if (compute(t, h, x) && out) out[t] = x;
+            }
         }
-        b = max(b, rule_key(v, t));
-        if (r.out) r.out[t] = v;
+        __syncthreads();
       }
     }
   }
+  if (bt != 0xffffffffu) b = max(b, rule_key(bv, bt));
+  else if (lowest != 0xffffffffu) b = max(b, rule_key(INT32_MIN, lowest));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
   if ((tid & 31) == 0) best[tid >> 5] = b;
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kRuleThreads / 32; ++w) b = max(b, best[w]);
-    cta_best = b;
+  if (tid < 32) {
+    b = tid < THREADS / 32 ? best[tid] : 0;
+#pragma unroll
+    for (int o = THREADS / 64; o > 0; o >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
+    if (tid == 0) cta_best = b;
   }
   cl.sync();
-  if (rank == 0 && tid == 0) {
-    for (int c = 1; c < CL; ++c) b = max(b, *cl.map_shared_rank(&cta_best, c));
-    tokens[row] = b ? ~(uint32_t)b : 0xffffffffu;
+  if (rank == 0 && tid < 32) {
+    b = tid < (int)CL ? *cl.map_shared_rank(&cta_best, tid) : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
+    if (tid == 0) tokens[row] = b ? ~(uint32_t)b : 0xffffffffu;
   }
   cl.sync();  // every CTA's shared memory stays until it has been read
 }
@@ -172,17 +319,25 @@ __global__ void __launch_bounds__(256) tree_commit_kernel(const __grid_constant_
 
 }  // namespace
 
+template <int THREADS>
+static void rules_attr() {
+  cudaFuncSetAttribute(logit_rules_kernel<THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                       (int)sizeof(RuleSmem));
+  cudaFuncSetAttribute(logit_rules_kernel<THREADS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+}
 void draft_ops_init() {
-  cudaFuncSetAttribute(logit_rules_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(RuleSmem));
+  rules_attr<256>();
+  rules_attr<1024>();
 }
 
-void launch_logit_rules(const RuleRows& r, int rows, uint32_t vocab, uint32_t* tokens, cudaStream_t s) {
-  const int tiles = (int)((vocab + kRuleTile - 1) / kRuleTile);
+template <int THREADS>
+static void rules_launch(const RuleRows& r, int rows, uint32_t vocab, uint32_t* tokens, int most, cudaStream_t s) {
+  const int tiles = (int)((vocab + THREADS * 16 - 1) / (THREADS * 16));
   int CL = 1;
-  while (CL < 8 && CL < tiles) CL *= 2;
+  while (CL < most && CL < tiles) CL *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(CL, rows, 1);
-  cfg.blockDim = dim3(kRuleThreads, 1, 1);
+  cfg.blockDim = dim3(THREADS, 1, 1);
   cfg.dynamicSmemBytes = sizeof(RuleSmem);
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
@@ -194,7 +349,15 @@ void launch_logit_rules(const RuleRows& r, int rows, uint32_t vocab, uint32_t* t
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  cudaLaunchKernelEx(&cfg, logit_rules_kernel, r, vocab, tokens);
+  cudaLaunchKernelEx(&cfg, logit_rules_kernel<THREADS>, r, vocab, tokens);
+}
+
+// Few rows take the largest clusters (sixteen CTAs) of large CTAs: one row of
+// 262144 logits under a history of 513 takes 7.7 us (512 threads and eight CTAs
+// a row: 9.7).  Many rows fill the GPU with small CTAs, four of them an SM.
+void launch_logit_rules(const RuleRows& r, int rows, uint32_t vocab, uint32_t* tokens, cudaStream_t s) {
+  if (rows * 16 <= 148) rules_launch<1024>(r, rows, vocab, tokens, 16, s);
+  else rules_launch<256>(r, rows, vocab, tokens, 8, s);
 }
 
 void launch_tree_commit(const CommitMoves& m, int moves, cudaStream_t s) {

@@ -426,8 +426,9 @@ struct RuleRow {
   const int32_t* bias_values;
   uint32_t history_len, n_bias;
   int32_t repetition, frequency, presence;
-  int32_t parent;  // row of the same launch, -1: none
   uint32_t token;
+  uint32_t has_path;               // some bit of path is set
+  uint64_t path[kRuleRows / 64];   // the launch's rows whose token counts for this one: itself and its ancestors
 };
 struct RuleRows {
   RuleRow row[kRuleRows];

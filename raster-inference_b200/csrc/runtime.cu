@@ -3471,9 +3471,18 @@ int32_t rdet_det_logits_rules(const rdet_logit_row* rows, uint32_t n_rows, uint3
       const uint32_t i0 = cut[c], i1 = cut[c + 1];
       for (uint32_t i = i0; i < i1; ++i) {
         const rdet_logit_row& r = rows[i];
-        part->row[i - i0] = RuleRow{r.logits, r.out, r.allow, r.history, r.bias_ids, r.bias_values, r.history_len,
-                                    r.n_bias, r.repetition, r.frequency, r.presence,
-                                    r.parent >= 0 ? r.parent - (int32_t)i0 : -1, r.token};
+        RuleRow& d = part->row[i - i0];
+        d = RuleRow{r.logits, r.out, r.allow, r.history, r.bias_ids, r.bias_values, r.history_len, r.n_bias,
+                    r.repetition, r.frequency, r.presence, r.token, 0, {}};
+        if (r.parent >= 0) {
+          const RuleRow& up = part->row[r.parent - i0];
+          std::copy(std::begin(up.path), std::end(up.path), d.path);
+          d.has_path = up.has_path;
+        }
+        if (r.token != RDET_NO_TOKEN) {
+          d.path[(i - i0) >> 6] |= 1ull << ((i - i0) & 63);
+          d.has_path = 1;
+        }
       }
       launch_logit_rules(*part, (int)(i1 - i0), vocab, tokens_out + i0, static_cast<cudaStream_t>(stream));
     }

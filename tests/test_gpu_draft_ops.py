@@ -430,3 +430,26 @@ def test_tree_attention_many_tiles_back_to_back():
     torch.cuda.synchronize()
     assert time.monotonic() - t < 0.9
     assert torch.equal(outs[0], outs[1])
+
+
+def test_logit_rules_every_token_special():
+    # more special and biased tokens in a tile than its lists hold
+    rng = np.random.default_rng(12)
+    vocab = 9000
+    lg = rng.integers(-2**20, 2**20, vocab).astype(np.int32)
+    hist = np.concatenate([rng.permutation(vocab)[:6000], rng.integers(0, vocab, 9000)]).astype(np.int32)
+    ids = np.concatenate([rng.permutation(vocab)[:5000], rng.integers(0, vocab, 300)]).astype(np.int32)
+    val = rng.integers(-2**20, 2**20, ids.size).astype(np.int32)
+    ld, hd, idd, vd = dev(lg), dev(hist), dev(ids), dev(val)
+    out = torch.zeros(vocab, dtype=torch.int32, device="cuda")
+    tok = torch.zeros(1, dtype=torch.int32, device="cuda")
+    rdet.det_logits_rules(rdet.logit_rows([dict(
+        logits=ld.data_ptr(), out=out.data_ptr(), history=hd.data_ptr(), history_len=hist.size, bias_ids=idd.data_ptr(),
+        bias_values=vd.data_ptr(), n_bias=ids.size, repetition=80000, frequency=1234, presence=777, token=3)]),
+        vocab, tok.data_ptr())
+    torch.cuda.synchronize()
+    count = {}
+    for t in list(hist) + [3]:
+        count[int(t)] = count.get(int(t), 0) + 1
+    want, best = R.rules_row(lg, count, 80000, 1234, 777, [(int(a), int(b)) for a, b in zip(ids, val)], None)
+    assert np.array_equal(out.cpu().numpy(), want) and tok.item() == best
