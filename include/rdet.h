@@ -34,6 +34,9 @@ extern "C" {
 #define RDET_E_RANGE (-6)
 #define RDET_E_OOM (-7)
 
+#define RDET_MAX_TREE_NODES 64     /* nodes of one drafted tree */
+#define RDET_NO_TOKEN 0xffffffffu  /* no token */
+
 typedef struct rdet_ctx rdet_ctx;
 typedef struct rdet_seq rdet_seq;
 
@@ -124,6 +127,48 @@ int32_t rdet_decode_finalize(rdet_ctx* ctx, rdet_seq* seq);
  * sequence's CUDA graph.  Writes the n_tokens selected ids; logits of the
  * last decode stay resident. */
 int32_t rdet_generate(rdet_ctx* ctx, rdet_seq* seq, uint32_t n_tokens, uint32_t* tokens_out);
+
+/* ---- drafted decoding -------------------------------------------------------
+ * Several drafted tokens of a sequence checked in one pass, and tokens selected
+ * under rules.  No counterpart in the reference; what an accepted path leaves
+ * (tokens, caches, logits, commitments) is bit for bit what decoding its
+ * tokens one by one with rdet_decode leaves.
+ *
+ * Rules of one sequence's selection (the values of rdet_logit_row, here in
+ * host memory, read before the call returns).  allow: [(vocab + 31) / 32]
+ * words, for rdet_tree_select one such mask per node, or NULL. */
+typedef struct rdet_rules {
+  const uint32_t* allow;
+  const uint32_t* history;
+  const uint32_t* bias_ids;
+  const int32_t* bias_values;
+  uint32_t history_len, n_bias;
+  int32_t repetition, frequency, presence; /* Q16.16; repetition > 0, 65536: none */
+} rdet_rules;
+/* The greedy token of each sequence's logits under rules[i] (NULL: no rules,
+ * as rdet_select_batch); RDET_NO_TOKEN where no token is allowed.  The logits
+ * stay as they are. */
+int32_t rdet_select_rules(rdet_ctx* ctx, rdet_seq* const* seqs, size_t n, const rdet_rules* rules,
+                          uint32_t* tokens_out);
+/* Runs every node of every sequence's drafted tree through the model at once:
+ * sequence i has counts[i] nodes (1 to RDET_MAX_TREE_NODES), its tokens and
+ * parents follow those of sequence i - 1 (parents within its own tree, before
+ * the node, -1: it follows the last committed token).  The nodes' K/V rows are
+ * written behind the committed rows of the caches, so max_ctx must hold them;
+ * the sequence's state does not change until rdet_tree_accept.  At most
+ * max_prefill nodes per call. */
+int32_t rdet_tree_decode(rdet_ctx* ctx, rdet_seq* const* seqs, size_t nseq, const uint32_t* counts,
+                         const uint32_t* tokens, const int32_t* parents);
+/* The greedy token after every node of the sequences' drafted trees, in their
+ * order, under rules[i] (NULL: none).  A node's own token and its ancestors'
+ * count as history behind rules[i].history. */
+int32_t rdet_tree_select(rdet_ctx* ctx, rdet_seq* const* seqs, size_t nseq, const rdet_rules* rules,
+                         uint32_t* tokens_out);
+/* Commits path_counts[i] nodes of sequence i's drafted tree (path_nodes: the
+ * paths one after the other; a path starts at a root, every node's parent is
+ * the node before it) and drops the tree; a count of 0 only drops it. */
+int32_t rdet_tree_accept(rdet_ctx* ctx, rdet_seq* const* seqs, size_t nseq, const uint32_t* path_counts,
+                         const uint32_t* path_nodes);
 
 /* ---- canonical bytes and commitments ----------------------------------------
  * rdet_read copies the canonical little-endian i32 values of a buffer into
@@ -238,7 +283,6 @@ int32_t rdet_det_attention_decode_noalloc(const int32_t* q, const int32_t* k_cac
  * their outputs and workspaces do not.  Their descriptor arrays are host
  * memory that is read before the call returns.  No counterpart in the
  * reference, which decodes one token at a time; the arithmetic is det_num v1's. */
-#define RDET_MAX_TREE_NODES 64
 typedef struct rdet_tree_seq {
   const int32_t* k_cache; /* device, [num_kv_heads, cap, head_dim]: rows [0, context) are attended */
   const int32_t* v_cache;
@@ -280,7 +324,6 @@ int32_t rdet_det_attention_tree(const rdet_tree_seq* seqs, uint32_t n_seqs, cons
  * history and bias ids outside the vocabulary are ignored.  parent: the row of
  * this call that holds the parent node (below the row's own index), -1: none;
  * token: the row's own drafted token, RDET_NO_TOKEN: none. */
-#define RDET_NO_TOKEN 0xffffffffu
 typedef struct rdet_logit_row {
   const int32_t* logits;       /* device, [vocab] */
   int32_t* out;                /* device, [vocab], or NULL */

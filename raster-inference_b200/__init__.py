@@ -36,7 +36,8 @@ SYMBOLS = [
     "rdet_open", "rdet_open_synthetic", "rdet_close", "rdet_get_model_info", "rdet_seq_new", "rdet_seq_free",
     "rdet_seq_position", "rdet_embed", "rdet_prefill", "rdet_prefill_begin", "rdet_prefill_range",
     "rdet_prefill_finalize", "rdet_select", "rdet_select_batch", "rdet_decode", "rdet_decode_begin", "rdet_decode_range",
-    "rdet_decode_finalize", "rdet_generate", "rdet_read", "rdet_commitment", "rdet_kv_prefix_commitments",
+    "rdet_decode_finalize", "rdet_generate", "rdet_select_rules", "rdet_tree_decode", "rdet_tree_select",
+    "rdet_tree_accept", "rdet_read", "rdet_commitment", "rdet_kv_prefix_commitments",
     "rdet_det_gemv", "rdet_det_linear",
     "rdet_det_attention_decode", "rdet_det_attention_decode_noalloc", "rdet_det_attention_prefill", "rdet_convert_to_wgt",
     "rdet_det_attention_tree_workspace", "rdet_det_attention_tree", "rdet_det_logits_rules", "rdet_det_tree_commit",
@@ -79,6 +80,13 @@ class LogitRow(C.Structure):
                 ("presence", C.c_int32), ("parent", C.c_int32), ("token", C.c_uint32)]
 
 
+class Rules(C.Structure):
+    """Rules of one sequence's selection (rdet_rules); pointers are host memory."""
+    _fields_ = [("allow", C.c_void_p), ("history", C.c_void_p), ("bias_ids", C.c_void_p),
+                ("bias_values", C.c_void_p), ("history_len", C.c_uint32), ("n_bias", C.c_uint32),
+                ("repetition", C.c_int32), ("frequency", C.c_int32), ("presence", C.c_int32)]
+
+
 class TreeMove(C.Structure):
     _fields_ = [("cache", C.c_void_p), ("draft", C.c_void_p), ("cap", C.c_uint32), ("draft_cap", C.c_uint32),
                 ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("context", C.c_uint32), ("path", C.c_uint32)]
@@ -117,6 +125,10 @@ def lib() -> C.CDLL:
         "rdet_decode_range": [p, p, u32, u32],
         "rdet_decode_finalize": [p, p],
         "rdet_generate": [p, p, u32, p],
+        "rdet_select_rules": [p, p, sz, p, p],
+        "rdet_tree_decode": [p, p, sz, p, p, p],
+        "rdet_tree_select": [p, p, sz, p, p],
+        "rdet_tree_accept": [p, p, sz, p, p],
         "rdet_read": [p, p, i32, i32, i32, p, sz, p],
         "rdet_commitment": [p, p, i32, i32, C.c_char_p],
         "rdet_kv_prefix_commitments": [p, p, C.c_uint32, C.c_char_p],
@@ -173,6 +185,7 @@ class Model:
         self.H, self.V, self.L = info.hidden_size, info.vocab_size, info.num_layers
         self.Hq, self.P, self.F = info.num_heads, info.ple_dim, info.intermediate_size
         self.weight_bytes = info.weight_bytes
+        self.max_prefill = 4096
 
     @classmethod
     def open(cls, model_dir: str, device: int = 0, max_prefill: int = 0, layer_commitments: bool = False,
@@ -183,7 +196,9 @@ class Model:
         _check(lib().rdet_open(model_dir.encode(), C.byref(opts), C.byref(h)))
         with open(os.path.join(model_dir, "config.json")) as f:
             cfg = json.load(f)
-        return cls(h, cfg)
+        model = cls(h, cfg)
+        model.max_prefill = max_prefill or model.max_prefill
+        return model
 
     @classmethod
     def synthetic(cls, config: dict, seed: int, width: int = 16, device: int = 0, max_prefill: int = 0,
@@ -192,7 +207,9 @@ class Model:
         opts = Opts(device, max_prefill, flags)
         h = C.c_void_p()
         _check(lib().rdet_open_synthetic(json.dumps(config).encode(), seed, width, C.byref(opts), C.byref(h)))
-        return cls(h, config)
+        model = cls(h, config)
+        model.max_prefill = max_prefill or model.max_prefill
+        return model
 
     def close(self):
         if getattr(self, "_h", None):
@@ -253,7 +270,9 @@ class Model:
     def new_sequence(self, max_ctx: int) -> "Sequence":
         h = C.c_void_p()
         _check(lib().rdet_seq_new(self._h, max_ctx, C.byref(h)))
-        return Sequence(self, h)
+        seq = Sequence(self, h)
+        seq.max_ctx = max_ctx
+        return seq
 
     def embed(self, ids) -> np.ndarray:
         ids = np.ascontiguousarray(ids, dtype=np.uint32)
@@ -382,6 +401,87 @@ def select_batch(model: Model, seqs) -> list[int]:
     out = np.zeros(max(n, 1), dtype=np.uint32)
     _check(lib().rdet_select_batch(model._h, arr, n, _ptr(out)))
     return [int(v) for v in out[:n]]
+
+
+# ---- drafted decoding ----------------------------------------------------------------
+def _handles(seqs):
+    return (C.c_void_p * max(len(seqs), 1))(*[s._h for s in seqs])
+
+
+def _rules(model, rules, masks):
+    """rdet_rules array from one dict per sequence (masks[i]: the allow masks
+    of sequence i), or None: allow (u32 words,
+    for tree_select one row per node), history (token ids), bias ({token id:
+    Q16.16 value}), repetition, frequency and presence (Q16.16); what a dict
+    leaves out is no rule of that kind.  The array keeps the memory it names."""
+    if rules is None:
+        return None
+    if len(rules) != len(masks):
+        raise ValueError("one dict of rules per sequence")
+    out = (Rules * max(len(rules), 1))()
+    out.keep = []
+    for o, r, n in zip(out, rules, masks):
+        unknown = set(r) - {"allow", "history", "bias", "repetition", "frequency", "presence"}
+        if unknown:
+            raise TypeError(f"unknown rules {sorted(unknown)}")
+        hist = np.ascontiguousarray(r.get("history", ()), dtype=np.uint32)
+        bias = r.get("bias", {})
+        ids = np.array(list(bias.keys()), dtype=np.uint32)
+        vals = np.array(list(bias.values()), dtype=np.int32)
+        if hist.ndim != 1:
+            raise ValueError("history: a list of token ids")
+        out.keep += [hist, ids, vals]
+        if r.get("allow") is not None:
+            allow = np.ascontiguousarray(r["allow"], dtype=np.uint32)
+            if allow.size != n * ((model.V + 31) // 32):
+                raise ValueError(f"allow: {n} masks of {(model.V + 31) // 32} words")
+            out.keep.append(allow)
+            o.allow = allow.ctypes.data
+        o.history, o.history_len = hist.ctypes.data, hist.size
+        o.bias_ids, o.bias_values, o.n_bias = ids.ctypes.data, vals.ctypes.data, ids.size
+        o.repetition = r.get("repetition", 1 << 16)
+        o.frequency, o.presence = r.get("frequency", 0), r.get("presence", 0)
+    return out
+
+
+def select_rules(model: Model, seqs, rules) -> list[int]:
+    """The greedy token of each sequence under its rules (rdet_select_rules);
+    NO_TOKEN where the mask allows none."""
+    out = np.zeros(max(len(seqs), 1), dtype=np.uint32)
+    _check(lib().rdet_select_rules(model._h, _handles(seqs), len(seqs), _rules(model, rules, [1] * len(seqs)), _ptr(out)))
+    return [int(v) for v in out[:len(seqs)]]
+
+
+def tree_decode(model: Model, seqs, tokens, parents):
+    """Every node of each sequence's drafted tree in one pass (rdet_tree_decode):
+    tokens[i] and parents[i] list sequence i's nodes."""
+    counts = np.array([len(t) for t in tokens], dtype=np.uint32)
+    if any(len(t) != len(q) for t, q in zip(tokens, parents)) or not len(seqs) == len(tokens) == len(parents):
+        raise ValueError("one list of tokens and one of parents per sequence, of the same length")
+    toks = np.array([t for row in tokens for t in row], dtype=np.uint32)
+    par = np.array([q for row in parents for q in row], dtype=np.int32)
+    _check(lib().rdet_tree_decode(model._h, _handles(seqs), len(seqs), _ptr(counts), _ptr(toks), _ptr(par)))
+    for s, t in zip(seqs, tokens):
+        s._tree = len(t)
+
+
+def tree_select(model: Model, seqs, rules=None) -> list[list[int]]:
+    """The greedy token after every node of each sequence's drafted tree
+    (rdet_tree_select), under rules when given."""
+    n = [getattr(s, "_tree", 0) for s in seqs]
+    out = np.zeros(max(sum(n), 1), dtype=np.uint32)
+    _check(lib().rdet_tree_select(model._h, _handles(seqs), len(seqs), _rules(model, rules, n), _ptr(out)))
+    at = np.cumsum([0] + n)
+    return [[int(v) for v in out[a:b]] for a, b in zip(at[:-1], at[1:])]
+
+
+def tree_accept(model: Model, seqs, paths):
+    """Commits one path of each sequence's drafted tree (rdet_tree_accept)."""
+    if len(paths) != len(seqs):
+        raise ValueError("one path per sequence")
+    counts = np.array([len(p) for p in paths], dtype=np.uint32)
+    nodes = np.array([n for p in paths for n in p] + [0], dtype=np.uint32)
+    _check(lib().rdet_tree_accept(model._h, _handles(seqs), len(seqs), _ptr(counts), _ptr(nodes)))
 
 
 # ---- reference-named entry points ---------------------------------------------------

@@ -1254,6 +1254,7 @@ __global__ void qkv_post_kernel(const QkvPostArgs a) {
   int32_t* const kcache = rows ? a.kc_rows[s] : a.k_cache;
   int32_t* const vcache = rows ? a.vc_rows[s] : a.v_cache;
   const int cap = rows ? a.cap_rows[s] : a.cap;
+  const uint32_t slot = a.slot_rows ? (uint32_t)a.slot_rows[s] : pos;
   const int h = head - a.Hq;
   // K: head norm + RoPE
   const int32_t* ks = a.k_in + (size_t)s * (a.ld ? a.ld : a.Hkv * d) + (size_t)h * d;
@@ -1265,7 +1266,7 @@ __global__ void qkv_post_kernel(const QkvPostArgs a) {
   if (a.rope_cs) rope_inplace_tab(vs, a.rotary, a.rope_cs + (size_t)s * a.rotary, pos);
   else rope_inplace(vs, a.rotary, a.inv_freq, pos);
   __syncthreads();
-  int32_t* kd = kcache + ((size_t)h * cap + pos) * d;
+  int32_t* kd = kcache + ((size_t)h * cap + slot) * d;
   for (int i = threadIdx.x; i < d; i += blockDim.x) kd[i] = vs[i];
   __syncthreads();
   // V: weightless value norm of the raw projection
@@ -1273,7 +1274,7 @@ __global__ void qkv_post_kernel(const QkvPostArgs a) {
   for (int i = threadIdx.x; i < d; i += blockDim.x) vs[i] = vsrc[i];
   __syncthreads();
   int32_t sv = block_norm_scale(vs, d, a.eps, red);
-  int32_t* vd = vcache + ((size_t)h * cap + pos) * d;
+  int32_t* vd = vcache + ((size_t)h * cap + slot) * d;
   for (int i = threadIdx.x; i < d; i += blockDim.x) vd[i] = mul_sat(vs[i], sv);
 }
 void launch_qkv_post(const QkvPostArgs& a, cudaStream_t s) {

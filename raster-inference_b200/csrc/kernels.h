@@ -219,6 +219,8 @@ struct QkvPostArgs {
   int32_t* const* kc_rows = nullptr;
   int32_t* const* vc_rows = nullptr;
   const int32_t* cap_rows = nullptr;
+  // drafted nodes: the cache row that row s is written to (nullptr: its position)
+  const int32_t* slot_rows = nullptr;
 };
 void launch_qkv_post(const QkvPostArgs& a, cudaStream_t s);
 // cs[p][i] = (cos, sin) of pos_angle(p, inv_freq[i]) for positions p in [0, S)

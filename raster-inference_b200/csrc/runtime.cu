@@ -580,6 +580,24 @@ struct Ctx {
     int32_t* logits = nullptr;     // [rows, V]
   } bw;
   TpState tp;
+  // drafted trees (rdet_tree_decode): one row per node of the last call
+  struct {
+    int rows = 0;                  // rows the buffers hold
+    uint64_t epoch = 0;            // tree decodes so far
+    int32_t* pos = nullptr;        // [rows] node positions, [rows] cache rows
+    int32_t* dec_out = nullptr;    // [rows][L, H] per-layer outputs
+    int32_t* logits = nullptr;     // [rows, V]
+    void* ws = nullptr;            // workspace of the tree attention
+    size_t ws_bytes = 0;
+  } tree;
+  // selection under rules: tokens (up to rows), the rules' arrays in pinned and device memory
+  struct {
+    uint32_t* tok = nullptr;
+    int rows = 0;
+    unsigned char* host = nullptr;
+    unsigned char* dev = nullptr;
+    size_t bytes = 0;
+  } rules;
   CommitPipe cp;
   KvStage kvs;
 
@@ -609,6 +627,7 @@ struct Ctx {
     for (cudaEvent_t e : kvs.ev)
       if (e) cudaEventDestroy(e);
     if (kvs.host) cudaFreeHost(kvs.host);
+    if (rules.host) cudaFreeHost(rules.host);
     for (void* p : tp.ipc_opened) cudaIpcCloseMemHandle(p);
     if (tp.comm) nccl_api().commDestroy(tp.comm);
     for (void* p : allocs) cudaFree(p);
@@ -649,6 +668,12 @@ struct Seq {
   // routine state
   int prefill_next = -1, prefill_S = 0;
   int32_t* prefill_cur = nullptr;
+  // drafted tree of the context's tree decode number tree_epoch, made at
+  // position tree_pos: its nodes' rows, parents and tokens
+  uint64_t tree_epoch = 0;
+  int tree_pos = -1, tree_row0 = 0;
+  std::vector<int32_t> tree_parents;
+  std::vector<uint32_t> tree_tokens;
   int decode_next = -1;
   int32_t* decode_cur = nullptr;
   cudaGraphExec_t graph = nullptr;  // one decode_transition for the token in d_token
@@ -1071,6 +1096,7 @@ static void prefill_begin(Ctx& c, Seq& q, const uint32_t* ids, size_t n) {
   CK(cudaMemsetAsync(q.d_pos, 0, 4, s));
   q.pos = 0;
   q.prefilled = false;
+  q.tree_parents.clear();
   launch_embed(w.ids, S, c.emb, c.emb_scale, w.x0, c.d_err, s);
   // RoPE factors of positions [0, S), once per distinct frequency table
   for (size_t t = 0; t < c.rope_list.size(); ++t)
@@ -1780,9 +1806,17 @@ static void kv_prefix_commitments(Ctx& c, Seq& q, int n, std::vector<std::string
 // each row's own position, caches and window.  Each row computes exactly
 // what decode_layer computes for that sequence alone.
 // ---------------------------------------------------------------------------
-static void batch_tables(Ctx& c, Seq* const* seqs, int B) {
+// One row of a batched pass: a sequence's next token, or a node of its drafted tree.
+struct BatchRow {
+  Seq* q;
+  int32_t* pos;      // device: the row's position
+  int32_t* dec_out;  // [L, H]
+  int32_t* logits;   // [V]
+};
+static void batch_tables(Ctx& c, const std::vector<BatchRow>& in) {
   const ModelCfg& m = c.cfg;
   auto& bw = c.bw;
+  const int B = (int)in.size();
   if (bw.rows < B) {
     const int rows = std::max(B, 8);
     const size_t ptrs = (size_t)rows * (4 + 2 * (size_t)m.L);
@@ -1806,10 +1840,10 @@ static void batch_tables(Ctx& c, Seq* const* seqs, int B) {
   bw.maps_ok = true;
   std::vector<int32_t> caps(2 * (size_t)rows, 0);  // [caps | row order]
   for (int b = 0; b < B; ++b) {
-    Seq& q = *seqs[b];
-    host[b] = q.d_pos;
-    host[rows + b] = q.dec_out;
-    host[2 * (size_t)rows + b] = q.logits;
+    const Seq& q = *in[b].q;
+    host[b] = in[b].pos;
+    host[rows + b] = in[b].dec_out;
+    host[2 * (size_t)rows + b] = in[b].logits;
     for (int l = 0; l < m.L; ++l) {
       const int own = m.layers[l].donor < 0 ? l : m.layers[l].donor;
       host[(3 + (size_t)l) * rows + b] = q.kc[own];
@@ -1822,9 +1856,56 @@ static void batch_tables(Ctx& c, Seq* const* seqs, int B) {
   // attention launch order: longest context first (ties by row)
   int32_t* order = caps.data() + rows;
   for (int b = 0; b < rows; ++b) order[b] = b;
-  std::stable_sort(order, order + B, [&](int32_t x, int32_t y) { return seqs[x]->pos > seqs[y]->pos; });
+  std::stable_sort(order, order + B, [&](int32_t x, int32_t y) { return in[x].q->pos > in[y].q->pos; });
   CK(cudaMemcpyAsync(bw.pos, host.data(), host.size() * 8, cudaMemcpyHostToDevice, c.stream));
   CK(cudaMemcpyAsync(bw.caps, caps.data(), caps.size() * 4, cudaMemcpyHostToDevice, c.stream));
+}
+static void batch_tables(Ctx& c, Seq* const* seqs, int B) {
+  std::vector<BatchRow> rows(B);
+  for (int b = 0; b < B; ++b) rows[b] = BatchRow{seqs[b], seqs[b]->d_pos, seqs[b]->dec_out, seqs[b]->logits};
+  batch_tables(c, rows);
+}
+
+// The drafted trees of one rdet_tree_decode: B batch rows, of which the first
+// `nodes` are nodes (the rest fill up to the tensor-core linear's least rows).
+struct TreeBatch {
+  int nodes = 0;
+  const int32_t* slots = nullptr;      // device: cache row of every node
+  std::vector<TreeGroup> groups;       // launch groups of the attention, without the layer's caches
+  std::vector<std::vector<Seq*>> seqs; // the sequences of each group
+};
+// The tree attention of layer l over `q`, the caches holding the nodes' rows
+// from each sequence's position on.
+static void tree_attention(Ctx& c, TreeBatch& tb, int l, const int32_t* q, int32_t* out) {
+  const LayerCfg& lc = c.cfg.layers[l];
+  const int own = lc.donor < 0 ? l : lc.donor, d = lc.head_dim;
+  size_t node = 0;
+  for (size_t i = 0; i < tb.groups.size(); ++i) {
+    TreeGroup& g = tb.groups[i];
+    g.Hq = c.cfg.Hq;
+    g.Hkv = lc.kv_heads;
+    g.d = d;
+    g.window = lc.window;
+    for (int j = 0; j < g.nseq; ++j) {
+      const Seq& s = *tb.seqs[i][j];
+      TreeSeq& t = g.seq[j];
+      t.k = s.kc[own];
+      t.v = s.vc[own];
+      t.kt = t.k + (size_t)t.ctx * d;
+      t.vt = t.v + (size_t)t.ctx * d;
+      t.kstride = t.tstride = (int64_t)s.cap * d;
+    }
+    const size_t need = tree_attn_plan(g);
+    if (c.tree.ws_bytes < need) {  // doubled, so that growing contexts replace it rarely
+      c.tree.ws_bytes = 2 * need;
+      c.tree.ws = c.dalloc(c.tree.ws_bytes);
+    }
+    g.q = q + node * c.cfg.Hq * d;
+    g.out = out + node * c.cfg.Hq * d;
+    g.ws = c.tree.ws;
+    launch_tree_attn(g, c.stream);
+    node += (size_t)g.nnode;
+  }
 }
 
 // in_planes: the layer input's norm already applied into w.nrm (and its
@@ -1833,7 +1914,8 @@ static void batch_tables(Ctx& c, Seq* const* seqs, int B) {
 // norm(output) * next_gain into w.nrm and its planes (the next layer's input
 // norm, or the final norm before lm_head), setting next_planes->ready.
 static const int32_t* decode_batch_layer(Ctx& c, int B, int maxcap, int l, int32_t* cur, ActPlanes* in_planes,
-                                         const int32_t* next_gain, ActPlanes* next_planes) {
+                                         const int32_t* next_gain, ActPlanes* next_planes,
+                                         TreeBatch* tb = nullptr) {
   const ModelCfg& m = c.cfg;
   const LayerDev& L = c.layers[l];
   const LayerCfg& lc = L.cfg;
@@ -1883,6 +1965,10 @@ static const int32_t* decode_batch_layer(Ctx& c, int B, int maxcap, int l, int32
       qa.vc_rows = bw.vc + (size_t)l * bw.rows;
     }
   }
+  if (tb) {
+    qa.S = tb->nodes;
+    qa.slot_rows = tb->slots;
+  }
   launch_qkv_post(qa, s);
   AttnDecodeArgs aa;
   aa.Hq = m.Hq; aa.Hkv = lc.kv_heads; aa.d = d; aa.window = lc.window; aa.q = w.qo; aa.out = w.comb;
@@ -1892,7 +1978,8 @@ static const int32_t* decode_batch_layer(Ctx& c, int B, int maxcap, int l, int32
   aa.row_order = bw.order;
   aa.map_rows = bw.maps_ok ? bw.maps : nullptr;
   aa.map_layer = lc.donor < 0 ? l : lc.donor;
-  launch_attn_decode_cluster(aa, s);
+  if (tb) tree_attention(c, *tb, l, w.qo, w.comb);
+  else launch_attn_decode_cluster(aa, s);
   prefill_linear(c, w.comb, B, L.o, L.to, w.attn, kEpiPlain, nullptr);
   const bool ple = m.P > 0;
   // post-attention norm + residual, then the MLP input norm (and its planes)
@@ -2285,15 +2372,14 @@ static bool batch_supported(Ctx& c, Seq* const* seqs, int B) {
   return true;
 }
 
-static void decode_batch(Ctx& c, Seq* const* seqs, const uint32_t* tokens, int B) {
+// The pass over the B rows that the batch tables describe: embedding, layers,
+// final norm and lm_head into each row's logits (the first `out_rows` of them).
+static void batch_pass(Ctx& c, const uint32_t* tokens, int B, int out_rows, int maxcap, TreeBatch* tb) {
   const ModelCfg& m = c.cfg;
   PrefillWs& w = c.pw;
   cudaStream_t s = c.stream;
-  batch_tables(c, seqs, B);
   batch_rope_tables(c, B);
   auto& bw = c.bw;
-  int maxcap = 0;
-  for (int i = 0; i < B; ++i) maxcap = std::max(maxcap, seqs[i]->cap);
   CK(cudaMemcpyAsync(bw.ids, tokens, (size_t)B * 4, cudaMemcpyHostToDevice, s));
   launch_embed(bw.ids, B, c.emb, c.emb_scale, w.xa, c.d_err, s);
   if (m.P > 0) {
@@ -2309,18 +2395,186 @@ static void decode_batch(Ctx& c, Seq* const* seqs, const uint32_t* tokens, int B
   for (int l = 0; l < m.L; ++l) {
     ActPlanes next;
     const int32_t* gain = l + 1 < m.L ? c.layers[l + 1].in_ln : c.final_norm;
-    cur = const_cast<int32_t*>(decode_batch_layer(c, B, maxcap, l, cur, &carry, gain, &next));
+    cur = const_cast<int32_t*>(decode_batch_layer(c, B, maxcap, l, cur, &carry, gain, &next, tb));
     carry = next;
   }
   if (!carry.normed) launch_rmsnorm_rows(cur, B, m.H, c.final_norm, c.eps, w.nrm, s);
   prefill_linear(c, w.nrm, B, c.lm_head, c.t_lm_head, bw.logits, kEpiPlain, nullptr, carry.ready ? &carry : nullptr);
-  launch_scatter_rows(bw.logits, B, m.V, bw.logits_dst, 0, s, m.has_softcap ? c.softcap : 0);
-  launch_add_i32_rows(bw.pos, B, 1, s);
+  launch_scatter_rows(bw.logits, out_rows, m.V, bw.logits_dst, 0, s, m.has_softcap ? c.softcap : 0);
+}
+
+static void decode_batch(Ctx& c, Seq* const* seqs, const uint32_t* tokens, int B) {
+  batch_tables(c, seqs, B);
+  int maxcap = 0;
+  for (int i = 0; i < B; ++i) maxcap = std::max(maxcap, seqs[i]->cap);
+  batch_pass(c, tokens, B, B, maxcap, nullptr);
+  launch_add_i32_rows(c.bw.pos, B, 1, c.stream);
   CK(cudaGetLastError());
   for (int i = 0; i < B; ++i) {
     seqs[i]->pos += 1;
     seqs[i]->last_was_prefill = false;
   }
+}
+
+// ---------------------------------------------------------------------------
+// Drafted trees: every node of every sequence's tree is one row of a batched
+// pass, its K/V written behind the committed rows of the caches.
+// ---------------------------------------------------------------------------
+static void tree_decode(Ctx& c, const std::vector<Seq*>& seqs, const uint32_t* counts, const uint32_t* tokens,
+                        const int32_t* parents) {
+  const ModelCfg& m = c.cfg;
+  int nodes = 0;
+  for (size_t i = 0; i < seqs.size(); ++i) nodes += (int)counts[i];
+  // with tensor cores, fill up to the rows from which the linears use them
+  const int B = c.tc && c.max_prefill >= (uint32_t)kTcMinRows ? std::max(nodes, kTcMinRows) : nodes;
+  auto& tr = c.tree;
+  if (tr.rows < B) {
+    const int rows = std::max(B, 64);
+    tr.pos = c.dalloc_n<int32_t>(2 * (size_t)rows);
+    tr.dec_out = c.dalloc_n<int32_t>((size_t)rows * m.L * m.H);
+    tr.logits = c.dalloc_n<int32_t>((size_t)rows * m.V);
+    tr.rows = rows;
+  }
+  TreeBatch tb;
+  tb.nodes = nodes;
+  tb.slots = tr.pos + tr.rows;
+  std::vector<int32_t> host(2 * (size_t)tr.rows, 0);  // [positions | cache rows]
+  std::vector<BatchRow> rows(B);
+  std::vector<uint32_t> ids(B, 0);
+  int maxcap = 0, row = 0;
+  for (size_t i = 0; i < seqs.size(); ++i) {
+    Seq& q = *seqs[i];
+    const int n = (int)counts[i];
+    if (tb.groups.empty() || tb.groups.back().nseq == kTreeGroupSeqs || tb.groups.back().nnode + n > kTreeGroupNodes) {
+      tb.groups.emplace_back();
+      tb.seqs.emplace_back();
+    }
+    TreeGroup& g = tb.groups.back();
+    TreeSeq& t = g.seq[g.nseq++];
+    tb.seqs.back().push_back(&q);
+    t.ctx = q.pos;
+    t.n = n;
+    t.node0 = g.nnode;
+    std::vector<int> depth(n);
+    for (int j = 0; j < n; ++j, ++row) {
+      const int p = parents[row];
+      depth[j] = p >= 0 ? depth[p] + 1 : 0;
+      g.mask[g.nnode + j] = (p >= 0 ? g.mask[g.nnode + p] : 0) | 1ull << j;
+      host[row] = q.pos + depth[j];
+      host[tr.rows + row] = q.pos + j;
+      rows[row] = BatchRow{&q, tr.pos + row, tr.dec_out + (size_t)row * m.L * m.H, tr.logits + (size_t)row * m.V};
+      ids[row] = tokens[row];
+    }
+    g.nnode += n;
+    maxcap = std::max(maxcap, q.cap);
+  }
+  for (int r = nodes; r < B; ++r)
+    rows[r] = BatchRow{seqs[0], tr.pos + r, tr.dec_out + (size_t)r * m.L * m.H, tr.logits + (size_t)r * m.V};
+  tr.epoch += 1;  // earlier trees' buffers are overwritten from here on
+  CK(cudaMemcpyAsync(tr.pos, host.data(), host.size() * 4, cudaMemcpyHostToDevice, c.stream));
+  batch_tables(c, rows);
+  batch_pass(c, ids.data(), B, nodes, maxcap, &tb);
+  CK(cudaGetLastError());
+  CK(cudaStreamSynchronize(c.stream));
+  check_err_flag(c, "tree decode");
+  row = 0;
+  for (size_t i = 0; i < seqs.size(); ++i) {
+    Seq& q = *seqs[i];
+    q.tree_epoch = tr.epoch;
+    q.tree_pos = q.pos;
+    q.tree_row0 = row;
+    q.tree_parents.assign(parents + row, parents + row + counts[i]);
+    q.tree_tokens.assign(tokens + row, tokens + row + counts[i]);
+    row += (int)counts[i];
+  }
+}
+
+// The sequence's drafted tree is that of the context's last tree decode and
+// the sequence has not moved since.
+static void require_tree(const Ctx& c, const Seq& q) {
+  REQUIRE(!q.tree_parents.empty() && q.tree_epoch == c.tree.epoch && q.tree_pos == q.pos, RDET_E_STATE,
+          "the sequence has no drafted tree (run rdet_tree_decode first; a later tree decode, prefill or decode drops it)");
+}
+
+// The rules of n sequences with their arrays in device memory; sequence i has
+// masks[i] allow masks.  Host memory is read before this returns.
+static std::vector<rdet_rules> stage_rules(Ctx& c, const rdet_rules* rules, size_t n, const std::vector<size_t>& masks) {
+  std::vector<rdet_rules> out;
+  if (!rules) return out;
+  const size_t words = ((size_t)c.cfg.V + 31) / 32;
+  size_t bytes = 0;
+  for (size_t i = 0; i < n; ++i) {
+    const rdet_rules& r = rules[i];
+    REQUIRE((r.history_len == 0 || r.history) && (r.n_bias == 0 || (r.bias_ids && r.bias_values)), RDET_E_INVALID,
+            "null rules array");
+    bytes += ((r.allow ? masks[i] * words : 0) + r.history_len + 2 * (size_t)r.n_bias) * 4;
+  }
+  auto& rs = c.rules;
+  if (rs.bytes < bytes) {
+    if (rs.host) CK(cudaFreeHost(rs.host));
+    rs.host = nullptr;
+    rs.bytes = 0;
+    const size_t grown = 2 * bytes;  // histories grow by a token a step
+    void* h = nullptr;
+    CK(cudaHostAlloc(&h, grown, cudaHostAllocDefault));
+    rs.host = static_cast<unsigned char*>(h);
+    rs.dev = static_cast<unsigned char*>(c.dalloc(grown));
+    rs.bytes = grown;
+  }
+  size_t at = 0;
+  auto put = [&](const void* src, size_t count) -> const void* {
+    if (!src || count == 0) return nullptr;
+    memcpy(rs.host + at, src, count * 4);
+    const void* dst = rs.dev + at;
+    at += count * 4;
+    return dst;
+  };
+  for (size_t i = 0; i < n; ++i) {
+    rdet_rules r = rules[i];
+    r.allow = static_cast<const uint32_t*>(put(r.allow, masks[i] * words));
+    r.history = static_cast<const uint32_t*>(put(r.history, r.history_len));
+    r.bias_ids = static_cast<const uint32_t*>(put(r.bias_ids, r.n_bias));
+    r.bias_values = static_cast<const int32_t*>(put(r.bias_values, r.n_bias));
+    out.push_back(r);
+  }
+  if (at) CK(cudaMemcpyAsync(rs.dev, rs.host, at, cudaMemcpyHostToDevice, c.stream));
+  return out;
+}
+// One logit row under staged rules r (nullptr: none), whose mask is r's mask-th.
+static rdet_logit_row rules_row(const Ctx& c, const rdet_rules* r, const int32_t* logits, size_t mask) {
+  rdet_logit_row o{};
+  o.logits = logits;
+  o.repetition = kOneAct;
+  o.parent = -1;
+  o.token = RDET_NO_TOKEN;
+  if (!r) return o;
+  o.allow = r->allow ? r->allow + mask * (((size_t)c.cfg.V + 31) / 32) : nullptr;
+  o.history = r->history;
+  o.history_len = r->history_len;
+  o.bias_ids = r->bias_ids;
+  o.bias_values = r->bias_values;
+  o.n_bias = r->n_bias;
+  o.repetition = r->repetition;
+  o.frequency = r->frequency;
+  o.presence = r->presence;
+  return o;
+}
+// Greedy tokens of `rows` under their rules into host memory.
+static void select_under_rules(Ctx& c, const std::vector<rdet_logit_row>& rows, uint32_t* tokens_out) {
+  const int n = (int)rows.size();
+  if (n == 0) return;
+  if (c.rules.rows < n) {
+    const int cap = std::max(n, 64);
+    c.rules.tok = c.dalloc_n<uint32_t>((size_t)cap);
+    c.rules.rows = cap;
+  }
+  const int32_t rc = rdet_det_logits_rules(rows.data(), (uint32_t)n, (uint32_t)c.cfg.V, c.rules.tok, c.stream);
+  if (rc != RDET_OK) {
+    CK(cudaStreamSynchronize(c.stream));  // the staged rules may still be copied from
+    throw Fail{rc, g_last_error};
+  }
+  CK(cudaMemcpyAsync(tokens_out, c.rules.tok, (size_t)n * 4, cudaMemcpyDeviceToHost, c.stream));
+  CK(cudaStreamSynchronize(c.stream));
 }
 
 static void ensure_decode_graph(Ctx& c, Seq& q) {
@@ -2825,6 +3079,7 @@ int32_t rdet_decode_begin(rdet_ctx* ctx, rdet_seq* seq, uint32_t token) {
     CK(cudaMemcpyAsync(q.d_token, &token, 4, cudaMemcpyHostToDevice, c.stream));
     decode_embed(c, q, q.d_token);
     CK(cudaGetLastError());
+    q.tree_parents.clear();  // its layers overwrite the drafted rows
     q.decode_next = 0;
     q.decode_cur = c.dw.x0;
     c.decode_owner = &q;
@@ -2945,6 +3200,146 @@ int32_t rdet_generate(rdet_ctx* ctx, rdet_seq* seq, uint32_t n_tokens, uint32_t*
     check_err_flag(c, "generate");
     q.pos += (int)n_tokens;
     q.last_was_prefill = false;
+  });
+}
+
+int32_t rdet_select_rules(rdet_ctx* ctx, rdet_seq* const* seqs, size_t n, const rdet_rules* rules,
+                          uint32_t* tokens_out) {
+  return guard([&] {
+    REQUIRE(ctx && (n == 0 || (seqs && tokens_out)), RDET_E_INVALID, "null argument");
+    REQUIRE(n <= (1u << 20), RDET_E_RANGE, "at most 2^20 sequences per call");
+    Ctx& c = *ctx->c;
+    CK(cudaSetDevice(c.device));
+    for (size_t i = 0; i < n; ++i) {
+      REQUIRE(seqs[i] && seqs[i]->owner == ctx, RDET_E_INVALID, "sequence belongs to another context");
+      require_logits(*seqs[i]->s);
+    }
+    const std::vector<rdet_rules> staged = stage_rules(c, rules, n, std::vector<size_t>(n, 1));
+    std::vector<rdet_logit_row> rows;
+    for (size_t i = 0; i < n; ++i) rows.push_back(rules_row(c, rules ? &staged[i] : nullptr, seqs[i]->s->logits, 0));
+    select_under_rules(c, rows, tokens_out);
+  });
+}
+
+int32_t rdet_tree_decode(rdet_ctx* ctx, rdet_seq* const* seqs, size_t nseq, const uint32_t* counts,
+                         const uint32_t* tokens, const int32_t* parents) {
+  return guard([&] {
+    REQUIRE(ctx && (nseq == 0 || (seqs && counts && tokens && parents)), RDET_E_INVALID, "null argument");
+    Ctx& c = *ctx->c;
+    CK(cudaSetDevice(c.device));
+    REQUIRE(c.decode_owner == nullptr, RDET_E_STATE, "a routine-granular decode is in flight on this context");
+    REQUIRE(!c.tp.comm, RDET_E_STATE, "drafted trees are not sharded over tensor-parallel ranks");
+    std::vector<Seq*> batch(nseq);
+    size_t row = 0;
+    for (size_t i = 0; i < nseq; ++i) {
+      REQUIRE(seqs[i] && seqs[i]->owner == ctx, RDET_E_INVALID, "sequence belongs to another context");
+      Seq& q = *(batch[i] = seqs[i]->s.get());
+      for (size_t j = 0; j < i; ++j) REQUIRE(batch[j] != &q, RDET_E_INVALID, "a sequence is listed twice");
+      check_decode_ready(c, q);
+      REQUIRE(counts[i] >= 1 && counts[i] <= RDET_MAX_TREE_NODES, RDET_E_RANGE, "a tree has between 1 and 64 nodes");
+      REQUIRE(q.pos + (int)counts[i] <= q.cap, RDET_E_RANGE, "the drafted nodes would overflow the sequence KV cache");
+      for (const LayerCfg& lc : c.cfg.layers) {
+        REQUIRE(lc.head_dim <= 512, RDET_E_RANGE, "drafted trees need head dims of at most 512");
+        REQUIRE((lc.window > 0 ? std::min(q.pos, lc.window) : q.pos) + (int)counts[i] <= kTreeMaxKeys, RDET_E_RANGE,
+                "a drafted tree attends at most 523264 rows");
+      }
+      for (uint32_t j = 0; j < counts[i]; ++j, ++row) {
+        REQUIRE(parents[row] >= -1 && parents[row] < (int32_t)j, RDET_E_INVALID,
+                "a node's parent must come before it (-1: none)");
+        check_token(c, tokens[row]);
+      }
+      REQUIRE(row <= c.max_prefill, RDET_E_RANGE, "more nodes than the context's max_prefill");
+    }
+    if (nseq == 0) return;
+    tree_decode(c, batch, counts, tokens, parents);
+  });
+}
+
+int32_t rdet_tree_select(rdet_ctx* ctx, rdet_seq* const* seqs, size_t nseq, const rdet_rules* rules,
+                         uint32_t* tokens_out) {
+  return guard([&] {
+    REQUIRE(ctx && (nseq == 0 || (seqs && tokens_out)), RDET_E_INVALID, "null argument");
+    Ctx& c = *ctx->c;
+    CK(cudaSetDevice(c.device));
+    std::vector<size_t> nodes(nseq);
+    for (size_t i = 0; i < nseq; ++i) {
+      REQUIRE(seqs[i] && seqs[i]->owner == ctx, RDET_E_INVALID, "sequence belongs to another context");
+      require_tree(c, *seqs[i]->s);
+      nodes[i] = seqs[i]->s->tree_parents.size();
+    }
+    const std::vector<rdet_rules> staged = stage_rules(c, rules, nseq, nodes);
+    std::vector<rdet_logit_row> rows;
+    for (size_t i = 0; i < nseq; ++i) {
+      const Seq& q = *seqs[i]->s;
+      const int32_t first = (int32_t)rows.size();
+      for (size_t j = 0; j < nodes[i]; ++j) {
+        rows.push_back(rules_row(c, rules ? &staged[i] : nullptr, c.tree.logits + (q.tree_row0 + j) * c.cfg.V, j));
+        rows.back().parent = q.tree_parents[j] >= 0 ? first + q.tree_parents[j] : -1;
+        if (rules) rows.back().token = q.tree_tokens[j];
+      }
+    }
+    select_under_rules(c, rows, tokens_out);
+  });
+}
+
+int32_t rdet_tree_accept(rdet_ctx* ctx, rdet_seq* const* seqs, size_t nseq, const uint32_t* path_counts,
+                         const uint32_t* path_nodes) {
+  return guard([&] {
+    REQUIRE(ctx && (nseq == 0 || (seqs && path_counts)), RDET_E_INVALID, "null argument");
+    Ctx& c = *ctx->c;
+    const ModelCfg& m = c.cfg;
+    CK(cudaSetDevice(c.device));
+    std::vector<rdet_tree_move> moves;
+    std::vector<uint32_t> off{0};
+    for (size_t i = 0; i < nseq; ++i) {
+      REQUIRE(seqs[i] && seqs[i]->owner == ctx, RDET_E_INVALID, "sequence belongs to another context");
+      for (size_t j = 0; j < i; ++j) REQUIRE(seqs[j] != seqs[i], RDET_E_INVALID, "a sequence is listed twice");
+      const Seq& q = *seqs[i]->s;
+      require_tree(c, q);
+      REQUIRE(path_counts[i] <= q.tree_parents.size() && (path_counts[i] == 0 || path_nodes), RDET_E_INVALID,
+              "a path is longer than its tree");
+      bool moved = false;  // some accepted row is not in its place yet
+      for (uint32_t k = 0; k < path_counts[i]; ++k) {
+        const uint32_t node = path_nodes[off.back() + k];
+        REQUIRE(node < q.tree_parents.size() &&
+                    q.tree_parents[node] == (k == 0 ? -1 : (int32_t)path_nodes[off.back() + k - 1]),
+                RDET_E_INVALID, "a path starts at a root and every node's parent is the node before it");
+        moved = moved || node != k;
+      }
+      if (moved)
+        for (int l = 0; l < m.L; ++l) {
+          const LayerCfg& lc = m.layers[l];
+          if (lc.donor >= 0) continue;
+          for (int32_t* base : {q.kc[l], q.vc[l]})
+            moves.push_back(rdet_tree_move{base, base + (size_t)q.pos * lc.head_dim, (uint32_t)q.cap, (uint32_t)q.cap,
+                                           (uint32_t)lc.kv_heads, (uint32_t)lc.head_dim, (uint32_t)q.pos, (uint32_t)i});
+        }
+      off.push_back(off.back() + path_counts[i]);
+    }
+    if (!moves.empty()) {
+      const int32_t rc = rdet_det_tree_commit(moves.data(), (uint32_t)moves.size(), path_nodes, off.data(),
+                                              (uint32_t)nseq, c.stream);
+      if (rc != RDET_OK) throw Fail{rc, g_last_error};
+    }
+    for (size_t i = 0; i < nseq; ++i) {
+      Seq& q = *seqs[i]->s;
+      const uint32_t n = path_counts[i];
+      if (n > 0) {
+        // the state that decoding the path's tokens one by one leaves
+        const size_t row = (size_t)q.tree_row0 + path_nodes[off[i] + n - 1];
+        CK(cudaMemcpyAsync(q.logits, c.tree.logits + row * m.V, (size_t)m.V * 4, cudaMemcpyDeviceToDevice, c.stream));
+        CK(cudaMemcpyAsync(q.dec_out, c.tree.dec_out + row * m.L * m.H, (size_t)m.L * m.H * 4, cudaMemcpyDeviceToDevice,
+                           c.stream));
+        launch_add_i32(q.d_pos, (int32_t)n, c.stream);
+        q.pos += (int)n;
+        q.last_was_prefill = false;
+        q.logits_sharded = false;
+      }
+      q.tree_parents.clear();
+      q.tree_tokens.clear();
+    }
+    CK(cudaGetLastError());
+    CK(cudaStreamSynchronize(c.stream));
   });
 }
 
