@@ -65,8 +65,9 @@ constexpr int kTrPlane = 128 * 64;     // one digit plane of a stage: 128 rows o
 constexpr int kTrPlanes = 4 * kTrPlane;
 constexpr int kTrConv = 512;           // converter threads (warps 0-15)
 constexpr int kTrConvWarps = kTrConv / 32;
-constexpr int kQkThreads = 672;        // + warps 16-19 drain the accumulators, warp 20 issues the MMAs
+constexpr int kQkThreads = 736;        // + warps 16-19 drain, warp 20 issues the MMAs, warps 21-22 load
 constexpr int kQkDrainWarps = 20;      // warps 0-19
+constexpr int kTrLoaders = 64;         // loading threads
 constexpr int kPvThreads = 544;        // + warp 16 issues the MMAs
 constexpr int kTrMaxDigit = 0x7f7f7f7f;
 constexpr int kTrSplitKeys = 32704;    // keys of one value CTA at most: 3 * 2^14 each in s32
@@ -188,6 +189,32 @@ __device__ __forceinline__ void ld4(uint32_t& v, const void* p, bool on) {
                : "+r"(v)
                : "l"(p), "r"((int)on));
 }
+// kind::i8 MMA with operand A in TMEM (128 lanes, four K bytes a column)
+__device__ __forceinline__ void ta_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::i8 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void ta_st4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
+}
+__device__ __forceinline__ void ta_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+constexpr int kTrA = 448;  // TMEM column of operand A's two buffers of 32 columns
+
+// asynchronous copies into shared memory, zeros where `on` is false, and their
+// arrival on a barrier once all of the thread's copies so far are there
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(on ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(su32(bar)) : "memory");
+}
+__device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // four dims from `dim` on of a row of d: 16 bytes where every row is 16-byte
 // aligned, else one value at a time; what lies past the head is left alone
 template <bool VEC>
@@ -238,11 +265,20 @@ __device__ __forceinline__ int64_t shift_sum(int64_t add, int32_t c0, int32_t c1
 // ---------------------------------------------------------------------------
 // scores
 // ---------------------------------------------------------------------------
-// plane buffers between the converters and the MMAs
+// A stage is 64 dims of a tile's 128 keys, 32 KB as they are in a ring of slots
+// in shared memory (16-byte piece c of key k at c ^ (k & 7), so that 32 keys'
+// pieces are read without bank conflicts).  The key bytes go to the MMAs
+// through TMEM, operand A lying there: written to shared memory and read back
+// by the MMAs they made its bandwidth the bound (1550 cycles a stage at 64 rows,
+// of which the MMAs take 1024).  Two buffers of 32 dims, eight columns a byte.
+constexpr int kQkMaxStages = 6;
+constexpr int kSmemMost = 232448;  // a CTA's shared memory
 template <int NR>
-__host__ __device__ constexpr int qk_stages() { return NR == 64 ? 3 : 4; }
+struct QkRows;
 template <int NR>
-__host__ __device__ constexpr int qk_smem(int ns) { return qk_stages<NR>() * kTrPlanes + ns * 4 * NR * 64 + 1024; }
+__host__ __device__ constexpr int qk_stages(int ns);
+template <int NR>
+__host__ __device__ constexpr int qk_smem(int ns) { return qk_stages<NR>(ns) * kTrPlanes + ns * 4 * NR * 64 + 512; }
 
 // what draining a tile needs, per row of the block
 template <int NR>
@@ -255,30 +291,49 @@ struct QkRows {
   int32_t* sc;             // scores of the block's row 0
   int32_t pad, nr, ctx, lo, len, maxstart;
 };
+template <int NR>
+struct QkShared {
+  uint64_t raw_full[kQkMaxStages], raw_empty[kQkMaxStages], a_full[2], a_empty[2], acc_full[2], acc_empty[2], last_full;
+  uint32_t tmem;
+  int fail;
+  QkRows<NR> rows;
+};
+template <int NR>
+__host__ __device__ constexpr int qk_stages(int ns) {
+  const int n = (kSmemMost - 512 - (int)sizeof(QkShared<NR>) - ns * 4 * NR * 64) / kTrPlanes;
+  return n < kQkMaxStages ? n : kQkMaxStages;
+}
 // Scores of the row quads quad, quad + step, .. of a tile from TMEM (this
 // lane's key is j, the tile's first one j0), and each row's largest one.
 template <int NR>
 __device__ __noinline__ void qk_drain(QkRows<NR>& c, uint32_t taddr, int j0, int quad, int step) {
   const int lane = threadIdx.x & 31, j = j0 + 32 * ((threadIdx.x >> 5) & 3) + lane, key = c.lo + j;
   const bool in = j < c.len, all = c.lo + j0 >= c.maxstart && c.lo + j0 + kTrKeys <= c.ctx;  // every row attends every key
+  const int nr = c.nr;
   int32_t* out = c.sc + (int64_t)(4 * quad) * c.pad + j;
-  for (int r = 4 * quad; r < c.nr; r += 4 * step, out += 4 * (int64_t)step * c.pad) {
+  for (int r = 4 * quad; r < nr; r += 4 * step, out += 4 * (int64_t)step * c.pad) {
     int32_t v[7][4];
 #pragma unroll
     for (int b = 0; b < 7; ++b) ta_ld4(taddr + b * NR + r, v[b]);
     tmem_wait_ld();
+    uint32_t top[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int32_t s = requantize(shift_sum(c.corr[r + i], v[0][i], v[1][i], v[2][i], v[3][i], v[4][i], v[5][i], v[6][i]));
-      bool vis = in && r + i < c.nr;
-      if (vis) out[(int64_t)i * c.pad] = s;
-      if (!all) {
-        const int n = key - c.ctx;
-        vis = vis && (n < 0 ? key >= c.start[r + i] : (c.mask[r + i] >> n & 1) && c.npos[n] >= c.start[r + i]);
-      }
-      const uint32_t top = __reduce_max_sync(0xffffffffu, vis ? (uint32_t)s ^ 0x80000000u : 0u);
-      if (lane == 0) atomicMax(&c.top[r + i], top);
+      if (in && r + i < nr) out[(int64_t)i * c.pad] = s;
+      top[i] = (uint32_t)s ^ 0x80000000u;
     }
+    if (!all) {
+      const int n = key - c.ctx;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool vis = in && (n < 0 ? key >= c.start[r + i] : (c.mask[r + i] >> n & 1) && c.npos[n] >= c.start[r + i]);
+        if (!vis) top[i] = 0;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top[i] = __reduce_max_sync(0xffffffffu, top[i]);
+    if (lane < 4) atomicMax(&c.top[r + lane], lane < 2 ? (lane == 0 ? top[0] : top[1]) : (lane == 2 ? top[2] : top[3]));
   }
 }
 // The same by direct wrapping sums, for a block with a query value outside
@@ -306,24 +361,20 @@ __device__ __noinline__ void qk_drain_direct(QkRows<NR>& c, const int32_t* k, co
 
 template <int NR, bool VEC>
 __global__ void __launch_bounds__(kQkThreads, 1) tree_qk(const __grid_constant__ TreeGroup g) {
-  constexpr int kCols = 7 * NR, kTmem = NR == 16 ? 256 : 512;
+  constexpr int kCols = 7 * NR;
   constexpr int kBuf = NR == 64 ? 1 : 2;        // accumulator buffers in TMEM
   constexpr int na = 4;                         // query digits
   extern __shared__ __align__(16) unsigned char tr_raw[];
-  unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(tr_raw) + 1023) & ~(uintptr_t)1023);
-  constexpr int kSt = qk_stages<NR>();
-  unsigned char* planes = sm;                   // [kSt][4 bytes][128 keys][64 B]
-  unsigned char* qpl = sm + kSt * kTrPlanes;    // [chunk][4 NR rows][64 B]
-  __shared__ __align__(8) uint64_t planes_full[kSt], mma_done[kSt], acc_full[2], acc_empty[2], last_full;
-  __shared__ uint32_t tmem_holder;
-  __shared__ int s_fail;
-  __shared__ QkRows<NR> s_rows;
+  unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(tr_raw) + 511) & ~(uintptr_t)511);
+  __shared__ __align__(16) QkShared<NR> sh;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   // item -> sequence, KV head, row block, key tiles [t0, t1)
   const int si = seq_of(g.qk_first, g.nseq, blockIdx.x);
   const TreeSeq t = g.seq[si];
-  const int d = g.d, ns = (d + 63) / 64, G = g.G, Hq = g.Hq;
+  const int d = g.d, ns = (d + 63) / 64, G = g.G, Hq = g.Hq, nst = qk_stages<NR>(ns);
+  unsigned char* const slots = sm;                    // [nst][128 keys]
+  unsigned char* const qpl = sm + nst * kTrPlanes;    // [chunk][4 NR rows][64 B]
   const int rows = t.n * G, nrb = (rows + NR - 1) / NR, tiles = (t.len + kTrKeys - 1) / kTrKeys, qt = g.qk_tiles;
   const int it = blockIdx.x - g.qk_first[si];
   const int blk = it / t.qk_per, part = it - blk * t.qk_per, t0 = part * qt, t1 = min(tiles, t0 + qt);
@@ -333,210 +384,223 @@ __global__ void __launch_bounds__(kQkThreads, 1) tree_qk(const __grid_constant__
   const int32_t* const kc = t.k + (int64_t)kvh * t.kstride;
   const int32_t* const kt = t.kt + (int64_t)kvh * t.tstride;
   const int32_t* const qb = g.q + ((int64_t)t.node0 * Hq + kvh * G) * d;
-  ta_wait();
-  ta_go();
-
-  // a converter thread's part of stage (tile, s): keys 8 warp + 2 i + lane / 16,
-  // dims 64 s + 4 (lane % 16) ..  Keys past the sequence read its last key and
-  // dims past the head keep what the registers held: the first give scores
-  // that nothing reads, the second meet zero query digits.
-  const uint32_t lkey = 8 * warp + (lane >> 4), off0 = (lkey * (uint32_t)d + 4 * (lane & 15)) * 4, step = 8 * (uint32_t)d;
-  const int last_key = t.lo + t.len - 1;
-  uint4 x[2][4] = {};  // two stages in flight
-  int lt = 0, ls = 0;  // next stage to load
-  auto next = [&](uint4 (&y)[4]) {
-    const int key0 = t.lo + (t0 + lt) * kTrKeys;
-    const unsigned char* p[4];
-    if (key0 + kTrKeys <= t.ctx) {  // cache rows only
-      const unsigned char* base = reinterpret_cast<const unsigned char*>(kc + (int64_t)key0 * d + ls * 64);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = base + (off0 + i * step);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = min(key0 + (int)lkey + 2 * i, last_key);
-        p[i] = reinterpret_cast<const unsigned char*>((key < t.ctx ? kc + (int64_t)key * d : kt + (int64_t)(key - t.ctx) * d) +
-                                                      ls * 64 + 4 * (lane & 15));
-      }
-    }
-    const int dim = ls * 64 + 4 * (lane & 15);
-    const bool on = lt < t1 - t0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) load4<VEC>(y[i], reinterpret_cast<const int32_t*>(p[i]) - dim, dim, d, on);
-    if (++ls == ns) { ls = 0; ++lt; }
-  };
-  if (warp < kTrConvWarps) {
-    next(x[0]);
-    next(x[1]);
-  }
-
+  const int last_key = t.lo + t.len - 1, last_tile = t1 - t0 - 1;
   if (tid == 0) {
-    for (int i = 0; i < kSt; ++i) {
-      mbar_init(&planes_full[i], kTrConvWarps);
-      mbar_init(&mma_done[i], 1);
+    for (int i = 0; i < nst; ++i) {
+      mbar_init(&sh.raw_full[i], kTrLoaders);
+      mbar_init(&sh.raw_empty[i], kTrConvWarps);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], kBuf == 1 ? kQkDrainWarps : 4);
+      mbar_init(&sh.a_full[i], kTrConvWarps / 2);
+      mbar_init(&sh.a_empty[i], 1);
+      mbar_init(&sh.acc_full[i], 1);
+      mbar_init(&sh.acc_empty[i], kBuf == 1 ? kQkDrainWarps : 4);
     }
-    mbar_init(&last_full, 1);
+    mbar_init(&sh.last_full, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    s_fail = 0;
-    s_rows.sc = static_cast<int32_t*>(g.ws) + t.soff + ((int64_t)kvh * rows + r0) * t.pad;
-    s_rows.pad = t.pad;
-    s_rows.nr = nr;
-    s_rows.ctx = t.ctx;
-    s_rows.lo = t.lo;
-    s_rows.len = t.len;
+    sh.fail = 0;
+    sh.rows.sc = static_cast<int32_t*>(g.ws) + t.soff + ((int64_t)kvh * rows + r0) * t.pad;
+    sh.rows.pad = t.pad;
+    sh.rows.nr = nr;
+    sh.rows.ctx = t.ctx;
+    sh.rows.lo = t.lo;
+    sh.rows.len = t.len;
     // (no row's window begins later than that of a node at the tree's greatest possible depth)
-    s_rows.maxstart = g.window > 0 ? max(0, t.ctx + t.n - g.window) : 0;
+    sh.rows.maxstart = g.window > 0 ? max(0, t.ctx + t.n - g.window) : 0;
   }
-  if (tid < t.n) s_rows.npos[tid] = t.ctx + __popcll(g.mask[t.node0 + tid]) - 1;
-  if (warp == 20) ta_alloc<kTmem>(&tmem_holder);
-  auto wait = [&](uint64_t* bar, uint32_t parity) {
-    if (!ta_mbar_wait(bar, parity)) s_fail = 1;
-  };
+  if (tid < t.n) sh.rows.npos[tid] = t.ctx + __popcll(g.mask[t.node0 + tid]) - 1;
+  if (warp == 20) ta_alloc<512>(&sh.tmem);
   if (tid < NR) {
     const uint64_t m = tid < nr ? g.mask[t.node0 + (r0 + tid) / G] : 0;
-    s_rows.mask[tid] = m;
-    s_rows.start[tid] = tid < nr ? first_pos(g, t, m) : 0;
-    s_rows.top[tid] = 0;
+    sh.rows.mask[tid] = m;
+    sh.rows.start[tid] = tid < nr ? first_pos(g, t, m) : 0;
+    sh.rows.top[tid] = 0;
   }
-  // query digits: chunk s holds dims [64 s, 64 s + 64) of rows a * NR + r; two
-  // rows per warp and step, 16-byte pieces lane + 32 i of each
-  int32_t qmax = INT32_MIN;
-  auto qrow = [&](int r) {  // node * G + head of the group
-    const int rr = r0 + min(r, nr - 1), node = rr / G;
-    return qb + ((int64_t)node * Hq + (rr - node * G)) * d;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (!ta_mbar_wait(bar, parity)) sh.fail = 1;
   };
-#pragma unroll 1
-  for (int rp = 2 * warp; rp < NR; rp += kQkThreads / 16) {
-    uint4 v[2][4] = {};
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int32_t* q = qrow(rp + h);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) load4<VEC>(v[h][i], q, 4 * (lane + 32 * i), d, rp + h < nr);
+
+  // Stage u into its slot.  Keys past the sequence and dims past the head are zero.
+  int lt = t0, ls = 0, lb = 0, lph = 1;  // next stage's tile, chunk, slot and the parity of the slot's last use
+  auto load = [&]() {
+    const uint32_t slot = su32(slots) + lb * kTrPlanes;
+    const int key0 = t.lo + lt * kTrKeys, p = tid & (kTrLoaders - 1);
+    if (VEC) {  // 16 bytes of keys p / 16, p / 16 + 4, ..
+      const int dim = ls * 64 + 4 * (p & 15), row0 = p >> 4;
+      const bool on = dim < d;
+      const uint32_t dst0 = slot + row0 * 256 + 16 * ((p & 15) ^ row0), dst1 = dst0 ^ 64;  // even, odd i: bit 2 of the row
+      const int od = on ? dim : 0;
+      if (key0 + kTrKeys <= t.ctx) {  // cache rows only
+        const int32_t* src = kc + (int64_t)(key0 + row0) * d + od;
+#pragma unroll 8
+        for (int i = 0; i < 32; ++i) cp16((i & 1 ? dst1 : dst0) + i * 1024, src + (int64_t)i * (4 * d), on);
+      } else {
+        for (int i = 0; i < 32; ++i) {
+          const int key = min(key0 + row0 + 4 * i, last_key);
+          cp16((i & 1 ? dst1 : dst0) + i * 1024, (key < t.ctx ? kc + (int64_t)key * d : kt + (int64_t)(key - t.ctx) * d) + od,
+               on && key0 + row0 + 4 * i <= last_key);
+        }
+      }
+    } else {  // one dim of every key
+      const int dim = ls * 64 + p, od = min(dim, d - 1);
+      for (int i = 0; i < kTrKeys; ++i) {
+        const int key = min(key0 + i, last_key);
+        cp4(slot + i * 256 + 16 * ((p >> 2) ^ (i & 7)) + 4 * (p & 3), (key < t.ctx ? kc + (int64_t)key * d : kt + (int64_t)(key - t.ctx) * d) + od,
+            dim < d && key0 + i <= last_key);
+      }
     }
+    cp_arrive(&sh.raw_full[lb]);
+    if (++ls == ns) { ls = 0; ++lt; }
+    if (++lb == nst) { lb = 0; lph ^= 1; }
+  };
+  ta_wait();
+  ta_go();
+  __syncthreads();  // the barriers are there
+  int32_t qmax = INT32_MIN;
+  if (warp > 20) {
+    for (int u = 0; u < min(nst, total); ++u) load();
+  } else {
+    // query digits: chunk s holds dims [64 s, 64 s + 64) of rows a * NR + r; a
+    // half warp takes a row, 16 bytes a lane and chunk
+    const int half = lane >> 4, l16 = lane & 15;
+#pragma unroll 1
+    for (int rp = 2 * warp; rp < NR; rp += 42) {
+      const int r = rp + half, rr = r0 + min(r, nr - 1), node = rr / G;
+      const int32_t* q = qb + ((int64_t)node * Hq + (rr - node * G)) * d;
+      uint4 v[8] = {};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+      for (int s = 0; s < 8; ++s)
+        if (s < ns) load4<VEC>(v[s], q, 64 * s + 4 * l16, d, r < nr);
       int64_t sum = 0;
+      unsigned char* const dst = qpl + ta_sw(r, l16 >> 2) + 4 * (l16 & 3);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int dg = lane + 32 * i;
-        sum += (int64_t)(int32_t)v[h][i].x + (int32_t)v[h][i].y + (int32_t)v[h][i].z + (int32_t)v[h][i].w;
-        if (dg >= ns * 16) continue;
-        uint32_t o[4];
-        ta_t4(ta_digits((int32_t)v[h][i].x), ta_digits((int32_t)v[h][i].y), ta_digits((int32_t)v[h][i].z),
-              ta_digits((int32_t)v[h][i].w), o);
-        qmax = max4(qmax, v[h][i]);
+      for (int s = 0; s < 8; ++s) {
+        if (s < ns) {
+          sum += (int64_t)(int32_t)v[s].x + (int32_t)v[s].y + (int32_t)v[s].z + (int32_t)v[s].w;
+          qmax = max4(qmax, v[s]);
+          uint32_t o[4];
+          ta_t4(ta_digits((int32_t)v[s].x), ta_digits((int32_t)v[s].y), ta_digits((int32_t)v[s].z),
+                ta_digits((int32_t)v[s].w), o);
 #pragma unroll
-        for (int a = 0; a < 4; ++a)
-          *reinterpret_cast<uint32_t*>(qpl + (dg >> 4) * (4 * NR * 64) + ta_sw(a * NR + rp + h, (dg & 15) >> 2) +
-                                       4 * (dg & 3)) = o[a];
+          for (int a = 0; a < 4; ++a) *reinterpret_cast<uint32_t*>(dst + s * (4 * NR * 64) + a * (NR * 64)) = o[a];
+        }
       }
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (lane == 0) s_rows.corr[rp + h] = sum * kTrBias;
+      for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (l16 == 0) sh.rows.corr[r] = sum * kTrBias;
     }
+    ta_fence_async();
   }
-  ta_fence_async();
   fence_before();
   // a query value outside the digits' range: the block's scores are taken directly
   const bool qover = __syncthreads_or(qmax > kTrMaxDigit);
   fence_after();
-  const uint32_t tmem = tmem_holder;
-  auto drain = [&](int tile, int quad, int step) {
-    const int j0 = (t0 + tile) * kTrKeys;
+  const uint32_t tmem = sh.tmem;
+  // the tile's rows, its own share of them where `all` twenty warps drain
+  auto drain = [&](int tile, bool all) {
+    const int ab = kBuf == 1 ? 0 : tile & 1, j0 = (t0 + tile) * kTrKeys;
+    const int quad = warp < kTrConvWarps ? 1 + (warp >> 2) : 0, step = all ? 5 : 1;
+    fence_after();
     if (!qover) {
-      qk_drain<NR>(s_rows, tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)((kBuf == 1 ? 0 : tile & 1) * kCols), j0,
-                   quad, step);
+      qk_drain<NR>(sh.rows, tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)(ab * kCols), j0, quad, step);
     } else {
       const int key = t.lo + j0 + 32 * (warp & 3) + lane;
-      qk_drain_direct<NR>(s_rows, key < t.ctx ? kc + (int64_t)key * d : kt + (int64_t)(key - t.ctx) * d, qb, r0, G, Hq, d,
+      qk_drain_direct<NR>(sh.rows, key < t.ctx ? kc + (int64_t)key * d : kt + (int64_t)(key - t.ctx) * d, qb, r0, G, Hq, d,
                           j0, quad, step);
     }
+    fence_before();
+    __syncwarp();
   };
-  const int last_tile = t1 - t0 - 1;
 
   if (warp < kTrConvWarps) {
-    // rows 8 warp + 2 i + lane / 16 of the planes: bits 1-2 of the row are i
-    const int ch = (lane & 15) >> 2;
-    unsigned char* const pl0 = planes + lkey * 64 + 4 * (lane & 3);
-    const int plx[4] = {ch << 4, 128 + ((ch ^ 1) << 4), 256 + ((ch ^ 2) << 4), 384 + ((ch ^ 3) << 4)};
-    int tile = 0, s = 0, pb = 0, ph = 1;  // plane buffer, parity of its last use's end
-    for (int u = 0; u < total; u += 2) {
+    // key 32 (warp % 4) + lane, dims 16 (warp / 4) .. + 16 of the stage
+    const int key = 32 * (warp & 3) + lane, grp = warp >> 2, h = grp >> 1;
+    const uint32_t at = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + kTrA + 32 * h + 4 * (grp & 1);
+    const unsigned char* const row = slots + key * 256;
+    int dt = 0, due = ns + 1, pb = 0, ph = 0;
+    for (int u = 0; u < total; ++u) {
+      wait(&sh.raw_full[pb], ph);
+      uint4 x[4];
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        if (u + p < total) {
-          if (u + p >= kSt) wait(&mma_done[pb], ph);
-          unsigned char* const pl = pl0 + pb * kTrPlanes;
+      for (int i = 0; i < 4; ++i)
+        x[i] = *reinterpret_cast<const uint4*>(row + pb * kTrPlanes + 16 * ((4 * grp + i) ^ (key & 7)));
+      uint32_t o[4][4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t o[4];
-            ta_bytes(x[p][i].x, x[p][i].y, x[p][i].z, x[p][i].w, o);
+      for (int i = 0; i < 4; ++i) ta_bytes(x[i].x, x[i].y, x[i].z, x[i].w, o[i]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.raw_empty[pb]);
+      if (++pb == nst) { pb = 0; ph ^= 1; }
+      if (u > 0) wait(&sh.a_empty[h], (u - 1) & 1);
+      fence_after();
 #pragma unroll
-            for (int b = 0; b < 4; ++b) *reinterpret_cast<uint32_t*>(pl + plx[i] + b * kTrPlane) = o[b];
-          }
-          ta_fence_async();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&planes_full[pb]);
-          if (++pb == kSt) { pb = 0; ph ^= 1; }
-          next(x[p]);
-          if (kBuf == 1 && ++s == ns) {  // the one accumulator is drained by everyone
-            wait(&acc_full[0], tile & 1);
-            fence_after();
-            drain(tile, 1 + (warp >> 2), 5);
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&acc_empty[0]);
-            s = 0;
-            ++tile;
-          }
-        }
+      for (int b = 0; b < 4; ++b) ta_st4(at + 8 * b, o[0][b], o[1][b], o[2][b], o[3][b]);
+      ta_wait_st();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sh.a_full[h]);
+      // The one accumulator is drained by everyone, once the next tile's first
+      // stage (which waits for no MMA of that tile) is converted.
+      if (kBuf == 1 && (u + 1 == due || u + 1 == total)) {
+        wait(&sh.acc_full[0], dt & 1);
+        drain(dt, true);
+        if (lane == 0) mbar_arrive(&sh.acc_empty[0]);
+        ++dt;
+        due += ns;
       }
+    }
+    if (kBuf == 1 && dt <= last_tile) {
+      wait(&sh.acc_full[0], dt & 1);
+      drain(dt, true);
     }
     if (kBuf == 2) {
       // the last tile is drained by all five groups of four warps.  A barrier
       // of its own: a converter does not follow acc_full's phases, and a parity
       // tells neighbouring phases apart only
-      wait(&last_full, 0);
-      fence_after();
-      drain(last_tile, 1 + (warp >> 2), 5);
+      wait(&sh.last_full, 0);
+      drain(last_tile, true);
+    }
+  } else if (warp < 20) {
+    for (int tile = 0; tile <= last_tile; ++tile) {
+      const int ab = kBuf == 1 ? 0 : tile & 1;
+      wait(&sh.acc_full[ab], (tile / kBuf) & 1);
+      drain(tile, kBuf == 1 || tile == last_tile);
+      if (lane == 0) mbar_arrive(&sh.acc_empty[ab]);
     }
   } else if (warp == 20) {
     if (lane == 0) {
       const uint32_t full = ta_idesc(na * NR), low = ta_idesc((na - 1) * NR), one = ta_idesc(NR);
-      const uint64_t pdesc = smem_desc_sw64(su32(planes)), qdesc = smem_desc_sw64(su32(qpl));
-      int tile = 0, s = 0, pb = 0, ph = 0;
+      const uint64_t qdesc = smem_desc_sw64(su32(qpl));
+      int tile = 0, s = 0;
       for (int u = 0; u < total; ++u) {
         const int ab = kBuf == 1 ? 0 : tile & 1;
-        if (s == 0 && tile >= kBuf) wait(&acc_empty[ab], ((tile - kBuf) / kBuf) & 1);
-        wait(&planes_full[pb], ph);
+        if (s == 0 && tile >= kBuf) wait(&sh.acc_empty[ab], ((tile - kBuf) / kBuf) & 1);
+        const uint64_t qd = ta_adv(qdesc, s * (4 * NR * 64));
+        const uint32_t dcol = tmem + (uint32_t)(ab * kCols), a = tmem + kTrA;
+        wait(&sh.a_full[0], u & 1);
         fence_after();
-        const uint64_t pd = ta_adv(pdesc, pb * kTrPlanes), qd = ta_adv(qdesc, s * (4 * NR * 64));
-        const uint32_t dcol = tmem + (uint32_t)(ab * kCols);
         if (s == 0) {
           // the first products of a tile open its column blocks: byte b adds
           // to the blocks that the bytes before it opened and opens block
           // b + na - 1
-          mma_i8(dcol, pd, qd, full, 0);
+          ta_mma(dcol, a, qd, full, 0);
 #pragma unroll
           for (int b = 1; b < 4; ++b) {
-            mma_i8(dcol + b * NR, ta_adv(pd, b * kTrPlane), qd, low, 1);
-            mma_i8(dcol + (b + na - 1) * NR, ta_adv(pd, b * kTrPlane), ta_adv(qd, (na - 1) * NR * 64), one, 0);
+            ta_mma(dcol + b * NR, a + 8 * b, qd, low, 1);
+            ta_mma(dcol + (b + na - 1) * NR, a + 8 * b, ta_adv(qd, (na - 1) * NR * 64), one, 0);
           }
         } else {
 #pragma unroll
-          for (int b = 0; b < 4; ++b) mma_i8(dcol + b * NR, ta_adv(pd, b * kTrPlane), qd, full, 1);
+          for (int b = 0; b < 4; ++b) ta_mma(dcol + b * NR, a + 8 * b, qd, full, 1);
         }
+        mma_commit(&sh.a_empty[0]);
+        wait(&sh.a_full[1], u & 1);
+        fence_after();
 #pragma unroll
-        for (int b = 0; b < 4; ++b) mma_i8(dcol + b * NR, ta_adv(pd, b * kTrPlane + 32), ta_adv(qd, 32), full, 1);
-        mma_commit(&mma_done[pb]);
-        if (++pb == kSt) { pb = 0; ph ^= 1; }
+        for (int b = 0; b < 4; ++b) ta_mma(dcol + b * NR, a + 32 + 8 * b, ta_adv(qd, 32), full, 1);
+        mma_commit(&sh.a_empty[1]);
         if (s == ns - 1) {
-          mma_commit(&acc_full[ab]);
-          if (u == total - 1) mma_commit(&last_full);
+          mma_commit(&sh.acc_full[ab]);
+          if (u == total - 1) mma_commit(&sh.last_full);
           s = 0;
           ++tile;
         } else {
@@ -545,27 +609,21 @@ __global__ void __launch_bounds__(kQkThreads, 1) tree_qk(const __grid_constant__
       }
     }
   } else {
-    // warps 16-19: accumulator lane (key) 32 (warp % 4) + lane
-    for (int tile = 0; tile <= last_tile; ++tile) {
-      const int ab = kBuf == 1 ? 0 : tile & 1;
-      wait(&acc_full[ab], (tile / kBuf) & 1);
-      fence_after();
-      if (kBuf == 1 || tile == last_tile) drain(tile, 0, 5);
-      else drain(tile, 0, 1);
-      fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&acc_empty[ab]);
+    for (int u = nst; u < total; ++u) {
+      wait(&sh.raw_empty[lb], lph);
+      load();
     }
+    cp_wait_all();
   }
   fence_before();
   __syncthreads();
   if (tid < nr) {
     uint32_t* tmax = reinterpret_cast<uint32_t*>(static_cast<unsigned char*>(g.ws) + g.max_off) + t.moff;
-    tmax[((int64_t)kvh * rows + r0 + tid) * t.qk_per + part] = s_rows.top[tid];
+    tmax[((int64_t)kvh * rows + r0 + tid) * t.qk_per + part] = sh.rows.top[tid];
   }
-  if (s_fail && tid == 0) atomicExch(&g_tree_err, 1);
+  if (sh.fail && tid == 0) atomicExch(&g_tree_err, 1);
   fence_after();
-  if (warp == 20) ta_dealloc<kTmem>(tmem);
+  if (warp == 20) ta_dealloc<512>(tmem);
 }
 
 // ---------------------------------------------------------------------------
@@ -913,7 +971,9 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
 
 template <int NR, bool VEC>
 void qk_attr() {
-  cudaFuncSetAttribute(tree_qk<NR, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, qk_smem<NR>(8));
+  int most = 0;
+  for (int ns = 1; ns <= 8; ++ns) most = std::max(most, qk_smem<NR>(ns));
+  cudaFuncSetAttribute(tree_qk<NR, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
 }
 template <int NR>
 void pv_attr() {
