@@ -41,6 +41,29 @@ RDET_HD int32_t requantize(int64_t a) {
   return q + (int32_t)inc;
 }
 
+// The same without branches, for loops that round many sums: rounded in 64
+// bits (where that wraps, the value was out of range), kept if the result's
+// upper half is a sign extension.
+RDET_HD int32_t requantize_flat(int64_t a) {
+  const uint64_t r = (uint64_t)a + 0x7fffu + (((uint64_t)a >> 16) & 1u);
+  const uint32_t hi = (uint32_t)(r >> 32);
+  return hi + 0x8000u < 0x10000u ? (int32_t)(uint32_t)(r >> 16) : (int32_t)(a >> 63) ^ INT32_MAX;
+}
+
+// requantize(add + sum of c[g] 2^(8 g), g = 0 .. 6), wrapping, in 32-bit
+// pieces: 16 bits, 16 bits and the high word.  The digit sums are at most 2^26
+// in magnitude; `add` comes as its own low, middle and high piece.
+RDET_HD int32_t requantize_digits(int32_t c0, int32_t c1, int32_t c2, int32_t c3, int32_t c4, int32_t c5, int32_t c6,
+                                  int32_t add0, int32_t add16, int32_t add32) {
+  const int32_t a = c0 + ((c1 & 0xff) << 8) + add0;
+  const int32_t b = c2 + (c1 >> 8) + (a >> 16) + ((c3 & 0xff) << 8) + add16;
+  const uint32_t h = (uint32_t)c4 + (uint32_t)(c3 >> 8) + ((uint32_t)c5 << 8) + ((uint32_t)c6 << 16) + (uint32_t)add32;
+  const int32_t up = b + (((a & 0xffff) + 0x7fff + (b & 1)) >> 16);  // rounded
+  const uint32_t hi = h + (uint32_t)(up >> 16);
+  return hi + 0x8000u < 0x10000u ? (int32_t)(hi << 16 | ((uint32_t)up & 0xffffu))
+                                 : ((int32_t)(h + (uint32_t)(b >> 16)) >> 31) ^ INT32_MAX;
+}
+
 // ops.rs:770 for an arbitrary shift in [1, 63]
 RDET_HD int64_t rshift_rte(int64_t a, uint32_t s) {
   if (s == 0) return a;

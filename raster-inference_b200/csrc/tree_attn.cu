@@ -68,7 +68,7 @@ constexpr int kTrConvWarps = kTrConv / 32;
 constexpr int kQkThreads = 736;        // + warps 16-19 drain, warp 20 issues the MMAs, warps 21-22 load
 constexpr int kQkDrainWarps = 20;      // warps 0-19
 constexpr int kTrLoaders = 64;         // loading threads
-constexpr int kPvThreads = 544;        // + warp 16 issues the MMAs
+constexpr int kPvThreads = 608;        // + warp 16 issues the MMAs, warps 17-18 load
 constexpr int kTrMaxDigit = 0x7f7f7f7f;
 constexpr int kTrSplitKeys = 32704;    // keys of one value CTA at most: 3 * 2^14 each in s32
 
@@ -189,6 +189,13 @@ __device__ __forceinline__ void ld4(uint32_t& v, const void* p, bool on) {
                : "+r"(v)
                : "l"(p), "r"((int)on));
 }
+// the warp's number, known to be the same in all lanes
+__device__ __forceinline__ int ta_warp() { return __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0); }
+__device__ __forceinline__ bool ta_elect() {
+  uint32_t one;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+  return one != 0;
+}
 // kind::i8 MMA with operand A in TMEM (128 lanes, four K bytes a column)
 __device__ __forceinline__ void ta_mma(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
@@ -201,7 +208,6 @@ __device__ __forceinline__ void ta_st4(uint32_t taddr, uint32_t a, uint32_t b, u
                : "memory");
 }
 __device__ __forceinline__ void ta_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-constexpr int kTrA = 448;  // TMEM column of operand A's two buffers of 32 columns
 
 // asynchronous copies into shared memory, zeros where `on` is false, and their
 // arrival on a barrier once all of the thread's copies so far are there
@@ -270,7 +276,10 @@ __device__ __forceinline__ int64_t shift_sum(int64_t add, int32_t c0, int32_t c1
 // pieces are read without bank conflicts).  The key bytes go to the MMAs
 // through TMEM, operand A lying there: written to shared memory and read back
 // by the MMAs they made its bandwidth the bound (1550 cycles a stage at 64 rows,
-// of which the MMAs take 1024).  Two buffers of 32 dims, eight columns a byte.
+// of which the MMAs take 1024).  A unit of operand A is half the stage's dims of
+// the four key bytes, eight columns each; one refills while the other is
+// multiplied.  (Eight units beside smaller accumulators, or four of two bytes,
+// measured the same or slower.)
 constexpr int kQkMaxStages = 6;
 constexpr int kSmemMost = 232448;  // a CTA's shared memory
 template <int NR>
@@ -283,7 +292,7 @@ __host__ __device__ constexpr int qk_smem(int ns) { return qk_stages<NR>(ns) * k
 // what draining a tile needs, per row of the block
 template <int NR>
 struct QkRows {
-  int64_t corr[NR];        // 0x808080 times the sum of the query row
+  int4 corr[NR];           // 0x808080 times the sum of the query row: 16 bits, 16 bits, high word
   uint64_t mask[NR];       // the node's ancestors and itself
   int32_t start[NR];       // the first position it attends
   uint32_t top[NR];        // its largest score so far, order-preserving as u32
@@ -293,7 +302,7 @@ struct QkRows {
 };
 template <int NR>
 struct QkShared {
-  uint64_t raw_full[kQkMaxStages], raw_empty[kQkMaxStages], a_full[2], a_empty[2], acc_full[2], acc_empty[2], last_full;
+  uint64_t raw_full[kQkMaxStages], raw_empty[kQkMaxStages], a_full[2], a_empty[2], acc_full, acc_empty;
   uint32_t tmem;
   int fail;
   QkRows<NR> rows;
@@ -319,7 +328,8 @@ __device__ __noinline__ void qk_drain(QkRows<NR>& c, uint32_t taddr, int j0, int
     uint32_t top[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int32_t s = requantize(shift_sum(c.corr[r + i], v[0][i], v[1][i], v[2][i], v[3][i], v[4][i], v[5][i], v[6][i]));
+      const int4 k = c.corr[r + i];
+      const int32_t s = requantize_digits(v[0][i], v[1][i], v[2][i], v[3][i], v[4][i], v[5][i], v[6][i], k.x, k.y, k.z);
       if (in && r + i < nr) out[(int64_t)i * c.pad] = s;
       top[i] = (uint32_t)s ^ 0x80000000u;
     }
@@ -361,13 +371,12 @@ __device__ __noinline__ void qk_drain_direct(QkRows<NR>& c, const int32_t* k, co
 
 template <int NR, bool VEC>
 __global__ void __launch_bounds__(kQkThreads, 1) tree_qk(const __grid_constant__ TreeGroup g) {
-  constexpr int kCols = 7 * NR;
-  constexpr int kBuf = NR == 64 ? 1 : 2;        // accumulator buffers in TMEM
   constexpr int na = 4;                         // query digits
+  constexpr int kA = 448;                       // TMEM column of operand A's two units
   extern __shared__ __align__(16) unsigned char tr_raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(tr_raw) + 511) & ~(uintptr_t)511);
   __shared__ __align__(16) QkShared<NR> sh;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = ta_warp(), lane = tid & 31;
 
   // item -> sequence, KV head, row block, key tiles [t0, t1)
   const int si = seq_of(g.qk_first, g.nseq, blockIdx.x);
@@ -393,10 +402,9 @@ __global__ void __launch_bounds__(kQkThreads, 1) tree_qk(const __grid_constant__
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sh.a_full[i], kTrConvWarps / 2);
       mbar_init(&sh.a_empty[i], 1);
-      mbar_init(&sh.acc_full[i], 1);
-      mbar_init(&sh.acc_empty[i], kBuf == 1 ? kQkDrainWarps : 4);
     }
-    mbar_init(&sh.last_full, 1);
+    mbar_init(&sh.acc_full, 1);
+    mbar_init(&sh.acc_empty, kQkDrainWarps);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     sh.fail = 0;
     sh.rows.sc = static_cast<int32_t*>(g.ws) + t.soff + ((int64_t)kvh * rows + r0) * t.pad;
@@ -455,22 +463,27 @@ __global__ void __launch_bounds__(kQkThreads, 1) tree_qk(const __grid_constant__
   };
   ta_wait();
   ta_go();
+  // Query digits: chunk s holds dims [64 s, 64 s + 64) of rows a * NR + r; a
+  // half warp takes a row, 16 bytes a lane and chunk.
+  const int half = lane >> 4, l16 = lane & 15;
+  uint4 v[8];
+  auto load_q = [&](int r) {
+#pragma unroll
+    for (int s = 0; s < 8; ++s) v[s] = make_uint4(0, 0, 0, 0);
+    const int rr = r0 + min(r, nr - 1), node = rr / G;
+    const int32_t* q = qb + ((int64_t)node * Hq + (rr - node * G)) * d;
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+      if (s < ns) load4<VEC>(v[s], q, 64 * s + 4 * l16, d, r < nr);
+  };
   __syncthreads();  // the barriers are there
   int32_t qmax = INT32_MIN;
   if (warp > 20) {
     for (int u = 0; u < min(nst, total); ++u) load();
   } else {
-    // query digits: chunk s holds dims [64 s, 64 s + 64) of rows a * NR + r; a
-    // half warp takes a row, 16 bytes a lane and chunk
-    const int half = lane >> 4, l16 = lane & 15;
 #pragma unroll 1
-    for (int rp = 2 * warp; rp < NR; rp += 42) {
-      const int r = rp + half, rr = r0 + min(r, nr - 1), node = rr / G;
-      const int32_t* q = qb + ((int64_t)node * Hq + (rr - node * G)) * d;
-      uint4 v[8] = {};
-#pragma unroll
-      for (int s = 0; s < 8; ++s)
-        if (s < ns) load4<VEC>(v[s], q, 64 * s + 4 * l16, d, r < nr);
+    for (int r = 2 * warp + half; r < NR; r += 42) {
+      load_q(r);
       int64_t sum = 0;
       unsigned char* const dst = qpl + ta_sw(r, l16 >> 2) + 4 * (l16 & 3);
 #pragma unroll
@@ -487,7 +500,10 @@ __global__ void __launch_bounds__(kQkThreads, 1) tree_qk(const __grid_constant__
       }
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (l16 == 0) sh.rows.corr[r] = sum * kTrBias;
+      if (l16 == 0) {
+        const int64_t k = sum * kTrBias;
+        sh.rows.corr[r] = make_int4((int32_t)(k & 0xffff), (int32_t)((k >> 16) & 0xffff), (int32_t)(k >> 32), 0);
+      }
     }
     ta_fence_async();
   }
@@ -495,27 +511,33 @@ __global__ void __launch_bounds__(kQkThreads, 1) tree_qk(const __grid_constant__
   // a query value outside the digits' range: the block's scores are taken directly
   const bool qover = __syncthreads_or(qmax > kTrMaxDigit);
   fence_after();
-  const uint32_t tmem = sh.tmem;
-  // the tile's rows, its own share of them where `all` twenty warps drain
-  auto drain = [&](int tile, bool all) {
-    const int ab = kBuf == 1 ? 0 : tile & 1, j0 = (t0 + tile) * kTrKeys;
-    const int quad = warp < kTrConvWarps ? 1 + (warp >> 2) : 0, step = all ? 5 : 1;
+  // All 512 columns are this CTA's: they begin at 0 (a constant address keeps
+  // the MMA warp's operands uniform).
+  constexpr uint32_t tmem = 0;
+  if (tid == 0 && sh.tmem != 0) sh.fail = 1;
+  // a fifth of the tile's rows by each of the five groups of four warps
+  auto drain = [&](int tile) {
+    const int j0 = (t0 + tile) * kTrKeys, quad = warp < kTrConvWarps ? 1 + (warp >> 2) : 0;
+    wait(&sh.acc_full, tile & 1);
     fence_after();
     if (!qover) {
-      qk_drain<NR>(sh.rows, tmem + ((uint32_t)(32 * (warp & 3)) << 16) + (uint32_t)(ab * kCols), j0, quad, step);
+      qk_drain<NR>(sh.rows, tmem + ((uint32_t)(32 * (warp & 3)) << 16), j0, quad, 5);
     } else {
       const int key = t.lo + j0 + 32 * (warp & 3) + lane;
       qk_drain_direct<NR>(sh.rows, key < t.ctx ? kc + (int64_t)key * d : kt + (int64_t)(key - t.ctx) * d, qb, r0, G, Hq, d,
-                          j0, quad, step);
+                          j0, quad, 5);
     }
     fence_before();
     __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.acc_empty);
   };
 
   if (warp < kTrConvWarps) {
-    // key 32 (warp % 4) + lane, dims 16 (warp / 4) .. + 16 of the stage
+    // Key 32 (warp % 4) + lane, dims 16 (warp / 4) .. + 16 of the stage.  A tile
+    // is drained once the next one's first stage is converted (which waits
+    // for no MMA of that next tile).
     const int key = 32 * (warp & 3) + lane, grp = warp >> 2, h = grp >> 1;
-    const uint32_t at = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + kTrA + 32 * h + 4 * (grp & 1);
+    const uint32_t at = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + kA + 32 * h + 4 * (grp & 1);
     const unsigned char* const row = slots + key * 256;
     int dt = 0, due = ns + 1, pb = 0, ph = 0;
     for (int u = 0; u < total; ++u) {
@@ -538,74 +560,54 @@ __global__ void __launch_bounds__(kQkThreads, 1) tree_qk(const __grid_constant__
       fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sh.a_full[h]);
-      // The one accumulator is drained by everyone, once the next tile's first
-      // stage (which waits for no MMA of that tile) is converted.
-      if (kBuf == 1 && (u + 1 == due || u + 1 == total)) {
-        wait(&sh.acc_full[0], dt & 1);
-        drain(dt, true);
-        if (lane == 0) mbar_arrive(&sh.acc_empty[0]);
-        ++dt;
+      if (u + 1 == due) {
+        drain(dt++);
         due += ns;
       }
     }
-    if (kBuf == 1 && dt <= last_tile) {
-      wait(&sh.acc_full[0], dt & 1);
-      drain(dt, true);
-    }
-    if (kBuf == 2) {
-      // the last tile is drained by all five groups of four warps.  A barrier
-      // of its own: a converter does not follow acc_full's phases, and a parity
-      // tells neighbouring phases apart only
-      wait(&sh.last_full, 0);
-      drain(last_tile, true);
-    }
+    while (dt <= last_tile) drain(dt++);
   } else if (warp < 20) {
-    for (int tile = 0; tile <= last_tile; ++tile) {
-      const int ab = kBuf == 1 ? 0 : tile & 1;
-      wait(&sh.acc_full[ab], (tile / kBuf) & 1);
-      drain(tile, kBuf == 1 || tile == last_tile);
-      if (lane == 0) mbar_arrive(&sh.acc_empty[ab]);
-    }
+    for (int tile = 0; tile <= last_tile; ++tile) drain(tile);
   } else if (warp == 20) {
-    if (lane == 0) {
-      const uint32_t full = ta_idesc(na * NR), low = ta_idesc((na - 1) * NR), one = ta_idesc(NR);
-      const uint64_t qdesc = smem_desc_sw64(su32(qpl));
-      int tile = 0, s = 0;
-      for (int u = 0; u < total; ++u) {
-        const int ab = kBuf == 1 ? 0 : tile & 1;
-        if (s == 0 && tile >= kBuf) wait(&sh.acc_empty[ab], ((tile - kBuf) / kBuf) & 1);
-        const uint64_t qd = ta_adv(qdesc, s * (4 * NR * 64));
-        const uint32_t dcol = tmem + (uint32_t)(ab * kCols), a = tmem + kTrA;
-        wait(&sh.a_full[0], u & 1);
-        fence_after();
-        if (s == 0) {
-          // the first products of a tile open its column blocks: byte b adds
-          // to the blocks that the bytes before it opened and opens block
-          // b + na - 1
-          ta_mma(dcol, a, qd, full, 0);
+    // The whole warp follows the loop and one lane issues: a loop in a branch of
+    // one lane moves every operand to a uniform register by itself, about 80
+    // cycles an MMA, which made the issue the bound (132 us instead of 121 for
+    // 64 nodes at context 32768).
+    const bool leader = ta_elect();
+    const uint32_t full = ta_idesc(na * NR), low = ta_idesc((na - 1) * NR), one = ta_idesc(NR);
+    const uint64_t qdesc = smem_desc_sw64(su32(qpl));
+    int tile = 0, s = 0;
+    for (int u = 0; u < total; ++u) {
+      if (s == 0 && tile >= 1) wait(&sh.acc_empty, (tile - 1) & 1);
 #pragma unroll
-          for (int b = 1; b < 4; ++b) {
-            ta_mma(dcol + b * NR, a + 8 * b, qd, low, 1);
-            ta_mma(dcol + (b + na - 1) * NR, a + 8 * b, ta_adv(qd, (na - 1) * NR * 64), one, 0);
+      for (int h = 0; h < 2; ++h) {
+        const uint64_t qd = ta_adv(qdesc, s * (4 * NR * 64) + 32 * h);
+        const uint32_t a = tmem + kA + 32 * h;
+        wait(&sh.a_full[h], u & 1);
+        fence_after();
+        if (leader) {
+          if (h == 0 && s == 0) {
+            // the first products of a tile open its column blocks: byte b adds
+            // to the blocks that the bytes before it opened and opens block
+            // b + na - 1
+            ta_mma(tmem, a, qd, full, 0);
+#pragma unroll
+            for (int b = 1; b < 4; ++b) {
+              ta_mma(tmem + b * NR, a + 8 * b, qd, low, 1);
+              ta_mma(tmem + (b + na - 1) * NR, a + 8 * b, ta_adv(qd, (na - 1) * NR * 64), one, 0);
+            }
+          } else {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) ta_mma(tmem + b * NR, a + 8 * b, qd, full, 1);
           }
-        } else {
-#pragma unroll
-          for (int b = 0; b < 4; ++b) ta_mma(dcol + b * NR, a + 8 * b, qd, full, 1);
+          mma_commit(&sh.a_empty[h]);
+          if (h == 1 && s == ns - 1) mma_commit(&sh.acc_full);
         }
-        mma_commit(&sh.a_empty[0]);
-        wait(&sh.a_full[1], u & 1);
-        fence_after();
-#pragma unroll
-        for (int b = 0; b < 4; ++b) ta_mma(dcol + b * NR, a + 32 + 8 * b, ta_adv(qd, 32), full, 1);
-        mma_commit(&sh.a_empty[1]);
-        if (s == ns - 1) {
-          mma_commit(&sh.acc_full[ab]);
-          if (u == total - 1) mma_commit(&sh.last_full);
-          s = 0;
-          ++tile;
-        } else {
-          ++s;
-        }
+        __syncwarp();
+      }
+      if (++s == ns) {
+        s = 0;
+        ++tile;
       }
     }
   } else {
@@ -715,20 +717,28 @@ __global__ void __launch_bounds__(kExThreads) tree_exp(const __grid_constant__ T
 // sums in distributed shared memory measured worse: only about 13 clusters of
 // eight large CTAs fit the GPU at once, so 16 took two waves.)
 // ---------------------------------------------------------------------------
-constexpr int kPvStages = 4;
+// A stage is 64 keys of the 128 dims, 32 KB as they are in a ring of slots; the
+// value bytes go to the MMAs through TMEM like the key bytes above (a thread
+// holds one dim of 16 keys), the weights' digits through shared memory.
+constexpr int kPvStages = 6;  // slots
+constexpr int kPvW = 4;       // weight tiles
 template <int NR>
-__host__ __device__ constexpr int pv_smem() { return kPvStages * (kTrPlanes + 3 * NR * 64) + 1024; }
+__host__ __device__ constexpr int pv_stages() { return NR == 64 ? 5 : kPvStages; }
+template <int NR>
+__host__ __device__ constexpr int pv_smem() { return pv_stages<NR>() * kTrPlanes + kPvW * 3 * NR * 64 + 512; }
 
-template <int NR>
+template <int NR, bool VEC>
 __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__ TreeGroup g) {
-  constexpr int kTmem = NR == 16 ? 128 : NR == 32 ? 256 : 512;
+  constexpr int kA = 448;                       // TMEM column of operand A's two units
+  constexpr int kSt = pv_stages<NR>();
   constexpr int kW = 3 * NR * 64;               // one stage's weight tile
   constexpr int kE = (NR * 16 + kTrConv - 1) / kTrConv;  // (row, four keys) pieces of it per converter thread
   extern __shared__ __align__(16) unsigned char tr_raw[];
-  unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(tr_raw) + 1023) & ~(uintptr_t)1023);
-  unsigned char* planes = sm;                   // [stage][4 bytes][128 dims][64 keys]
-  unsigned char* wsm = sm + kPvStages * kTrPlanes;  // [stage][3 NR rows][64 keys]
-  __shared__ __align__(8) uint64_t planes_full[kPvStages], mma_done[kPvStages], acc_full;
+  unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(tr_raw) + 511) & ~(uintptr_t)511);
+  unsigned char* slots = sm;                    // [slot][64 keys][128 dims]
+  unsigned char* wsm = sm + kSt * kTrPlanes;    // [tile][3 NR rows][64 keys]
+  __shared__ __align__(8) uint64_t raw_full[kPvStages], raw_empty[kPvStages], a_full[2], a_empty[2], w_full[kPvW], w_empty[kPvW],
+      acc_full;
   __shared__ uint32_t tmem_holder;
   __shared__ int s_fail;
   __shared__ uint64_t s_sum[NR];                // each row's sum of terms
@@ -736,7 +746,7 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
   __shared__ uint32_t s_inv[NR];
   __shared__ int32_t s_wsum[NR];                // each row's sum of this CTA's weights
   __shared__ uint32_t s_last;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = ta_warp(), lane = tid & 31;
 
   const int si = seq_of(g.pv_first, g.nseq, blockIdx.x);
   const TreeSeq t = g.seq[si];
@@ -751,28 +761,40 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
   const uint32_t* const ex = reinterpret_cast<const uint32_t*>(ws) + t.soff + (int64_t)lrow0 * t.pad + c0 * 64;
   const int32_t* const vc = t.v + (int64_t)kvh * t.kstride;
   const int32_t* const vt = t.vt + (int64_t)kvh * t.tstride;
+  const int last_key = t.lo + t.len - 1;
 
-  // a converter thread's part of a stage: dim tid % 128, keys 16 (tid / 128) .. + 16
-  const int dl = tid & 127, quarter = (tid >> 7) & 3, dim = db * 128 + dl;
-  // keys past the sequence read its last key (their weights are zero), dims
-  // past the head its last dim (their sums are not stored)
-  const int cdim = min(dim, d - 1), last_key = t.lo + t.len - 1;
-  const uint32_t off0 = ((uint32_t)(16 * quarter) * d + cdim) * 4, step = 4 * (uint32_t)d;
-  uint32_t x[2][16] = {};  // two stages in flight
-  auto load = [&](uint32_t (&y)[16], int u) {
-    const int key0 = t.lo + (c0 + u) * 64;
-    const bool on = u < total;
-    if (key0 + 64 <= t.ctx) {  // cache rows only
-      const unsigned char* base = reinterpret_cast<const unsigned char*>(vc + (int64_t)key0 * d);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) ld4(y[i], base + (off0 + i * step), on);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int key = min(key0 + 16 * quarter + i, last_key);
-        ld4(y[i], (key < t.ctx ? vc + (int64_t)key * d : vt + (int64_t)(key - t.ctx) * d) + cdim, on);
+  // Stage lu into its slot.  Keys past the sequence (their weights are zero) and
+  // dims past the head (their sums are not stored) are zero.
+  int lu = 0, lb = 0, lph = 1;  // next stage, its slot and the parity of the slot's last use
+  auto load = [&]() {
+    const uint32_t slot = su32(slots) + lb * kTrPlanes;
+    const int key0 = t.lo + (c0 + lu) * 64, p = tid & (kTrLoaders - 1);
+    if (VEC) {  // 16 bytes of keys p / 32, p / 32 + 2, ..
+      const int dim = db * 128 + 4 * (p & 31), row0 = p >> 5;
+      const bool on = dim < d;
+      const uint32_t dst = slot + row0 * 512 + 16 * (p & 31);
+      const int od = on ? dim : 0;
+      if (key0 + 64 <= t.ctx) {  // cache rows only
+        const int32_t* src = vc + (int64_t)(key0 + row0) * d + od;
+#pragma unroll 8
+        for (int i = 0; i < 32; ++i) cp16(dst + i * 1024, src + (int64_t)i * (2 * d), on);
+      } else {
+        for (int i = 0; i < 32; ++i) {
+          const int key = min(key0 + row0 + 2 * i, last_key);
+          cp16(dst + i * 1024, (key < t.ctx ? vc + (int64_t)key * d : vt + (int64_t)(key - t.ctx) * d) + od,
+               on && key0 + row0 + 2 * i <= last_key);
+        }
+      }
+    } else {  // two dims of every key
+      for (int i = 0; i < 128; ++i) {
+        const int dl = p + 64 * (i & 1), dim = db * 128 + dl, k = i >> 1, key = min(key0 + k, last_key);
+        cp4(slot + k * 512 + 4 * dl, (key < t.ctx ? vc + (int64_t)key * d : vt + (int64_t)(key - t.ctx) * d) + min(dim, d - 1),
+            dim < d && key0 + k <= last_key);
       }
     }
+    cp_arrive(&raw_full[lb]);
+    ++lu;
+    if (++lb == kSt) { lb = 0; lph ^= 1; }
   };
   // its part of the weights: rows tid / 16 + 32 i (at most the block's last),
   // keys 4 (tid % 16) .. + 4
@@ -782,23 +804,30 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
 #pragma unroll
     for (int i = 0; i < kE; ++i) ld16(ev[i], ex + (int64_t)min(wr + 32 * i, nr - 1) * t.pad + u * 64 + 4 * wq, u < total);
   };
-  // The values do not depend on the terms: their first stages load before the
-  // wait (this grid starts only after the score kernel has completed, and with
-  // it everything before it).
-  if (warp < kTrConvWarps) {
-    load(x[0], 0);
-    load(x[1], 1);
-  }
   if (tid == 0) {
-    for (int i = 0; i < kPvStages; ++i) {
-      mbar_init(&planes_full[i], kTrConvWarps);
-      mbar_init(&mma_done[i], 1);
+    for (int i = 0; i < kSt; ++i) {
+      mbar_init(&raw_full[i], kTrLoaders);
+      mbar_init(&raw_empty[i], kTrConvWarps);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&a_full[i], kTrConvWarps / 2);
+      mbar_init(&a_empty[i], 1);
+    }
+    for (int i = 0; i < kPvW; ++i) {
+      mbar_init(&w_full[i], kTrConvWarps);
+      mbar_init(&w_empty[i], 1);
     }
     mbar_init(&acc_full, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     s_fail = 0;
   }
-  if (warp == kTrConvWarps) ta_alloc<kTmem>(&tmem_holder);
+  if (warp == kTrConvWarps) ta_alloc<512>(&tmem_holder);
+  __syncthreads();  // the barriers are there
+  // The values do not depend on the terms: their first stages load before the
+  // wait (this grid starts only after the score kernel has completed, and with
+  // it everything before it).
+  if (warp > kTrConvWarps)
+    for (int u = 0; u < min(kSt, total); ++u) load();
   ta_wait();
   ta_go();
   if (warp < kTrConvWarps) load_e(0);
@@ -829,55 +858,60 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = tmem_holder;
+  constexpr uint32_t tmem = 0;  // all 512 columns, as above
+  if (tid == 0 && tmem_holder != 0) s_fail = 1;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
     if (!ta_mbar_wait(bar, parity)) s_fail = 1;
   };
 
   if (warp < kTrConvWarps) {
+    // dim 32 (warp % 4) + lane, keys 16 (warp / 4) .. + 16 of the stage
+    const int grp = warp >> 2, h = grp >> 1;
+    const uint32_t at = ((uint32_t)(32 * (warp & 3)) << 16) + kA + 32 * h + 4 * (grp & 1);
+    const unsigned char* const col = slots + 16 * grp * 512 + 4 * (32 * (warp & 3) + lane);
     int32_t wsum[kE] = {};
-    int pb = 0, ph = 1;  // plane buffer, parity of its last use's end
-    for (int u0 = 0; u0 < total; u0 += 2) {
+    int pb = 0, ph = 0;
+    for (int u = 0; u < total; ++u) {
+      // weights first: they need the values' MMAs before the last ones only
+      const int wb = u & (kPvW - 1);
+      if (u >= kPvW) wait(&w_empty[wb], (u / kPvW - 1) & 1);
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const int u = u0 + p;
-        if (u < total) {
-          if (u >= kPvStages) wait(&mma_done[pb], ph);
+      for (int i = 0; i < kE; ++i) {
+        const int r = wr + 32 * i;
+        if (r >= NR) break;
+        const uint32_t inv = s_inv[r];
+        const uint64_t sum = s_sum[r];
+        const int32_t w0 = ta_weight(ev[i].x, inv, sum), w1 = ta_weight(ev[i].y, inv, sum),
+                      w2 = ta_weight(ev[i].z, inv, sum), w3 = ta_weight(ev[i].w, inv, sum);
+        wsum[i] += w0 + w1 + w2 + w3;
+        uint32_t o[4];
+        ta_t4(ta_digits(w0), ta_digits(w1), ta_digits(w2), ta_digits(w3), o);
 #pragma unroll
-          for (int i = 0; i < kE; ++i) {
-            const int r = wr + 32 * i;
-            if (r >= NR) break;
-            const uint32_t inv = s_inv[r];
-            const uint64_t sum = s_sum[r];
-            const int32_t w0 = ta_weight(ev[i].x, inv, sum), w1 = ta_weight(ev[i].y, inv, sum),
-                          w2 = ta_weight(ev[i].z, inv, sum), w3 = ta_weight(ev[i].w, inv, sum);
-            wsum[i] += w0 + w1 + w2 + w3;
-            uint32_t o[4];
-            ta_t4(ta_digits(w0), ta_digits(w1), ta_digits(w2), ta_digits(w3), o);
-#pragma unroll
-            for (int a = 0; a < 3; ++a)
-              *reinterpret_cast<uint32_t*>(wsm + pb * kW + ta_sw(a * NR + r, wq >> 2) + 4 * (wq & 3)) = o[a];
-          }
-          unsigned char* pl = planes + pb * kTrPlanes + ta_sw(dl, quarter);
-          uint32_t o[4][4];  // one 16-byte piece of each byte plane
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t q[4];
-            ta_bytes(x[p][4 * k], x[p][4 * k + 1], x[p][4 * k + 2], x[p][4 * k + 3], q);
-#pragma unroll
-            for (int b = 0; b < 4; ++b) o[b][k] = q[b];
-          }
-#pragma unroll
-          for (int b = 0; b < 4; ++b)
-            *reinterpret_cast<uint4*>(pl + b * kTrPlane) = make_uint4(o[b][0], o[b][1], o[b][2], o[b][3]);
-          ta_fence_async();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&planes_full[pb]);
-          if (++pb == kPvStages) { pb = 0; ph ^= 1; }
-          load_e(u + 1);
-          load(x[p], u + 2);
-        }
+        for (int a = 0; a < 3; ++a)
+          *reinterpret_cast<uint32_t*>(wsm + wb * kW + ta_sw(a * NR + r, wq >> 2) + 4 * (wq & 3)) = o[a];
       }
+      ta_fence_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&w_full[wb]);
+      load_e(u + 1);
+      wait(&raw_full[pb], ph);
+      uint32_t x[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = *reinterpret_cast<const uint32_t*>(col + pb * kTrPlanes + 512 * i);
+      uint32_t o[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ta_bytes(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3], o[i]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&raw_empty[pb]);
+      if (++pb == kSt) { pb = 0; ph ^= 1; }
+      if (u > 0) wait(&a_empty[h], (u - 1) & 1);
+      fence_after();
+#pragma unroll
+      for (int b = 0; b < 4; ++b) ta_st4(at + 8 * b, o[0][b], o[1][b], o[2][b], o[3][b]);
+      ta_wait_st();
+      fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&a_full[h]);
     }
     // a row's weights lie in the 16 threads of its keys
 #pragma unroll
@@ -887,36 +921,50 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
       for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
       if (wq == 0 && wr + 32 * i < NR) s_wsum[wr + 32 * i] = v;
     }
-  } else if (lane == 0 && total > 0) {
+  } else if (warp == kTrConvWarps) {
+    const bool leader = ta_elect();
     const uint32_t full = ta_idesc(3 * NR), low = ta_idesc(2 * NR), one = ta_idesc(NR);
-    const uint64_t pdesc = smem_desc_sw64(su32(planes)), wdesc = smem_desc_sw64(su32(wsm));
-    int pb = 0, ph = 0;
+    const uint64_t wdesc = smem_desc_sw64(su32(wsm));
     for (int u = 0; u < total; ++u) {
-      wait(&planes_full[pb], ph);
-      fence_after();
-      const uint64_t pd = ta_adv(pdesc, pb * kTrPlanes), wd = ta_adv(wdesc, pb * kW);
-      if (u == 0) {  // opens the column blocks, as in the score kernel
-        mma_i8(tmem, pd, wd, full, 0);
+      const int wb = u & (kPvW - 1);
+      wait(&w_full[wb], (u / kPvW) & 1);
 #pragma unroll
-        for (int b = 1; b < 4; ++b) {
-          mma_i8(tmem + b * NR, ta_adv(pd, b * kTrPlane), wd, low, 1);
-          mma_i8(tmem + (b + 2) * NR, ta_adv(pd, b * kTrPlane), ta_adv(wd, 2 * NR * 64), one, 0);
+      for (int h = 0; h < 2; ++h) {
+        const uint64_t wd = ta_adv(wdesc, wb * kW + 32 * h);
+        const uint32_t a = tmem + kA + 32 * h;
+        wait(&a_full[h], u & 1);
+        fence_after();
+        if (leader) {
+          if (h == 0 && u == 0) {  // opens the column blocks, as in the score kernel
+            ta_mma(tmem, a, wd, full, 0);
+#pragma unroll
+            for (int b = 1; b < 4; ++b) {
+              ta_mma(tmem + b * NR, a + 8 * b, wd, low, 1);
+              ta_mma(tmem + (b + 2) * NR, a + 8 * b, ta_adv(wd, 2 * NR * 64), one, 0);
+            }
+          } else {
+#pragma unroll
+            for (int b = 0; b < 4; ++b) ta_mma(tmem + b * NR, a + 8 * b, wd, full, 1);
+          }
+          mma_commit(&a_empty[h]);
+          if (h == 1) mma_commit(&w_empty[wb]);
+          if (h == 1 && u == total - 1) mma_commit(&acc_full);
         }
-      } else {
-#pragma unroll
-        for (int b = 0; b < 4; ++b) mma_i8(tmem + b * NR, ta_adv(pd, b * kTrPlane), wd, full, 1);
+        __syncwarp();
       }
-#pragma unroll
-      for (int b = 0; b < 4; ++b) mma_i8(tmem + b * NR, ta_adv(pd, b * kTrPlane + 32), ta_adv(wd, 32), full, 1);
-      mma_commit(&mma_done[pb]);
-      if (++pb == kPvStages) { pb = 0; ph ^= 1; }
-      if (u == total - 1) mma_commit(&acc_full);
     }
-    wait(&acc_full, 0);
+    if (total > 0) wait(&acc_full, 0);
+  } else {
+    for (int u = kSt; u < total; ++u) {
+      wait(&raw_empty[lb], lph);
+      load();
+    }
+    cp_wait_all();
   }
   __syncthreads();
   fence_after();
   // ---- the block's partial sums: lane dl, rows split over the four quarters
+  const int dl = tid & 127, quarter = (tid >> 7) & 3, dim = db * 128 + dl;
   auto orow = [&](int r) {
     const int rr = r0 + r, node = rr / G;
     return g.out + ((int64_t)(t.node0 + node) * Hq + kvh * G + (rr - node * G)) * d;
@@ -929,7 +977,7 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
     const int key = t.lo + s_first[r];
     const int32_t* p = key < t.ctx ? vc + (int64_t)key * d : vt + (int64_t)(key - t.ctx) * d;
     v += (uint64_t)(kTrBias * wt) + (uint64_t)mul_wide(sub_sat(kOneAct, wt), p[dim]);
-    orow(r)[dim] = requantize((int64_t)v);
+    orow(r)[dim] = requantize_flat((int64_t)v);
   };
   if (warp < kTrConvWarps && total > 0) {
     constexpr int kQ = NR / 4;
@@ -966,7 +1014,7 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
   __syncthreads();
   if (s_fail && tid == 0) atomicExch(&g_tree_err, 1);
   fence_after();
-  if (warp == kTrConvWarps) ta_dealloc<kTmem>(tmem);
+  if (warp == kTrConvWarps) ta_dealloc<512>(tmem);
 }
 
 template <int NR, bool VEC>
@@ -975,9 +1023,9 @@ void qk_attr() {
   for (int ns = 1; ns <= 8; ++ns) most = std::max(most, qk_smem<NR>(ns));
   cudaFuncSetAttribute(tree_qk<NR, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
 }
-template <int NR>
+template <int NR, bool VEC>
 void pv_attr() {
-  cudaFuncSetAttribute(tree_pv<NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, pv_smem<NR>());
+  cudaFuncSetAttribute(tree_pv<NR, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, pv_smem<NR>());
 }
 
 }  // namespace
@@ -989,9 +1037,12 @@ void tree_attn_init() {
   qk_attr<32, false>();
   qk_attr<64, true>();
   qk_attr<64, false>();
-  pv_attr<16>();
-  pv_attr<32>();
-  pv_attr<64>();
+  pv_attr<16, true>();
+  pv_attr<16, false>();
+  pv_attr<32, true>();
+  pv_attr<32, false>();
+  pv_attr<64, true>();
+  pv_attr<64, false>();
 }
 
 int tree_attn_error_flag(bool reset) {
@@ -1093,23 +1144,26 @@ size_t tree_attn_plan(TreeGroup& g) {
   return (size_t)up(g.cnt_off + (int64_t)counters * 4);
 }
 
-template <int NR>
-static void tree_launch(const TreeGroup& g, bool vec, cudaStream_t s) {
+template <int NR, bool VEC>
+static void tree_launch(const TreeGroup& g, cudaStream_t s) {
   const int ns = (g.d + 63) / 64;
-  if (vec) ta_launch(tree_qk<NR, true>, dim3(g.qk_items), dim3(kQkThreads), qk_smem<NR>(ns), 1, s, g);
-  else ta_launch(tree_qk<NR, false>, dim3(g.qk_items), dim3(kQkThreads), qk_smem<NR>(ns), 1, s, g);
+  ta_launch(tree_qk<NR, VEC>, dim3(g.qk_items), dim3(kQkThreads), qk_smem<NR>(ns), 1, s, g);
   ta_launch(tree_exp, dim3((unsigned)g.rows * g.ex_chunks), dim3(kExThreads), 0, 1, s, g);
-  ta_launch(tree_pv<NR>, dim3(g.pv_items), dim3(kPvThreads), pv_smem<NR>(), 1, s, g);
+  ta_launch(tree_pv<NR, VEC>, dim3(g.pv_items), dim3(kPvThreads), pv_smem<NR>(), 1, s, g);
 }
 
 void launch_tree_attn(const TreeGroup& g, cudaStream_t s) {
+  // 16-byte copies where every row is 16-byte aligned
   uintptr_t bits = reinterpret_cast<uintptr_t>(g.q);
-  for (int i = 0; i < g.nseq; ++i)
-    bits |= reinterpret_cast<uintptr_t>(g.seq[i].k) | reinterpret_cast<uintptr_t>(g.seq[i].kt);
+  for (int i = 0; i < g.nseq; ++i) {
+    const TreeSeq& t = g.seq[i];
+    bits |= reinterpret_cast<uintptr_t>(t.k) | reinterpret_cast<uintptr_t>(t.kt);
+    bits |= reinterpret_cast<uintptr_t>(t.v) | reinterpret_cast<uintptr_t>(t.vt);
+  }
   const bool vec = g.d % 4 == 0 && (bits & 15) == 0;
-  if (g.nr == 16) tree_launch<16>(g, vec, s);
-  else if (g.nr == 32) tree_launch<32>(g, vec, s);
-  else tree_launch<64>(g, vec, s);
+  if (g.nr == 16) vec ? tree_launch<16, true>(g, s) : tree_launch<16, false>(g, s);
+  else if (g.nr == 32) vec ? tree_launch<32, true>(g, s) : tree_launch<32, false>(g, s);
+  else vec ? tree_launch<64, true>(g, s) : tree_launch<64, false>(g, s);
 }
 
 }  // namespace rdet

@@ -30,6 +30,49 @@ static int64_t one(uint64_t e, uint64_t sum) {
   int32_t w;
   return softmax_weight_near(coded, softmax_inverse(sum), &w) && w != softmax_weight((int64_t)e, (int64_t)sum);
 }
+// the branch-free rounding, around every power of two, at every tie beside the
+// ends of the range and at random
+int64_t requantize_random(uint64_t seed, int64_t n) {
+  int64_t bad = 0;
+  auto check = [&](uint64_t v) { bad += requantize_flat((int64_t)v) != requantize((int64_t)v); };
+  for (int sh = 0; sh < 64; ++sh)
+    for (int64_t o = -70000; o <= 70000; ++o) {
+      check((1ull << sh) + (uint64_t)o);
+      check(0 - (1ull << sh) + (uint64_t)o);
+    }
+  for (int64_t i = 0; i < n; ++i) {
+    const uint64_t v = mix(seed + i);
+    check(v);
+    check((uint64_t)((int64_t)v >> (i % 64)));
+    check((uint64_t)((int64_t)v >> 16) & ~0xffffull | 0x8000u);
+  }
+  return bad;
+}
+// digit sums with an addend, against the same in 64 bits: random ones and ones
+// beside the ends of the range
+int64_t digits_random(uint64_t seed, int64_t n) {
+  int64_t bad = 0;
+  for (int64_t i = 0; i < n; ++i) {
+    int32_t c[7];
+    for (int g = 0; g < 7; ++g) {
+      const uint64_t z = mix(seed + 16 * i + g);
+      c[g] = (int32_t)(z >> 37) - (1 << 26);
+      if (z % 5 == 0) c[g] = 0;
+      if (z % 7 == 0) c[g] = z & 64 ? 1 << 26 : -(1 << 26);
+      if ((i & 3) && g > 3) c[g] = (int32_t)(z % 3) - 1;
+    }
+    uint64_t v = 0;
+    for (int g = 0; g < 7; ++g) v += (uint64_t)(int64_t)c[g] << (8 * g);
+    uint64_t add = mix(seed + 16 * i + 8) >> (i % 64);
+    if (i % 3 == 0) {  // the sum at a chosen place
+      const uint64_t at = mix(seed + 16 * i + 9);
+      add = ((at & 1 ? 1ull : ~0ull) << (at >> 8) % 64) + (uint64_t)((int64_t)((at >> 16) % 262144) - 131072) - v;
+    }
+    bad += requantize_digits(c[0], c[1], c[2], c[3], c[4], c[5], c[6], (int32_t)(add & 0xffff),
+                             (int32_t)(add >> 16 & 0xffff), (int32_t)(add >> 32)) != requantize((int64_t)(v + add));
+  }
+  return bad;
+}
 // how many of n random weights the reciprocal leaves open
 int64_t weights_open(uint64_t seed, int64_t n) {
   int64_t open = 0;

@@ -21,7 +21,8 @@ def host():
                         os.path.join(HERE, "draft_dev_host.cpp"), "-o", out], capture_output=True, text=True)
     assert r.returncode == 0, r.stderr
     L = C.CDLL(out)
-    for name, args in (("exp_all", [C.c_int32]), ("exp_second", []), ("weights_random", [C.c_uint64, C.c_int64]),
+    for name, args in (("requantize_random", [C.c_uint64, C.c_int64]), ("digits_random", [C.c_uint64, C.c_int64]),
+                        ("exp_all", [C.c_int32]), ("exp_second", []), ("weights_random", [C.c_uint64, C.c_int64]),
                        ("weights_ties", [C.c_uint64, C.c_int64]), ("weights_open", [C.c_uint64, C.c_int64]), ("weights_one", [C.c_int64])):
         getattr(L, name).argtypes, getattr(L, name).restype = args, C.c_int64
     return L
@@ -40,6 +41,11 @@ def test_the_code_of_one_is_free(host):
 def test_weights(host, seed):
     assert host.weights_random(seed * 10**9, 2_000_000) == 0
     assert host.weights_ties(seed * 10**9, 400_000) == 0
+
+
+def test_rounding_without_branches(host):
+    assert host.requantize_random(5, 2_000_000) == 0
+    assert host.digits_random(7 * 10**12, 4_000_000) == 0
 
 
 def test_weights_of_a_lone_key(host):
