@@ -410,7 +410,7 @@ struct TreeGroup {
   // value sums, weight sums and arrivals per value item
   int32_t G = 1, nr = 0, qk_tiles = 1, ex_keys = 0, ex_chunks = 1, qk_items = 0, pv_items = 0, rows = 0;
   int32_t qk_first[kTreeGroupSeqs], pv_first[kTreeGroupSeqs], row_first[kTreeGroupSeqs];
-  int64_t max_off = 0, sum_off = 0, idx_off = 0, acc_off = 0, wt_off = 0, cnt_off = 0;
+  int64_t max_off = 0, sum_off = 0, idx_off = 0, acc_off = 0, cnt_off = 0;
 };
 size_t tree_attn_plan(TreeGroup& g);           // returns the workspace bytes
 void launch_tree_attn(const TreeGroup& g, cudaStream_t s);

@@ -209,6 +209,19 @@ __device__ __forceinline__ void ta_st4(uint32_t taddr, uint32_t a, uint32_t b, u
 }
 __device__ __forceinline__ void ta_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// thread-block cluster: barrier, and the word at the same place in CTA `rank`
+__device__ __forceinline__ void ta_cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void ta_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint64_t ta_ld_cluster(const uint64_t* p, int rank) {
+  uint64_t v;
+  asm volatile(
+      "{\n .reg .b32 a;\n mapa.shared::cluster.u32 a, %1, %2;\n ld.shared::cluster.u64 %0, [a];\n}"
+      : "=l"(v)
+      : "r"(su32(p)), "r"(rank)
+      : "memory");
+  return v;
+}
+
 // asynchronous copies into shared memory, zeros where `on` is false, and their
 // arrival on a barrier once all of the thread's copies so far are there
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool on) {
@@ -629,12 +642,16 @@ __global__ void __launch_bounds__(kQkThreads, 1) tree_qk(const __grid_constant__
 }
 
 // ---------------------------------------------------------------------------
-// exp terms: a CTA takes one chunk of keys of one row.  Terms replace the
-// scores, as u32: the one value of 2^32 (a score equal to the maximum) is
+// Softmax: a cluster takes a row, a CTA one chunk of its keys.  The chunk's exp
+// terms stay in shared memory while the cluster adds up its sums; the weights'
+// digits then replace the scores, as the value kernel's operand tiles want them
+// (three planes of 64 bytes per 64 keys, at every 256 bytes of the row).  A
+// term is held as u32: the one value of 2^32 (a score equal to the maximum) is
 // coded 2^32 - 1, which no other score gives (the next lower score's term is
 // below 2^32 - 2^15).
 // ---------------------------------------------------------------------------
 constexpr int kExThreads = 256;
+constexpr int kExMostKeys = 32768;  // of a CTA: 128 KB of terms
 
 __device__ __forceinline__ uint64_t ta_warp_sum(uint64_t v) {
 #pragma unroll
@@ -642,12 +659,14 @@ __device__ __forceinline__ uint64_t ta_warp_sum(uint64_t v) {
   return v;
 }
 
-__global__ void __launch_bounds__(kExThreads) tree_exp(const __grid_constant__ TreeGroup g) {
-  __shared__ uint64_t red[kExThreads / 32];
-  __shared__ int32_t redi[kExThreads / 32];
+__global__ void __launch_bounds__(kExThreads) tree_softmax(const __grid_constant__ TreeGroup g) {
+  extern __shared__ __align__(16) unsigned char tr_raw[];
+  uint4* const terms = reinterpret_cast<uint4*>(tr_raw);  // four keys each
+  __shared__ uint64_t red[kExThreads / 32], s_part;
+  __shared__ int32_t redi[kExThreads / 32], redw[kExThreads / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // row of the group: (sequence, KV head, node, head of the KV head's group)
-  const int grow = blockIdx.x / g.ex_chunks, chunk = blockIdx.x - grow * g.ex_chunks;
+  const int C = g.ex_chunks, grow = blockIdx.x / C, chunk = blockIdx.x - grow * C;
   const int si = seq_of(g.row_first, g.nseq, grow);
   const TreeSeq t = g.seq[si];
   const int rows = t.n * g.G, lrow = grow - g.row_first[si], rr = lrow % rows;
@@ -662,18 +681,16 @@ __global__ void __launch_bounds__(kExThreads) tree_exp(const __grid_constant__ T
     uint64_t* acc = reinterpret_cast<uint64_t*>(ws + g.acc_off) + (int64_t)grow * g.d;
     for (int i = tid; i < g.d; i += kExThreads) acc[i] = 0;
     const int items = t.cfirst + (lrow / rows * ((rows + g.nr - 1) / g.nr) + rr / g.nr) * ((g.d + 127) / 128);
-    if (tid < (g.d + 127) / 128) reinterpret_cast<int32_t*>(ws + g.wt_off)[(int64_t)tid * g.rows + grow] = 0;
     if (rr % g.nr == 0 && tid < (g.d + 127) / 128) reinterpret_cast<uint32_t*>(ws + g.cnt_off)[items + tid] = 0;
   }
-  const int k0 = chunk * g.ex_keys, k1 = min(t.pad, k0 + g.ex_keys);
-  if (k0 >= k1 && chunk > 0) return;
+  const int k0 = chunk * g.ex_keys, k1 = min(t.pad, k0 + g.ex_keys);  // (k0 >= k1: no keys)
   uint32_t top = 0;
   for (int i = lane; i < t.qk_per; i += 32) top = max(top, tmax[i]);
   const uint32_t m = __reduce_max_sync(0xffffffffu, top) ^ 0x80000000u;
   uint64_t sum = 0;
   int32_t first = INT32_MAX;  // the thread's first key at the maximum
   for (int j = k0 + 4 * tid; j < k1; j += 4 * kExThreads) {
-    uint4 v = *reinterpret_cast<const uint4*>(sc + j);
+    const uint4 v = *reinterpret_cast<const uint4*>(sc + j);
     const int key = t.lo + j;
     uint32_t vis = 15u;
     if (!(key >= start && key + 3 < t.ctx)) {
@@ -689,8 +706,7 @@ __global__ void __launch_bounds__(kExThreads) tree_exp(const __grid_constant__ T
       first = min(first, j + i);
       return 0xffffffffu;
     };
-    v = make_uint4(term(v.x, 0), term(v.y, 1), term(v.z, 2), term(v.w, 3));
-    *reinterpret_cast<uint4*>(sc + j) = v;
+    terms[(j - k0) >> 2] = make_uint4(term(v.x, 0), term(v.y, 1), term(v.z, 2), term(v.w, 3));
   }
   sum = ta_warp_sum(sum);
   first = __reduce_min_sync(0xffffffffu, first);
@@ -699,14 +715,38 @@ __global__ void __launch_bounds__(kExThreads) tree_exp(const __grid_constant__ T
     redi[warp] = first;
   }
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kExThreads / 32; ++w) {
-      sum += red[w];
-      first = min(first, redi[w]);
-    }
-    reinterpret_cast<uint64_t*>(ws + g.sum_off)[(int64_t)grow * g.ex_chunks + chunk] = sum;
-    reinterpret_cast<int32_t*>(ws + g.idx_off)[(int64_t)grow * g.ex_chunks + chunk] = first;
+  sum = ta_warp_sum(lane < kExThreads / 32 ? red[lane] : 0);
+  first = __reduce_min_sync(0xffffffffu, lane < kExThreads / 32 ? redi[lane] : INT32_MAX);
+  if (C > 1) {
+    if (tid == 0) s_part = sum;
+    ta_cluster_arrive();
+    ta_cluster_wait();
+    sum = ta_warp_sum(lane < C ? ta_ld_cluster(&s_part, lane) : 0);
+    ta_cluster_arrive();  // (waited for before the CTA ends: its part is read by the others)
   }
+  const uint32_t inv = softmax_inverse(sum);
+  int32_t wsum = 0;
+  for (int j = k0 + 4 * tid; j < k1; j += 4 * kExThreads) {
+    const uint4 e = terms[(j - k0) >> 2];
+    const int32_t w0 = ta_weight(e.x, inv, sum), w1 = ta_weight(e.y, inv, sum), w2 = ta_weight(e.z, inv, sum),
+                  w3 = ta_weight(e.w, inv, sum);
+    wsum += w0 + w1 + w2 + w3;
+    uint32_t o[4];
+    ta_t4(ta_digits(w0), ta_digits(w1), ta_digits(w2), ta_digits(w3), o);
+    // (a chunk of 64 keys lies with 16 neighbouring threads, whose scores it replaces)
+    uint32_t* const out = reinterpret_cast<uint32_t*>(sc) + (j & ~63) + ((j & 63) >> 2);
+#pragma unroll
+    for (int a = 0; a < 3; ++a) out[16 * a] = o[a];
+  }
+  wsum = __reduce_add_sync(0xffffffffu, wsum);
+  if (lane == 0) redw[warp] = wsum;
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < kExThreads / 32; ++w) wsum += redw[w];
+    reinterpret_cast<int32_t*>(ws + g.sum_off)[(int64_t)grow * C + chunk] = wsum;
+    reinterpret_cast<int32_t*>(ws + g.idx_off)[(int64_t)grow * C + chunk] = first;
+  }
+  if (C > 1) ta_cluster_wait();
 }
 
 // ---------------------------------------------------------------------------
@@ -719,32 +759,27 @@ __global__ void __launch_bounds__(kExThreads) tree_exp(const __grid_constant__ T
 // ---------------------------------------------------------------------------
 // A stage is 64 keys of the 128 dims, 32 KB as they are in a ring of slots; the
 // value bytes go to the MMAs through TMEM like the key bytes above (a thread
-// holds one dim of 16 keys), the weights' digits through shared memory.
-constexpr int kPvStages = 6;  // slots
-constexpr int kPvW = 4;       // weight tiles
+// holds one dim of 16 keys); the weights' digits, operand B, lie behind them.
+constexpr int kPvStages = 6;
 template <int NR>
-__host__ __device__ constexpr int pv_stages() { return NR == 64 ? 5 : kPvStages; }
+__host__ __device__ constexpr int pv_slot() { return kTrPlanes + 3 * NR * 64; }
 template <int NR>
-__host__ __device__ constexpr int pv_smem() { return pv_stages<NR>() * kTrPlanes + kPvW * 3 * NR * 64 + 512; }
+__host__ __device__ constexpr int pv_stages() { return NR == 16 ? kPvStages : 5; }
+template <int NR>
+__host__ __device__ constexpr int pv_smem() { return pv_stages<NR>() * pv_slot<NR>() + 512; }
 
 template <int NR, bool VEC>
 __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__ TreeGroup g) {
   constexpr int kA = 448;                       // TMEM column of operand A's two units
-  constexpr int kSt = pv_stages<NR>();
-  constexpr int kW = 3 * NR * 64;               // one stage's weight tile
-  constexpr int kE = (NR * 16 + kTrConv - 1) / kTrConv;  // (row, four keys) pieces of it per converter thread
+  constexpr int kSt = pv_stages<NR>(), kSlot = pv_slot<NR>();
   extern __shared__ __align__(16) unsigned char tr_raw[];
   unsigned char* sm = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(tr_raw) + 511) & ~(uintptr_t)511);
-  unsigned char* slots = sm;                    // [slot][64 keys][128 dims]
-  unsigned char* wsm = sm + kSt * kTrPlanes;    // [tile][3 NR rows][64 keys]
-  __shared__ __align__(8) uint64_t raw_full[kPvStages], raw_empty[kPvStages], a_full[2], a_empty[2], w_full[kPvW], w_empty[kPvW],
-      acc_full;
+  unsigned char* slots = sm;                    // [slot][64 keys][128 dims], [3 NR rows][64 keys]
+  __shared__ __align__(8) uint64_t raw_full[kPvStages], raw_empty[kPvStages], a_full[2], a_empty[2], acc_full;
   __shared__ uint32_t tmem_holder;
   __shared__ int s_fail;
-  __shared__ uint64_t s_sum[NR];                // each row's sum of terms
-  __shared__ int32_t s_first[NR];               // its first maximum
-  __shared__ uint32_t s_inv[NR];
-  __shared__ int32_t s_wsum[NR];                // each row's sum of this CTA's weights
+  __shared__ int32_t s_first[NR];               // each row's first maximum
+  __shared__ int32_t s_wsum[NR];                // its sum of weights
   __shared__ uint32_t s_last;
   const int tid = threadIdx.x, warp = ta_warp(), lane = tid & 31;
 
@@ -758,7 +793,7 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
   const int r0 = rb * NR, nr = min(NR, rows - r0), total = c1 - c0;
   const int lrow0 = kvh * rows + r0, grow0 = g.row_first[si] + lrow0;
   unsigned char* const ws = static_cast<unsigned char*>(g.ws);
-  const uint32_t* const ex = reinterpret_cast<const uint32_t*>(ws) + t.soff + (int64_t)lrow0 * t.pad + c0 * 64;
+  const unsigned char* const wts = ws + 4 * (t.soff + (int64_t)lrow0 * t.pad + c0 * 64);  // 256 bytes per row and stage
   const int32_t* const vc = t.v + (int64_t)kvh * t.kstride;
   const int32_t* const vt = t.vt + (int64_t)kvh * t.tstride;
   const int last_key = t.lo + t.len - 1;
@@ -767,7 +802,7 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
   // dims past the head (their sums are not stored) are zero.
   int lu = 0, lb = 0, lph = 1;  // next stage, its slot and the parity of the slot's last use
   auto load = [&]() {
-    const uint32_t slot = su32(slots) + lb * kTrPlanes;
+    const uint32_t slot = su32(slots) + lb * kSlot;
     const int key0 = t.lo + (c0 + lu) * 64, p = tid & (kTrLoaders - 1);
     if (VEC) {  // 16 bytes of keys p / 32, p / 32 + 2, ..
       const int dim = db * 128 + 4 * (p & 31), row0 = p >> 5;
@@ -792,30 +827,31 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
             dim < d && key0 + k <= last_key);
       }
     }
-    cp_arrive(&raw_full[lb]);
     ++lu;
     if (++lb == kSt) { lb = 0; lph ^= 1; }
   };
-  // its part of the weights: rows tid / 16 + 32 i (at most the block's last),
-  // keys 4 (tid % 16) .. + 4
-  const int wr = tid >> 4, wq = tid & 15;
-  uint4 ev[kE] = {};
-  auto load_e = [&](int u) {
+  // Stage u's weights into slot b, and the stage's arrival: 16 bytes of rows
+  // p / 4, p / 4 + 16, .. (rows past the block are zero)
+  auto load_w = [&](int u, int b) {
+    const int p = tid & (kTrLoaders - 1), c = p & 3;
+    const uint32_t dst = su32(slots) + b * kSlot + kTrPlanes;
 #pragma unroll
-    for (int i = 0; i < kE; ++i) ld16(ev[i], ex + (int64_t)min(wr + 32 * i, nr - 1) * t.pad + u * 64 + 4 * wq, u < total);
+    for (int i = 0; i < NR / 16; ++i) {
+      const int r = (p >> 2) + 16 * i;
+      const unsigned char* src = wts + (int64_t)min(r, nr - 1) * t.pad * 4 + u * 256 + 16 * c;
+#pragma unroll
+      for (int a = 0; a < 3; ++a) cp16(dst + ta_sw(a * NR + r, c), src + 64 * a, r < nr);
+    }
+    cp_arrive(&raw_full[b]);
   };
   if (tid == 0) {
     for (int i = 0; i < kSt; ++i) {
       mbar_init(&raw_full[i], kTrLoaders);
-      mbar_init(&raw_empty[i], kTrConvWarps);
+      mbar_init(&raw_empty[i], kTrConvWarps + 1);  // the converters have read the values, the MMAs the weights
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&a_full[i], kTrConvWarps / 2);
       mbar_init(&a_empty[i], 1);
-    }
-    for (int i = 0; i < kPvW; ++i) {
-      mbar_init(&w_full[i], kTrConvWarps);
-      mbar_init(&w_empty[i], 1);
     }
     mbar_init(&acc_full, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -830,18 +866,17 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
     for (int u = 0; u < min(kSt, total); ++u) load();
   ta_wait();
   ta_go();
-  if (warp < kTrConvWarps) load_e(0);
-  const uint64_t* psum = reinterpret_cast<const uint64_t*>(ws + g.sum_off);
-  const int32_t* pidx = reinterpret_cast<const int32_t*>(ws + g.idx_off);
-  const int nsum = (t.pad + g.ex_keys - 1) / g.ex_keys;  // chunks of this sequence's rows
+  if (warp > kTrConvWarps)
+    for (int u = 0; u < min(kSt, total); ++u) load_w(u, u);
+  const int32_t* pw = reinterpret_cast<const int32_t*>(ws + g.sum_off) + (int64_t)grow0 * g.ex_chunks;
+  const int32_t* pidx = reinterpret_cast<const int32_t*>(ws + g.idx_off) + (int64_t)grow0 * g.ex_chunks;
   if (tid < 8 * NR) {  // eight lanes a row
     const int r = tid >> 3;
-    uint64_t v = 0;
-    int32_t f = INT32_MAX;
+    int32_t v = 0, f = INT32_MAX;
     if (r < nr)
-      for (int i = tid & 7; i < nsum; i += 8) {
-        v += psum[(int64_t)(grow0 + r) * g.ex_chunks + i];
-        f = min(f, pidx[(int64_t)(grow0 + r) * g.ex_chunks + i]);
+      for (int i = tid & 7; i < g.ex_chunks; i += 8) {
+        v += pw[r * g.ex_chunks + i];
+        f = min(f, pidx[r * g.ex_chunks + i]);
       }
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) {
@@ -849,10 +884,8 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
       f = min(f, __shfl_xor_sync(0xffffffffu, f, o));
     }
     if ((tid & 7) == 0) {
-      s_sum[r] = v;
       s_first[r] = f;
-      s_inv[r] = r < nr ? softmax_inverse(v) : 0;
-      s_wsum[r] = 0;
+      s_wsum[r] = v;
     }
   }
   fence_before();
@@ -869,35 +902,13 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
     const int grp = warp >> 2, h = grp >> 1;
     const uint32_t at = ((uint32_t)(32 * (warp & 3)) << 16) + kA + 32 * h + 4 * (grp & 1);
     const unsigned char* const col = slots + 16 * grp * 512 + 4 * (32 * (warp & 3) + lane);
-    int32_t wsum[kE] = {};
     int pb = 0, ph = 0;
     for (int u = 0; u < total; ++u) {
-      // weights first: they need the values' MMAs before the last ones only
-      const int wb = u & (kPvW - 1);
-      if (u >= kPvW) wait(&w_empty[wb], (u / kPvW - 1) & 1);
-#pragma unroll
-      for (int i = 0; i < kE; ++i) {
-        const int r = wr + 32 * i;
-        if (r >= NR) break;
-        const uint32_t inv = s_inv[r];
-        const uint64_t sum = s_sum[r];
-        const int32_t w0 = ta_weight(ev[i].x, inv, sum), w1 = ta_weight(ev[i].y, inv, sum),
-                      w2 = ta_weight(ev[i].z, inv, sum), w3 = ta_weight(ev[i].w, inv, sum);
-        wsum[i] += w0 + w1 + w2 + w3;
-        uint32_t o[4];
-        ta_t4(ta_digits(w0), ta_digits(w1), ta_digits(w2), ta_digits(w3), o);
-#pragma unroll
-        for (int a = 0; a < 3; ++a)
-          *reinterpret_cast<uint32_t*>(wsm + wb * kW + ta_sw(a * NR + r, wq >> 2) + 4 * (wq & 3)) = o[a];
-      }
-      ta_fence_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&w_full[wb]);
-      load_e(u + 1);
       wait(&raw_full[pb], ph);
+      ta_fence_async();  // the weights' tile, for the MMAs
       uint32_t x[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] = *reinterpret_cast<const uint32_t*>(col + pb * kTrPlanes + 512 * i);
+      for (int i = 0; i < 16; ++i) x[i] = *reinterpret_cast<const uint32_t*>(col + pb * kSlot + 512 * i);
       uint32_t o[4][4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) ta_bytes(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3], o[i]);
@@ -913,24 +924,15 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
       __syncwarp();
       if (lane == 0) mbar_arrive(&a_full[h]);
     }
-    // a row's weights lie in the 16 threads of its keys
-#pragma unroll
-    for (int i = 0; i < kE; ++i) {
-      int32_t v = wsum[i];
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-      if (wq == 0 && wr + 32 * i < NR) s_wsum[wr + 32 * i] = v;
-    }
   } else if (warp == kTrConvWarps) {
     const bool leader = ta_elect();
     const uint32_t full = ta_idesc(3 * NR), low = ta_idesc(2 * NR), one = ta_idesc(NR);
-    const uint64_t wdesc = smem_desc_sw64(su32(wsm));
+    const uint64_t wdesc = smem_desc_sw64(su32(slots) + kTrPlanes);
+    int pb = 0;
     for (int u = 0; u < total; ++u) {
-      const int wb = u & (kPvW - 1);
-      wait(&w_full[wb], (u / kPvW) & 1);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint64_t wd = ta_adv(wdesc, wb * kW + 32 * h);
+        const uint64_t wd = ta_adv(wdesc, pb * kSlot + 32 * h);
         const uint32_t a = tmem + kA + 32 * h;
         wait(&a_full[h], u & 1);
         fence_after();
@@ -947,17 +949,20 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
             for (int b = 0; b < 4; ++b) ta_mma(tmem + b * NR, a + 8 * b, wd, full, 1);
           }
           mma_commit(&a_empty[h]);
-          if (h == 1) mma_commit(&w_empty[wb]);
+          if (h == 1) mma_commit(&raw_empty[pb]);
           if (h == 1 && u == total - 1) mma_commit(&acc_full);
         }
         __syncwarp();
       }
+      if (++pb == kSt) pb = 0;
     }
     if (total > 0) wait(&acc_full, 0);
   } else {
     for (int u = kSt; u < total; ++u) {
       wait(&raw_empty[lb], lph);
+      const int b = lb;
       load();
+      load_w(u, b);
     }
     cp_wait_all();
   }
@@ -969,11 +974,11 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
     const int rr = r0 + r, node = rr / G;
     return g.out + ((int64_t)(t.node0 + node) * Hq + kvh * G + (rr - node * G)) * d;
   };
-  // Row r's sum v of digit products and wt of weights to the output: the bytes'
+  // Row r's sum v of digit products to the output: the bytes'
   // bias, and what the weights' roundings left times the first maximum's value.
   unsigned long long* const acc = reinterpret_cast<unsigned long long*>(ws + g.acc_off) + (int64_t)grow0 * d;
-  int32_t* const wtot = reinterpret_cast<int32_t*>(ws + g.wt_off) + (int64_t)db * g.rows + grow0;  // sums of weights
-  auto finish = [&](int r, uint64_t v, int32_t wt) {
+  auto finish = [&](int r, uint64_t v) {
+    const int32_t wt = s_wsum[r];
     const int key = t.lo + s_first[r];
     const int32_t* p = key < t.ctx ? vc + (int64_t)key * d : vt + (int64_t)(key - t.ctx) * d;
     v += (uint64_t)(kTrBias * wt) + (uint64_t)mul_wide(sub_sat(kOneAct, wt), p[dim]);
@@ -992,14 +997,13 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
         const int64_t v = shift_sum(0, c[0][i], c[1][i], c[2][i], c[3][i], c[4][i], c[5][i], 0);
         if (r + i < nr && dim < d) {
           if (S > 1) atomicAdd(acc + (int64_t)(r + i) * d + dim, (unsigned long long)v);
-          else finish(r + i, (uint64_t)v, s_wsum[r + i]);
+          else finish(r + i, (uint64_t)v);
         }
       }
     }
   }
   if (S > 1) {
     uint32_t* const cnt = reinterpret_cast<uint32_t*>(ws + g.cnt_off) + t.cfirst + it;
-    if (tid < nr && total > 0) atomicAdd(wtot + tid, s_wsum[tid]);
     __threadfence();
     __syncthreads();
     if (tid == 0) s_last = atomicAdd(cnt, 1u) == (uint32_t)S - 1;
@@ -1007,7 +1011,7 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
     if (s_last && warp < kTrConvWarps && dim < d) {
       __threadfence();
       for (int r = quarter; r < nr; r += 4)
-        finish(r, __ldcg(acc + (int64_t)r * d + dim), __ldcg(wtot + r));
+        finish(r, __ldcg(acc + (int64_t)r * d + dim));
     }
   }
   fence_before();
@@ -1037,6 +1041,8 @@ void tree_attn_init() {
   qk_attr<32, false>();
   qk_attr<64, true>();
   qk_attr<64, false>();
+  cudaFuncSetAttribute(tree_softmax, cudaFuncAttributeMaxDynamicSharedMemorySize, 4 * kExMostKeys);
+  cudaFuncSetAttribute(tree_softmax, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   pv_attr<16, true>();
   pv_attr<16, false>();
   pv_attr<32, true>();
@@ -1130,17 +1136,19 @@ size_t tree_attn_plan(TreeGroup& g) {
   g.rows = rows;
   g.pv_items = pv;
   g.qk_items = qk;
-  // keys of one term CTA: four per thread, more where the rows alone fill the GPU
+  // Keys of a softmax CTA: four per thread, more where the rows alone fill the
+  // GPU, and so many that a row's cluster has at most eight CTAs (sixteen for the longest).
   g.ex_keys = 4 * kExThreads;
-  while (g.ex_keys < 16 * kExThreads && (int64_t)rows * (maxpad / g.ex_keys) > 32 * kSms) g.ex_keys *= 2;
-  g.ex_chunks = (maxpad + g.ex_keys - 1) / g.ex_keys;
+  while ((g.ex_keys < 16 * kExThreads && (int64_t)rows * (maxpad / g.ex_keys) > 32 * kSms) ||
+         ceil_div(maxpad, g.ex_keys) > (g.ex_keys < kExMostKeys ? 8 : 16))
+    g.ex_keys *= 2;
+  g.ex_chunks = ceil_div(maxpad, g.ex_keys);
   auto up = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
   g.max_off = up(soff * 4);
   g.sum_off = up(g.max_off + moff * 4);
-  g.idx_off = up(g.sum_off + (int64_t)rows * g.ex_chunks * 8);
+  g.idx_off = up(g.sum_off + (int64_t)rows * g.ex_chunks * 4);
   g.acc_off = up(g.idx_off + (int64_t)rows * g.ex_chunks * 4);
-  g.wt_off = up(g.acc_off + (int64_t)rows * g.d * 8);
-  g.cnt_off = up(g.wt_off + (int64_t)nd * rows * 4);
+  g.cnt_off = up(g.acc_off + (int64_t)rows * g.d * 8);
   return (size_t)up(g.cnt_off + (int64_t)counters * 4);
 }
 
@@ -1148,7 +1156,7 @@ template <int NR, bool VEC>
 static void tree_launch(const TreeGroup& g, cudaStream_t s) {
   const int ns = (g.d + 63) / 64;
   ta_launch(tree_qk<NR, VEC>, dim3(g.qk_items), dim3(kQkThreads), qk_smem<NR>(ns), 1, s, g);
-  ta_launch(tree_exp, dim3((unsigned)g.rows * g.ex_chunks), dim3(kExThreads), 0, 1, s, g);
+  ta_launch(tree_softmax, dim3((unsigned)g.rows * g.ex_chunks), dim3(kExThreads), 4 * (size_t)g.ex_keys, g.ex_chunks, s, g);
   ta_launch(tree_pv<NR, VEC>, dim3(g.pv_items), dim3(kPvThreads), pv_smem<NR>(), 1, s, g);
 }
 
