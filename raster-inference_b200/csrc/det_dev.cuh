@@ -303,25 +303,26 @@ RDET_HD uint32_t acc_mul_rte(uint32_t a, uint32_t b) {
   const uint64_t p = (uint64_t)a * b;
   return (uint32_t)((p + 0x7fffffffull + ((p >> 32) & 1)) >> 32);
 }
-// v / d for a constant even d, ties to even: up iff 2 r + (q odd) > d
+// v / d for a constant even d and v + d / 2 < 2^32, ties to even: half up,
+// less one where that was a tie with an odd result
 RDET_HD uint32_t div_rte(uint32_t v, uint32_t d) {
-  const uint32_t q = v / d, r = v - q * d;
-  return q + (2 * r + (q & 1) > d ? 1u : 0u);
+  const uint32_t h = v + d / 2, q = h / d;
+  return q * d == h ? q & ~1u : q;
 }
-// exp_term(max - D, max) for 0 <= D < 16 * 2^16 in 32-bit pieces.  The number
-// of halvings floor(D 2^16 / ln2) is one multiply by 2^62 / ln2 rounded down
-// (the host test compares every D with exp_term).
-RDET_HD uint64_t exp_term_below(uint32_t D) {
+// exp_term(max - D, max) for 0 < D < 16 * 2^16 (below 2^32) in 32-bit pieces.
+// The number of halvings floor(D 2^16 / ln2) is one multiply by 2^62 / ln2
+// rounded down (the host test compares every D with exp_term).
+RDET_HD uint32_t exp_term_below(uint32_t D) {
   const uint32_t LN2 = 2977044472u;
-  uint32_t shift = (uint32_t)(((uint64_t)D * 1549082004u) >> 46);  // <= 23
-  uint32_t r = (D << 16) - shift * LN2;                             // exact mod 2^32, below ln2
+  const uint32_t shift = (uint32_t)(((uint64_t)D * 1549082004u) >> 46);  // <= 23
+  const uint32_t r = (D << 16) - shift * LN2;                             // exact mod 2^32, below ln2
   const uint32_t r2 = acc_mul_rte(r, r), r3 = acc_mul_rte(r2, r), r4 = acc_mul_rte(r3, r), r5 = acc_mul_rte(r4, r);
   // the terms after 1 - r sum to a value in [0, 2^31): one 32-bit sum
   const uint32_t tail = ((r2 >> 1) + (r2 & (r2 >> 1) & 1)) - div_rte(r3, 6) + div_rte(r4, 24) - div_rte(r5, 120);
-  const uint64_t e = kOneAcc - (uint64_t)r + tail;  // > 0: at least 2^32 (1 - ln2)
-  if (shift == 0) return e;
-  const uint64_t half = (1ull << (shift - 1)) - 1 + ((e >> shift) & 1);
-  return (e + half) >> shift;
+  const uint32_t e = tail - r;  // 2^32 - r + tail, at least 2^32 (1 - ln2); r > 0
+  // e / 2^shift, ties to even: the bits shifted out, at the top of a word, against a half
+  const uint32_t q = e >> shift, out = (e << 1) << (31 - shift);
+  return q + (out + (q & 1) > 0x80000000u ? 1u : 0u);
 }
 
 // Softmax weights against one sum without a division each.  inv is 2^64 / sum

@@ -65,10 +65,10 @@ constexpr int kTrPlane = 128 * 64;     // one digit plane of a stage: 128 rows o
 constexpr int kTrPlanes = 4 * kTrPlane;
 constexpr int kTrConv = 512;           // converter threads (warps 0-15)
 constexpr int kTrConvWarps = kTrConv / 32;
-constexpr int kQkThreads = 736;        // + warps 16-19 drain, warp 20 issues the MMAs, warps 21-22 load
+constexpr int kQkThreads = 800;        // + warps 16-19 drain, warp 20 issues the MMAs, warps 21-24 load
 constexpr int kQkDrainWarps = 20;      // warps 0-19
-constexpr int kTrLoaders = 64;         // loading threads
-constexpr int kPvThreads = 608;        // + warp 16 issues the MMAs, warps 17-18 load
+constexpr int kTrLoaders = 128;        // loading threads (64 took as long to issue a stage's copies as its MMAs take)
+constexpr int kPvThreads = 672;        // + warp 16 issues the MMAs, warps 17-20 load
 constexpr int kTrMaxDigit = 0x7f7f7f7f;
 constexpr int kTrSplitKeys = 32704;    // keys of one value CTA at most: 3 * 2^14 each in s32
 
@@ -442,32 +442,33 @@ __global__ void __launch_bounds__(kQkThreads, 1) tree_qk(const __grid_constant__
   };
 
   // Stage u into its slot.  Keys past the sequence and dims past the head are zero.
+  const int lp = tid - (kQkThreads - kTrLoaders);
   int lt = t0, ls = 0, lb = 0, lph = 1;  // next stage's tile, chunk, slot and the parity of the slot's last use
   auto load = [&]() {
     const uint32_t slot = su32(slots) + lb * kTrPlanes;
-    const int key0 = t.lo + lt * kTrKeys, p = tid & (kTrLoaders - 1);
-    if (VEC) {  // 16 bytes of keys p / 16, p / 16 + 4, ..
-      const int dim = ls * 64 + 4 * (p & 15), row0 = p >> 4;
+    const int key0 = t.lo + lt * kTrKeys;
+    if (VEC) {  // 16 bytes of keys p / 16, p / 16 + 8, ..
+      const int p = lp, dim = ls * 64 + 4 * (p & 15), row0 = p >> 4;
       const bool on = dim < d;
-      const uint32_t dst0 = slot + row0 * 256 + 16 * ((p & 15) ^ row0), dst1 = dst0 ^ 64;  // even, odd i: bit 2 of the row
+      const uint32_t dst = slot + row0 * 256 + 16 * ((p & 15) ^ row0);
       const int od = on ? dim : 0;
       if (key0 + kTrKeys <= t.ctx) {  // cache rows only
         const int32_t* src = kc + (int64_t)(key0 + row0) * d + od;
-#pragma unroll 8
-        for (int i = 0; i < 32; ++i) cp16((i & 1 ? dst1 : dst0) + i * 1024, src + (int64_t)i * (4 * d), on);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) cp16(dst + i * 2048, src + (int64_t)i * (8 * d), on);
       } else {
-        for (int i = 0; i < 32; ++i) {
-          const int key = min(key0 + row0 + 4 * i, last_key);
-          cp16((i & 1 ? dst1 : dst0) + i * 1024, (key < t.ctx ? kc + (int64_t)key * d : kt + (int64_t)(key - t.ctx) * d) + od,
-               on && key0 + row0 + 4 * i <= last_key);
+        for (int i = 0; i < 16; ++i) {
+          const int key = min(key0 + row0 + 8 * i, last_key);
+          cp16(dst + i * 2048, (key < t.ctx ? kc + (int64_t)key * d : kt + (int64_t)(key - t.ctx) * d) + od,
+               on && key0 + row0 + 8 * i <= last_key);
         }
       }
-    } else {  // one dim of every key
-      const int dim = ls * 64 + p, od = min(dim, d - 1);
-      for (int i = 0; i < kTrKeys; ++i) {
+    } else {  // one dim of every other key
+      const int p = lp & 63, dim = ls * 64 + p, od = min(dim, d - 1);
+      for (int i = lp >> 6; i < kTrKeys; i += 2) {
         const int key = min(key0 + i, last_key);
-        cp4(slot + i * 256 + 16 * ((p >> 2) ^ (i & 7)) + 4 * (p & 3), (key < t.ctx ? kc + (int64_t)key * d : kt + (int64_t)(key - t.ctx) * d) + od,
-            dim < d && key0 + i <= last_key);
+        cp4(slot + i * 256 + 16 * ((p >> 2) ^ (i & 7)) + 4 * (p & 3),
+            (key < t.ctx ? kc + (int64_t)key * d : kt + (int64_t)(key - t.ctx) * d) + od, dim < d && key0 + i <= last_key);
       }
     }
     cp_arrive(&sh.raw_full[lb]);
@@ -699,12 +700,15 @@ __global__ void __launch_bounds__(kExThreads) tree_softmax(const __grid_constant
     }
     auto term = [&](uint32_t x, int i) -> uint32_t {
       const uint32_t D = m - x;  // below the maximum by D
-      uint64_t e = 0;
-      if ((vis >> i & 1) && D < (16u << 16)) e = exp_term_below(D);
+      const bool on = vis >> i & 1;
+      uint32_t e = on && D < (16u << 16) ? exp_term_below(D) : 0;
+      if (on && D == 0) {
+        e = 0xffffffffu;
+        first = min(first, j + i);
+        sum += 1;
+      }
       sum += e;
-      if (!(e >> 32)) return (uint32_t)e;
-      first = min(first, j + i);
-      return 0xffffffffu;
+      return e;
     };
     terms[(j - k0) >> 2] = make_uint4(term(v.x, 0), term(v.y, 1), term(v.z, 2), term(v.w, 3));
   }
@@ -800,47 +804,50 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
 
   // Stage lu into its slot.  Keys past the sequence (their weights are zero) and
   // dims past the head (their sums are not stored) are zero.
+  const int lp = tid - (kPvThreads - kTrLoaders);
   int lu = 0, lb = 0, lph = 1;  // next stage, its slot and the parity of the slot's last use
   auto load = [&]() {
     const uint32_t slot = su32(slots) + lb * kSlot;
-    const int key0 = t.lo + (c0 + lu) * 64, p = tid & (kTrLoaders - 1);
-    if (VEC) {  // 16 bytes of keys p / 32, p / 32 + 2, ..
-      const int dim = db * 128 + 4 * (p & 31), row0 = p >> 5;
+    const int key0 = t.lo + (c0 + lu) * 64;
+    if (VEC) {  // 16 bytes of keys p / 32, p / 32 + 4, ..
+      const int p = lp, dim = db * 128 + 4 * (p & 31), row0 = p >> 5;
       const bool on = dim < d;
       const uint32_t dst = slot + row0 * 512 + 16 * (p & 31);
       const int od = on ? dim : 0;
       if (key0 + 64 <= t.ctx) {  // cache rows only
         const int32_t* src = vc + (int64_t)(key0 + row0) * d + od;
-#pragma unroll 8
-        for (int i = 0; i < 32; ++i) cp16(dst + i * 1024, src + (int64_t)i * (2 * d), on);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) cp16(dst + i * 2048, src + (int64_t)i * (4 * d), on);
       } else {
-        for (int i = 0; i < 32; ++i) {
-          const int key = min(key0 + row0 + 2 * i, last_key);
-          cp16(dst + i * 1024, (key < t.ctx ? vc + (int64_t)key * d : vt + (int64_t)(key - t.ctx) * d) + od,
-               on && key0 + row0 + 2 * i <= last_key);
+        for (int i = 0; i < 16; ++i) {
+          const int key = min(key0 + row0 + 4 * i, last_key);
+          cp16(dst + i * 2048, (key < t.ctx ? vc + (int64_t)key * d : vt + (int64_t)(key - t.ctx) * d) + od,
+               on && key0 + row0 + 4 * i <= last_key);
         }
       }
-    } else {  // two dims of every key
-      for (int i = 0; i < 128; ++i) {
-        const int dl = p + 64 * (i & 1), dim = db * 128 + dl, k = i >> 1, key = min(key0 + k, last_key);
-        cp4(slot + k * 512 + 4 * dl, (key < t.ctx ? vc + (int64_t)key * d : vt + (int64_t)(key - t.ctx) * d) + min(dim, d - 1),
-            dim < d && key0 + k <= last_key);
+    } else {  // one dim of every key
+      const int dim = db * 128 + lp, od = min(dim, d - 1);
+      for (int i = 0; i < 64; ++i) {
+        const int key = min(key0 + i, last_key);
+        cp4(slot + i * 512 + 4 * lp, (key < t.ctx ? vc + (int64_t)key * d : vt + (int64_t)(key - t.ctx) * d) + od,
+            dim < d && key0 + i <= last_key);
       }
     }
     ++lu;
     if (++lb == kSt) { lb = 0; lph ^= 1; }
   };
   // Stage u's weights into slot b, and the stage's arrival: 16 bytes of rows
-  // p / 4, p / 4 + 16, .. (rows past the block are zero)
+  // p / 4, p / 4 + 32, .. (rows past the block are zero)
   auto load_w = [&](int u, int b) {
-    const int p = tid & (kTrLoaders - 1), c = p & 3;
+    const int c = lp & 3;
     const uint32_t dst = su32(slots) + b * kSlot + kTrPlanes;
 #pragma unroll
-    for (int i = 0; i < NR / 16; ++i) {
-      const int r = (p >> 2) + 16 * i;
+    for (int i = 0; i < (NR + 31) / 32; ++i) {
+      const int r = (lp >> 2) + 32 * i;
       const unsigned char* src = wts + (int64_t)min(r, nr - 1) * t.pad * 4 + u * 256 + 16 * c;
 #pragma unroll
-      for (int a = 0; a < 3; ++a) cp16(dst + ta_sw(a * NR + r, c), src + 64 * a, r < nr);
+      for (int a = 0; a < 3; ++a)
+        if (r < NR) cp16(dst + ta_sw(a * NR + r, c), src + 64 * a, r < nr);
     }
     cp_arrive(&raw_full[b]);
   };
@@ -1090,7 +1097,7 @@ size_t tree_attn_plan(TreeGroup& g) {
   auto pick = [&](int most, auto&& ctas, auto&& stages) {
     int size = 1;
     int64_t best = INT64_MAX;
-    for (int k = 1; k <= most; k += 1 + k / 8) {
+    for (int k = 1; k <= most; k += 1 + k / (g.nseq > 4 ? 8 : 64)) {
       const int64_t cost = (ctas(k) + kSms - 1) / kSms * stages(k);
       if (cost < best) {
         best = cost;
@@ -1107,7 +1114,7 @@ size_t tree_attn_plan(TreeGroup& g) {
         for (int i = 0; i < g.nseq; ++i) n += blocks(g.seq[i]) * ceil_div(ceil_div(g.seq[i].len, kTrKeys), k);
         return n;
       },
-      [&](int k) { return k * ns + 4; });
+      [&](int k) { return k * (ns + (g.nr == 64 ? 4 : 2)) + 8; });
   const int per = pick(
       kTrSplitKeys / 64,
       [&](int k) {
@@ -1115,7 +1122,7 @@ size_t tree_attn_plan(TreeGroup& g) {
         for (int i = 0; i < g.nseq; ++i) n += blocks(g.seq[i]) * nd * ceil_div(g.seq[i].pad / 64, k);
         return n;
       },
-      [&](int k) { return k + 4; });
+      [&](int k) { return k + 10; });
   for (int i = 0; i < g.nseq; ++i) {
     TreeSeq& t = g.seq[i];
     t.soff = soff;
@@ -1136,13 +1143,16 @@ size_t tree_attn_plan(TreeGroup& g) {
   g.rows = rows;
   g.pv_items = pv;
   g.qk_items = qk;
-  // Keys of a softmax CTA: four per thread, more where the rows alone fill the
-  // GPU, and so many that a row's cluster has at most eight CTAs (sixteen for the longest).
+  // Keys of a softmax CTA: four per thread, more where the CTAs would not be
+  // resident at once (a CTA is mostly latency: 1288 rows of up to 4108 keys take
+  // 46 us in clusters of three CTAs), and so many that a row's cluster has at
+  // most eight CTAs (sixteen for the longest).
   g.ex_keys = 4 * kExThreads;
-  while ((g.ex_keys < 16 * kExThreads && (int64_t)rows * (maxpad / g.ex_keys) > 32 * kSms) ||
+  while ((g.ex_keys < 32 * kExThreads && (int64_t)rows * ceil_div(maxpad, g.ex_keys) > 8 * kSms) ||
          ceil_div(maxpad, g.ex_keys) > (g.ex_keys < kExMostKeys ? 8 : 16))
     g.ex_keys *= 2;
   g.ex_chunks = ceil_div(maxpad, g.ex_keys);
+  g.ex_keys = std::min(g.ex_keys, maxpad);
   auto up = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
   g.max_off = up(soff * 4);
   g.sum_off = up(g.max_off + moff * 4);

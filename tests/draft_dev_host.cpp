@@ -19,7 +19,7 @@ int64_t exp_all(int32_t max_logit) {
   int64_t bad = 0;
   for (uint32_t D = 0; D < (16u << 16); ++D)
     if ((int64_t)max_logit - D >= INT32_MIN)
-      bad += (int64_t)exp_term_below(D) != exp_term((int32_t)((int64_t)max_logit - D), max_logit);
+      bad += (D ? (int64_t)exp_term_below(D) : kOneAcc) != exp_term((int32_t)((int64_t)max_logit - D), max_logit);
   return bad;
 }
 // the largest term below 2^32: the code 2^32 - 1 stands for 2^32 alone
