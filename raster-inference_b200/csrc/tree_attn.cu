@@ -690,8 +690,11 @@ __global__ void __launch_bounds__(kExThreads) tree_softmax(const __grid_constant
   const uint32_t m = __reduce_max_sync(0xffffffffu, top) ^ 0x80000000u;
   uint64_t sum = 0;
   int32_t first = INT32_MAX;  // the thread's first key at the maximum
+  uint4 next;
+  ld16(next, sc + k0 + 4 * tid, k0 + 4 * tid < k1);
   for (int j = k0 + 4 * tid; j < k1; j += 4 * kExThreads) {
-    const uint4 v = *reinterpret_cast<const uint4*>(sc + j);
+    const uint4 v = next;
+    ld16(next, sc + j + 4 * kExThreads, j + 4 * kExThreads < k1);
     const int key = t.lo + j;
     uint32_t vis = 15u;
     if (!(key >= start && key + 3 < t.ctx)) {
@@ -912,7 +915,6 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
     int pb = 0, ph = 0;
     for (int u = 0; u < total; ++u) {
       wait(&raw_full[pb], ph);
-      ta_fence_async();  // the weights' tile, for the MMAs
       uint32_t x[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) x[i] = *reinterpret_cast<const uint32_t*>(col + pb * kSlot + 512 * i);
@@ -942,6 +944,7 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
         const uint64_t wd = ta_adv(wdesc, pb * kSlot + 32 * h);
         const uint32_t a = tmem + kA + 32 * h;
         wait(&a_full[h], u & 1);
+        if (h == 0) ta_fence_async();  // the weights' tile: the converters saw its arrival before theirs
         fence_after();
         if (leader) {
           if (h == 0 && u == 0) {  // opens the column blocks, as in the score kernel
@@ -1152,7 +1155,7 @@ size_t tree_attn_plan(TreeGroup& g) {
          ceil_div(maxpad, g.ex_keys) > (g.ex_keys < kExMostKeys ? 8 : 16))
     g.ex_keys *= 2;
   g.ex_chunks = ceil_div(maxpad, g.ex_keys);
-  g.ex_keys = std::min(g.ex_keys, maxpad);
+  g.ex_keys = (ceil_div(maxpad, g.ex_chunks) + 63) & ~63;
   auto up = [](int64_t x) { return (x + 255) & ~(int64_t)255; };
   g.max_off = up(soff * 4);
   g.sum_off = up(g.max_off + moff * 4);
