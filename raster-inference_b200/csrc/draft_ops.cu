@@ -72,8 +72,8 @@ __device__ __forceinline__ void ld_word(uint32_t& v, const uint32_t* p, bool on)
                : "l"(p), "r"((int)on));
 }
 
-template <int THREADS>
-__global__ void __launch_bounds__(THREADS, 1024 / THREADS) logit_rules_kernel(const __grid_constant__ RuleRows rs,
+template <int THREADS, int ROWS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) logit_rules_kernel(const __grid_constant__ RuleRowsOf<ROWS> rs,
                                                                              uint32_t vocab, uint32_t* tokens) {
   constexpr uint32_t kStep = THREADS * 4 * kRuleVec;
   extern __shared__ __align__(16) unsigned char rule_raw[];
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logit_rules_kernel(co
       for (int k = 0; k < 2; ++k) local(bi[k], [&](uint32_t li) { g(li, (int32_t)bw[k]); });
       for (uint32_t k = tid + 2 * THREADS; k < nbias; k += THREADS)
         local(bias_ids[k], [&](uint32_t li) { g(li, (int32_t)bias_values[k]); });
-      if (tid < kRuleRows && (rs.row[row].path[tid >> 6] >> (tid & 63) & 1)) local(rs.row[tid].token, f);
+      if (tid < ROWS && (rs.row[row].path[tid >> 6] >> (tid & 63) & 1)) local(rs.row[tid].token, f);
     };
     // the slot of li; the table's load is low, so few probes reach it
     auto slot = [&](uint32_t li) {
@@ -296,42 +296,43 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logit_rules_kernel(co
 // and the path increases, so row i is written after it was read and after
 // every row before it.
 // ---------------------------------------------------------------------------
-template <typename T>
-__device__ __forceinline__ void move_rows(const CommitMoves& m, const CommitMove& v, int cols) {
+template <typename T, typename M>
+__device__ __forceinline__ void move_rows(const M& m, const CommitMove& v, int cols) {
   T* dst = reinterpret_cast<T*>(v.cache);
   const T* src = reinterpret_cast<const T*>(v.draft);
   const int n = m.len[v.path];
-  for (int64_t c = threadIdx.x + (int64_t)blockIdx.x * blockDim.x; c < (int64_t)v.kv_heads * cols;
-       c += (int64_t)gridDim.x * blockDim.x) {
+  for (int c = threadIdx.x; c < (int)(v.kv_heads_1 + 1) * cols; c += blockDim.x) {
     const int64_t h = c / cols, x = c % cols;
     for (int i = 0; i < n; ++i)
       dst[(h * v.cap + v.context + i) * cols + x] = src[(h * v.draft_cap + m.node[v.path][i]) * cols + x];
   }
 }
-__global__ void __launch_bounds__(256) tree_commit_kernel(const __grid_constant__ CommitMoves m) {
+template <int M, int P>
+__global__ void __launch_bounds__(256) tree_commit_kernel(const __grid_constant__ CommitMovesOf<M, P> m) {
   do_wait();
   do_go();
-  const CommitMove& v = m.mv[blockIdx.y];
-  const bool wide = v.head_dim % 4 == 0 && ((reinterpret_cast<uintptr_t>(v.cache) | reinterpret_cast<uintptr_t>(v.draft)) & 15) == 0;
-  if (wide) move_rows<int4>(m, v, v.head_dim / 4);
-  else move_rows<int32_t>(m, v, v.head_dim);
+  const CommitMove& v = m.mv[blockIdx.x];
+  const int d = v.head_dim_1 + 1;
+  const bool wide = d % 4 == 0 && ((reinterpret_cast<uintptr_t>(v.cache) | reinterpret_cast<uintptr_t>(v.draft)) & 15) == 0;
+  if (wide) move_rows<int4>(m, v, d / 4);
+  else move_rows<int32_t>(m, v, d);
 }
 
 }  // namespace
 
-template <int THREADS>
+template <int THREADS, int ROWS>
 static void rules_attr() {
-  cudaFuncSetAttribute(logit_rules_kernel<THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+  cudaFuncSetAttribute(logit_rules_kernel<THREADS, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                        (int)sizeof(RuleSmem));
-  cudaFuncSetAttribute(logit_rules_kernel<THREADS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  cudaFuncSetAttribute(logit_rules_kernel<THREADS, ROWS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
 }
 void draft_ops_init() {
-  rules_attr<256>();
-  rules_attr<1024>();
+  rules_attr<256, kRuleRows>();
+  rules_attr<1024, kRuleFew>();
 }
 
-template <int THREADS>
-static void rules_launch(const RuleRows& r, int rows, uint32_t vocab, uint32_t* tokens, int most, cudaStream_t s) {
+template <int THREADS, int ROWS>
+static void rules_launch(const RuleRowsOf<ROWS>& r, int rows, uint32_t vocab, uint32_t* tokens, int most, cudaStream_t s) {
   const int tiles = (int)((vocab + THREADS * 16 - 1) / (THREADS * 16));
   int CL = 1;
   while (CL < most && CL < tiles) CL *= 2;
@@ -349,20 +350,28 @@ static void rules_launch(const RuleRows& r, int rows, uint32_t vocab, uint32_t* 
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  cudaLaunchKernelEx(&cfg, logit_rules_kernel<THREADS>, r, vocab, tokens);
+  cudaLaunchKernelEx(&cfg, logit_rules_kernel<THREADS, ROWS>, r, vocab, tokens);
 }
 
-// Few rows take the largest clusters (sixteen CTAs) of large CTAs: one row of
-// 262144 logits under a history of 513 takes 7.7 us (512 threads and eight CTAs
-// a row: 9.7).  Many rows fill the GPU with small CTAs, four of them an SM.
+// Few rows (16 CTAs each at most one an SM) take the largest clusters (sixteen
+// CTAs) of large CTAs: one row of 262144 logits under a history of 513 takes
+// 7.7 us (512 threads and eight CTAs a row: 9.7).  Many rows fill the GPU with
+// small CTAs, four of them an SM.
 void launch_logit_rules(const RuleRows& r, int rows, uint32_t vocab, uint32_t* tokens, cudaStream_t s) {
-  if (rows * 16 <= 148) rules_launch<1024>(r, rows, vocab, tokens, 16, s);
-  else rules_launch<256>(r, rows, vocab, tokens, 8, s);
+  static_assert(kRuleFew == 148 / 16, "one CTA an SM");
+  if (rows <= kRuleFew) {
+    RuleRowsOf<kRuleFew> few;
+    std::copy(r.row, r.row + rows, few.row);
+    rules_launch<1024, kRuleFew>(few, rows, vocab, tokens, 16, s);
+  } else {
+    rules_launch<256, kRuleRows>(r, rows, vocab, tokens, 8, s);
+  }
 }
 
-void launch_tree_commit(const CommitMoves& m, int moves, cudaStream_t s) {
+template <int M, int P>
+static void commit_launch(const CommitMovesOf<M, P>& m, int moves, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(1, moves, 1);
+  cfg.gridDim = dim3(moves, 1, 1);
   cfg.blockDim = dim3(256, 1, 1);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -370,7 +379,18 @@ void launch_tree_commit(const CommitMoves& m, int moves, cudaStream_t s) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, tree_commit_kernel, m);
+  cudaLaunchKernelEx(&cfg, tree_commit_kernel<M, P>, m);
+}
+void launch_tree_commit(const CommitMoves& m, int moves, int paths, cudaStream_t s) {
+  if (moves <= kCommitFewMoves && paths <= kCommitFewPaths) {
+    CommitMovesOf<kCommitFewMoves, kCommitFewPaths> few;
+    std::copy(m.mv, m.mv + moves, few.mv);
+    std::copy(m.len, m.len + paths, few.len);
+    memcpy(few.node, m.node, sizeof(m.node[0]) * (size_t)paths);
+    commit_launch(few, moves, s);
+  } else {
+    commit_launch(m, moves, s);
+  }
 }
 
 }  // namespace rdet

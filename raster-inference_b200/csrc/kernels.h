@@ -408,6 +408,7 @@ struct TreeGroup {
   // sequences before each one, workspace sections (in
   // bytes, after the scores): partial maxima, partial sums, first maxima,
   // value sums, weight sums and arrivals per value item
+  size_t ws_bytes = 0;                         // (what tree_attn_plan returned)
   int32_t G = 1, nr = 0, qk_tiles = 1, ex_keys = 0, ex_chunks = 1, qk_items = 0, pv_items = 0, rows = 0;
   int32_t qk_first[kTreeGroupSeqs], pv_first[kTreeGroupSeqs], row_first[kTreeGroupSeqs];
   int64_t max_off = 0, sum_off = 0, idx_off = 0, acc_off = 0, cnt_off = 0;
@@ -432,26 +433,32 @@ struct RuleRow {
   uint32_t has_path;               // some bit of path is set
   uint64_t path[kRuleRows / 64];   // the launch's rows whose token counts for this one: itself and its ancestors
 };
-struct RuleRows {
-  RuleRow row[kRuleRows];
+// Few rows go with a smaller parameter block: a launch copies the whole of it.
+constexpr int kRuleFew = 9;
+template <int N>
+struct RuleRowsOf {
+  RuleRow row[N];
 };
+using RuleRows = RuleRowsOf<kRuleRows>;
 void launch_logit_rules(const RuleRows& r, int rows, uint32_t vocab, uint32_t* tokens, cudaStream_t s);
 
 // Accepted rows into the caches (rdet_det_tree_commit): moves by value.
-constexpr int kCommitMoves = 512, kCommitPaths = 64;
+constexpr int kCommitMoves = 880, kCommitPaths = 64;
+constexpr int kCommitFewMoves = 128, kCommitFewPaths = 4;  // of the smaller parameter block
 struct CommitMove {
   int32_t* cache;
   const int32_t* draft;
   uint32_t cap, draft_cap, context;
-  uint16_t head_dim, path;
-  uint32_t kv_heads;
+  uint32_t head_dim_1 : 10, kv_heads_1 : 10, path : 6;  // the first two less one
 };
-struct CommitMoves {
-  CommitMove mv[kCommitMoves];
-  uint8_t len[kCommitPaths];
-  uint8_t node[kCommitPaths][kTreeNodes];
+template <int M, int P>
+struct CommitMovesOf {
+  CommitMove mv[M];
+  uint8_t len[P];
+  uint8_t node[P][kTreeNodes];
 };
-void launch_tree_commit(const CommitMoves& m, int moves, cudaStream_t s);
+using CommitMoves = CommitMovesOf<kCommitMoves, kCommitPaths>;
+void launch_tree_commit(const CommitMoves& m, int moves, int paths, cudaStream_t s);
 void draft_ops_init();  // per-device kernel attributes (called by kernels_init)
 
 // ---- model ingestion: safetensors values -> Q16.16 weights (convert.cu) --------------

@@ -2700,24 +2700,15 @@ static unsigned char* noalloc_scratch_current_device() {
 
 // Calls f(group) for every launch group of the trees (at most kTreeGroupSeqs
 // sequences and kTreeGroupNodes nodes each, a sequence's tree in one group).
-template <typename F>
-static void tree_groups(const rdet_tree_seq* seqs, uint32_t n_seqs, uint32_t num_heads, uint32_t num_kv_heads,
-                        uint32_t head_dim, uint32_t window, F&& f) {
+static std::vector<std::unique_ptr<TreeGroup>> tree_groups(const rdet_tree_seq* seqs, uint32_t n_seqs,
+                                                           uint32_t num_heads, uint32_t num_kv_heads,
+                                                           uint32_t head_dim, uint32_t window) {
   REQUIRE(n_seqs == 0 || seqs, RDET_E_INVALID, "null argument");
   REQUIRE(num_kv_heads > 0 && num_heads > 0 && num_heads % num_kv_heads == 0, RDET_E_INVALID,
           "num_heads must be a multiple of num_kv_heads");
   REQUIRE(num_heads <= 1024, RDET_E_RANGE, "at most 1024 query heads");
   REQUIRE(head_dim > 0 && head_dim <= 512, RDET_E_RANGE, "head_dim must be in [1, 512]");
-  auto g = std::make_unique<TreeGroup>();
-  auto flush = [&] {
-    if (g->nseq == 0) return;
-    g->Hq = (int)num_heads;
-    g->Hkv = (int)num_kv_heads;
-    g->d = (int)head_dim;
-    g->window = (int)std::min<uint32_t>(window, 1u << 30);
-    f(*g);
-    g->nseq = g->nnode = 0;
-  };
+  std::vector<std::unique_ptr<TreeGroup>> groups;
   for (uint32_t i = 0; i < n_seqs; ++i) {
     const rdet_tree_seq& t = seqs[i];
     REQUIRE(t.n_nodes >= 1 && t.n_nodes <= RDET_MAX_TREE_NODES, RDET_E_RANGE, "a tree has between 1 and 64 nodes");
@@ -2728,7 +2719,16 @@ static void tree_groups(const rdet_tree_seq* seqs, uint32_t n_seqs, uint32_t num
     REQUIRE(t.context < (1u << 24), RDET_E_RANGE, "context must be below 2^24");
     const uint32_t rows = (window > 0 ? std::min(t.context, window) : t.context) + t.n_nodes;
     REQUIRE(rows <= (uint32_t)kTreeMaxKeys, RDET_E_RANGE, "a sequence attends at most 523264 rows");
-    if (g->nseq == kTreeGroupSeqs || g->nnode + (int)t.n_nodes > kTreeGroupNodes) flush();
+    if (groups.empty() || groups.back()->nseq == kTreeGroupSeqs ||
+        groups.back()->nnode + (int)t.n_nodes > kTreeGroupNodes) {
+      groups.push_back(std::make_unique<TreeGroup>());
+      TreeGroup& n = *groups.back();
+      n.Hq = (int)num_heads;
+      n.Hkv = (int)num_kv_heads;
+      n.d = (int)head_dim;
+      n.window = (int)std::min<uint32_t>(window, 1u << 30);
+    }
+    TreeGroup* const g = groups.back().get();
     TreeSeq& d = g->seq[g->nseq++];
     d.k = t.k_cache;
     d.v = t.v_cache;
@@ -2747,7 +2747,8 @@ static void tree_groups(const rdet_tree_seq* seqs, uint32_t n_seqs, uint32_t num
     }
     g->nnode += (int)t.n_nodes;
   }
-  flush();
+  for (auto& g : groups) tree_attn_plan(*g);
+  return groups;
 }
 
 }  // namespace rdet
@@ -3800,8 +3801,8 @@ int32_t rdet_det_attention_tree_workspace(const rdet_tree_seq* seqs, uint32_t n_
   return guard([&] {
     REQUIRE(bytes_out, RDET_E_INVALID, "null argument");
     size_t need = 0;
-    tree_groups(seqs, n_seqs, num_heads, num_kv_heads, head_dim, window,
-                [&](TreeGroup& g) { need = std::max(need, tree_attn_plan(g)); });
+    for (const auto& g : tree_groups(seqs, n_seqs, num_heads, num_kv_heads, head_dim, window))
+      need = std::max(need, g->ws_bytes);
     *bytes_out = need;
   });
 }
@@ -3812,22 +3813,21 @@ int32_t rdet_det_attention_tree(const rdet_tree_seq* seqs, uint32_t n_seqs, cons
   return guard([&] {
     REQUIRE(n_seqs == 0 || (q && out && workspace), RDET_E_INVALID, "null argument");
     REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, RDET_E_INVALID, "workspace must be 256-byte aligned");
+    const auto groups = tree_groups(seqs, n_seqs, num_heads, num_kv_heads, head_dim, window);
     // nothing is launched unless every group can be
-    tree_groups(seqs, n_seqs, num_heads, num_kv_heads, head_dim, window, [&](TreeGroup& g) {
-      REQUIRE(tree_attn_plan(g) <= workspace_bytes, RDET_E_RANGE,
+    for (const auto& g : groups)
+      REQUIRE(g->ws_bytes <= workspace_bytes, RDET_E_RANGE,
               "workspace is smaller than rdet_det_attention_tree_workspace asks for");
-    });
     kernels_init();
     size_t node = 0;
     const size_t row = (size_t)num_heads * head_dim;
-    tree_groups(seqs, n_seqs, num_heads, num_kv_heads, head_dim, window, [&](TreeGroup& g) {
-      tree_attn_plan(g);
-      g.q = q + node * row;
-      g.out = out + node * row;
-      g.ws = workspace;
-      launch_tree_attn(g, static_cast<cudaStream_t>(stream));
-      node += (size_t)g.nnode;
-    });
+    for (const auto& g : groups) {
+      g->q = q + node * row;
+      g->out = out + node * row;
+      g->ws = workspace;
+      launch_tree_attn(*g, static_cast<cudaStream_t>(stream));
+      node += (size_t)g->nnode;
+    }
     CK(cudaGetLastError());
   });
 }
@@ -3861,7 +3861,7 @@ int32_t rdet_det_logits_rules(const rdet_logit_row* rows, uint32_t n_rows, uint3
       cut.push_back(i1);
     }
     kernels_init();
-    auto part = std::make_unique<RuleRows>();
+    const std::unique_ptr<RuleRows> part(new RuleRows);
     for (size_t c = 0; c + 1 < cut.size(); ++c) {
       const uint32_t i0 = cut[c], i1 = cut[c + 1];
       for (uint32_t i = i0; i < i1; ++i) {
@@ -3908,7 +3908,7 @@ int32_t rdet_det_tree_commit(const rdet_tree_move* moves, uint32_t n_moves, cons
       REQUIRE(len == 0 || nodes[path_off[m.path + 1] - 1] < m.draft_cap, RDET_E_RANGE,
               "a path's node lies past the drafted rows");
     }
-    auto part = std::make_unique<CommitMoves>();
+    const std::unique_ptr<CommitMoves> part(new CommitMoves);
     for (uint32_t i0 = 0; i0 < n_moves;) {
       uint32_t i = i0, paths = 0;
       uint32_t local[kCommitPaths];  // the call's path of each path of this launch
@@ -3923,10 +3923,9 @@ int32_t rdet_det_tree_commit(const rdet_tree_move* moves, uint32_t n_moves, cons
           part->len[p] = (uint8_t)(path_off[m.path + 1] - o);
           for (uint32_t j = 0; j < part->len[p]; ++j) part->node[p][j] = (uint8_t)nodes[o + j];
         }
-        part->mv[i - i0] = CommitMove{m.cache, m.draft, m.cap, m.draft_cap, m.context, (uint16_t)m.head_dim,
-                                      (uint16_t)p, m.kv_heads};
+        part->mv[i - i0] = CommitMove{m.cache, m.draft, m.cap, m.draft_cap, m.context, m.head_dim - 1, m.kv_heads - 1, p};
       }
-      launch_tree_commit(*part, (int)(i - i0), static_cast<cudaStream_t>(stream));
+      launch_tree_commit(*part, (int)(i - i0), (int)paths, static_cast<cudaStream_t>(stream));
       i0 = i;
     }
     CK(cudaGetLastError());

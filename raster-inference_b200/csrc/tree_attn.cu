@@ -1095,23 +1095,29 @@ size_t tree_attn_plan(TreeGroup& g) {
   auto blocks = [&](const TreeSeq& t) { return (int64_t)g.Hkv * ((t.n * G + g.nr - 1) / g.nr); };
   auto ceil_div = [](int x, int y) { return (x + y - 1) / y; };
   // Key tiles of a score CTA and 64-key chunks of a value CTA: the size with
-  // the shortest run of work on one SM (CTAs in waves of one per SM; a CTA's
-  // fixed work counted in stages of its loop).
+  // the shortest run of work on one SM, from the least size of each number of
+  // waves (one CTA an SM; a CTA's fixed work is counted in stages of its loop).
   auto pick = [&](int most, auto&& ctas, auto&& stages) {
-    int size = 1;
+    int size = most;
     int64_t best = INT64_MAX;
-    for (int k = 1; k <= most; k += 1 + k / (g.nseq > 4 ? 8 : 64)) {
-      const int64_t cost = (ctas(k) + kSms - 1) / kSms * stages(k);
+    for (int waves = 1; waves <= 4; ++waves) {
+      int lo = 1, hi = most;  // the least size whose CTAs take `waves` waves
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (ctas(mid) <= (int64_t)waves * kSms) hi = mid;
+        else lo = mid + 1;
+      }
+      const int64_t cost = (ctas(lo) + kSms - 1) / kSms * stages(lo);
       if (cost < best) {
         best = cost;
-        size = k;
+        size = lo;
       }
     }
     return size;
   };
   const int ns = (g.d + 63) / 64;
   g.qk_tiles = pick(
-      16,
+      ceil_div(maxpad, kTrKeys),
       [&](int k) {
         int64_t n = 0;
         for (int i = 0; i < g.nseq; ++i) n += blocks(g.seq[i]) * ceil_div(ceil_div(g.seq[i].len, kTrKeys), k);
@@ -1119,7 +1125,7 @@ size_t tree_attn_plan(TreeGroup& g) {
       },
       [&](int k) { return k * (ns + (g.nr == 64 ? 4 : 2)) + 8; });
   const int per = pick(
-      kTrSplitKeys / 64,
+      std::min(kTrSplitKeys, maxpad) / 64,
       [&](int k) {
         int64_t n = 0;
         for (int i = 0; i < g.nseq; ++i) n += blocks(g.seq[i]) * nd * ceil_div(g.seq[i].pad / 64, k);
@@ -1162,7 +1168,7 @@ size_t tree_attn_plan(TreeGroup& g) {
   g.idx_off = up(g.sum_off + (int64_t)rows * g.ex_chunks * 4);
   g.acc_off = up(g.idx_off + (int64_t)rows * g.ex_chunks * 4);
   g.cnt_off = up(g.acc_off + (int64_t)rows * g.d * 8);
-  return (size_t)up(g.cnt_off + (int64_t)counters * 4);
+  return g.ws_bytes = (size_t)up(g.cnt_off + (int64_t)counters * 4);
 }
 
 template <int NR, bool VEC>
