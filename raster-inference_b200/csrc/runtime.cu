@@ -3897,37 +3897,41 @@ int32_t rdet_det_tree_commit(const rdet_tree_move* moves, uint32_t n_moves, cons
         REQUIRE(nodes[j] < RDET_MAX_TREE_NODES && (j == path_off[p] || nodes[j] > nodes[j - 1]), RDET_E_INVALID,
                 "a path's nodes must increase and be below 64");
     }
+    struct Part {
+      CommitMoves m;
+      uint32_t moves, paths, from[kCommitPaths];  // from: the call's path of each path of this launch
+    };
+    std::vector<std::unique_ptr<Part>> parts;  // nothing is launched unless every move can be
+    uint32_t p = 0;
     for (uint32_t i = 0; i < n_moves; ++i) {
       const rdet_tree_move& m = moves[i];
       REQUIRE(m.cache && m.draft, RDET_E_INVALID, "null argument");
       REQUIRE(m.path < n_paths, RDET_E_INVALID, "path out of range");
       REQUIRE(m.kv_heads > 0 && m.kv_heads <= 1024 && m.head_dim > 0 && m.head_dim <= 1024, RDET_E_RANGE,
               "kv_heads and head_dim must be in [1, 1024]");
-      const uint32_t len = path_off[m.path + 1] - path_off[m.path];
+      const uint32_t off = path_off[m.path], len = path_off[m.path + 1] - off;
       REQUIRE((uint64_t)m.context + len <= m.cap, RDET_E_RANGE, "the accepted rows would overflow the cache");
-      REQUIRE(len == 0 || nodes[path_off[m.path + 1] - 1] < m.draft_cap, RDET_E_RANGE,
-              "a path's node lies past the drafted rows");
-    }
-    const std::unique_ptr<CommitMoves> part(new CommitMoves);
-    for (uint32_t i0 = 0; i0 < n_moves;) {
-      uint32_t i = i0, paths = 0;
-      uint32_t local[kCommitPaths];  // the call's path of each path of this launch
-      for (; i < n_moves && i - i0 < (uint32_t)kCommitMoves; ++i) {
-        const rdet_tree_move& m = moves[i];
-        uint32_t p = 0;
-        while (p < paths && local[p] != m.path) ++p;
-        if (p == paths) {
-          if (paths == (uint32_t)kCommitPaths) break;
-          local[paths++] = m.path;
-          const uint32_t o = path_off[m.path];
-          part->len[p] = (uint8_t)(path_off[m.path + 1] - o);
-          for (uint32_t j = 0; j < part->len[p]; ++j) part->node[p][j] = (uint8_t)nodes[o + j];
+      REQUIRE(len == 0 || nodes[off + len - 1] < m.draft_cap, RDET_E_RANGE, "a path's node lies past the drafted rows");
+      Part* part = parts.empty() ? nullptr : parts.back().get();
+      if (!part || part->moves == (uint32_t)kCommitMoves || p >= part->paths || part->from[p] != m.path) {
+        if (part)
+          for (p = 0; p < part->paths && part->from[p] != m.path;) ++p;
+        if (!part || part->moves == (uint32_t)kCommitMoves || p == (uint32_t)kCommitPaths) {
+          parts.emplace_back(new Part);
+          part = parts.back().get();
+          part->moves = part->paths = p = 0;
         }
-        part->mv[i - i0] = CommitMove{m.cache, m.draft, m.cap, m.draft_cap, m.context, m.head_dim - 1, m.kv_heads - 1, p};
+        if (p == part->paths) {
+          part->from[part->paths++] = m.path;
+          part->m.len[p] = (uint8_t)len;
+          for (uint32_t j = 0; j < len; ++j) part->m.node[p][j] = (uint8_t)nodes[off + j];
+        }
       }
-      launch_tree_commit(*part, (int)(i - i0), (int)paths, static_cast<cudaStream_t>(stream));
-      i0 = i;
+      part->m.mv[part->moves++] =
+          CommitMove{m.cache, m.draft, m.cap, m.draft_cap, m.context, m.head_dim - 1, m.kv_heads - 1, p};
     }
+    for (const auto& part : parts)
+      launch_tree_commit(part->m, (int)part->moves, (int)part->paths, static_cast<cudaStream_t>(stream));
     CK(cudaGetLastError());
   });
 }
