@@ -404,10 +404,10 @@ struct TreeGroup {
   int32_t* out = nullptr;
   void* ws = nullptr;
   // filled by tree_attn_plan: heads per KV head, rows per block, key tiles
-  // per score CTA, keys per term CTA and CTAs per row, CTAs and rows of the
-  // sequences before each one, workspace sections (in
-  // bytes, after the scores): partial maxima, partial sums, first maxima,
-  // value sums, weight sums and arrivals per value item
+  // per score CTA, keys per softmax CTA and CTAs per row, CTAs and rows of the
+  // sequences before each one, workspace sections (in bytes, after the
+  // scores): partial maxima, partial sums of weights, first maxima, value sums
+  // and arrivals per value item
   size_t ws_bytes = 0;                         // (what tree_attn_plan returned)
   int32_t G = 1, nr = 0, qk_tiles = 1, ex_keys = 0, ex_chunks = 1, qk_items = 0, pv_items = 0, rows = 0;
   int32_t qk_first[kTreeGroupSeqs], pv_first[kTreeGroupSeqs], row_first[kTreeGroupSeqs];

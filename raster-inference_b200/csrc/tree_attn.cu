@@ -12,10 +12,9 @@
 // running softmax is exact: the scores of all keys come before the first exp
 // term, and all terms before the first weight.  Three kernels over a scratch,
 // coupled by programmatic dependent launch: scores with each block's row
-// maxima (tensor cores), exp terms with partial sums (CUDA cores), weights and
-// weighted values (tensor cores).  The residual 1 - sum w is a term of its
-// own, added with the first maximum's value where the sums are rounded.  A key
-// is an index into the sequence's [lo, lo + len): cache rows lo .. ctx - 1,
+// maxima (tensor cores), softmax (CUDA cores), weighted values (tensor cores).
+// The residual 1 - sum w is a term of its own, added with the first maximum's
+// value where the sums are rounded.  A key is an index into the sequence's [lo, lo + len): cache rows lo .. ctx - 1,
 // then the nodes (key ctx + i).  The order of keys is the order of positions
 // along every node's path, because parents come before their children.
 //
@@ -36,11 +35,19 @@
 // (columns [g NR, (g + 1) NR)) sums exactly the products of shift 8 g: seven
 // blocks, each at most 4 * 2^14 * 512 = 2^25 in magnitude, exact in s32.
 // A query row is a (node, head of the KV head's group); all of them read a
-// key tile at once, so the cache streams once per NR rows.
+// key tile at once, so the cache streams once per NR rows.  Keys rather than
+// query rows are the MMA's M: seven column blocks of NR leave TMEM room for
+// operand A, and a lane is a key, so that scores store coalesced.
 //
 // Weighted values.  M rows are 128 dims of the transposed value tile, B the
 // three digits of the weights (a weight lies in [0, 2^16]): six column
 // blocks, each at most 3 * 2^14 per key, exact in s32 up to 2^15 keys.
+//
+// Measured (eight heads of two KV heads, head_dim 512; warm passes in a graph).
+// 64 nodes at context 32768, 256 query rows a KV head: 306 us, of which scores
+// 119 (tensor pipe active 50%, its products alone take 62), softmax 83, values
+// 104 (58%, 46).  16 nodes at context 4096: 36 us (13.6, 8.5, 14), most of it
+// the start and the end of three dependent kernels of one CTA an SM.
 #include <cuda.h>
 #include <cuda_runtime.h>
 
@@ -61,8 +68,7 @@ namespace {
 using namespace tcx;
 
 constexpr int kTrKeys = 128;           // keys of a score tile (MMA M)
-constexpr int kTrPlane = 128 * 64;     // one digit plane of a stage: 128 rows of 64 bytes
-constexpr int kTrPlanes = 4 * kTrPlane;
+constexpr int kTrSlot = 128 * 64 * 4;  // a stage's rows: 128 keys of 64 dims, or 64 keys of 128
 constexpr int kTrConv = 512;           // converter threads (warps 0-15)
 constexpr int kTrConvWarps = kTrConv / 32;
 constexpr int kQkThreads = 800;        // + warps 16-19 drain, warp 20 issues the MMAs, warps 21-24 load
@@ -300,7 +306,7 @@ struct QkRows;
 template <int NR>
 __host__ __device__ constexpr int qk_stages(int ns);
 template <int NR>
-__host__ __device__ constexpr int qk_smem(int ns) { return qk_stages<NR>(ns) * kTrPlanes + ns * 4 * NR * 64 + 512; }
+__host__ __device__ constexpr int qk_smem(int ns) { return qk_stages<NR>(ns) * kTrSlot + ns * 4 * NR * 64 + 512; }
 
 // what draining a tile needs, per row of the block
 template <int NR>
@@ -322,11 +328,15 @@ struct QkShared {
 };
 template <int NR>
 __host__ __device__ constexpr int qk_stages(int ns) {
-  const int n = (kSmemMost - 512 - (int)sizeof(QkShared<NR>) - ns * 4 * NR * 64) / kTrPlanes;
+  const int n = (kSmemMost - 512 - (int)sizeof(QkShared<NR>) - ns * 4 * NR * 64) / kTrSlot;
   return n < kQkMaxStages ? n : kQkMaxStages;
 }
 // Scores of the row quads quad, quad + step, .. of a tile from TMEM (this
-// lane's key is j, the tile's first one j0), and each row's largest one.
+// lane's key is j, the tile's first one j0), and each row's largest one.  At 64
+// rows the accumulator fills TMEM, so the MMAs stand still meanwhile: 4500 of a
+// tile's 13700 cycles at head_dim 512, spread over all twenty warps, bound by
+// the instructions that join and round seven sums (in 32-bit pieces; in 64 bits
+// the call above took 4 us more).
 template <int NR>
 __device__ __noinline__ void qk_drain(QkRows<NR>& c, uint32_t taddr, int j0, int quad, int step) {
   const int lane = threadIdx.x & 31, j = j0 + 32 * ((threadIdx.x >> 5) & 3) + lane, key = c.lo + j;
@@ -382,6 +392,9 @@ __device__ __noinline__ void qk_drain_direct(QkRows<NR>& c, const int32_t* k, co
     }
 }
 
+// Scores.  Bound by the MMAs and shared memory about equally: a stage of 64
+// rows takes some 1150 cycles, the MMAs 1024, the rows' way in and out with the
+// MMAs' reads of the query digits the bandwidth of 1024.
 template <int NR, bool VEC>
 __global__ void __launch_bounds__(kQkThreads, 1) tree_qk(const __grid_constant__ TreeGroup g) {
   constexpr int na = 4;                         // query digits
@@ -396,7 +409,7 @@ __global__ void __launch_bounds__(kQkThreads, 1) tree_qk(const __grid_constant__
   const TreeSeq t = g.seq[si];
   const int d = g.d, ns = (d + 63) / 64, G = g.G, Hq = g.Hq, nst = qk_stages<NR>(ns);
   unsigned char* const slots = sm;                    // [nst][128 keys]
-  unsigned char* const qpl = sm + nst * kTrPlanes;    // [chunk][4 NR rows][64 B]
+  unsigned char* const qpl = sm + nst * kTrSlot;    // [chunk][4 NR rows][64 B]
   const int rows = t.n * G, nrb = (rows + NR - 1) / NR, tiles = (t.len + kTrKeys - 1) / kTrKeys, qt = g.qk_tiles;
   const int it = blockIdx.x - g.qk_first[si];
   const int blk = it / t.qk_per, part = it - blk * t.qk_per, t0 = part * qt, t1 = min(tiles, t0 + qt);
@@ -445,7 +458,7 @@ __global__ void __launch_bounds__(kQkThreads, 1) tree_qk(const __grid_constant__
   const int lp = tid - (kQkThreads - kTrLoaders);
   int lt = t0, ls = 0, lb = 0, lph = 1;  // next stage's tile, chunk, slot and the parity of the slot's last use
   auto load = [&]() {
-    const uint32_t slot = su32(slots) + lb * kTrPlanes;
+    const uint32_t slot = su32(slots) + lb * kTrSlot;
     const int key0 = t.lo + lt * kTrKeys;
     if (VEC) {  // 16 bytes of keys p / 16, p / 16 + 8, ..
       const int p = lp, dim = ls * 64 + 4 * (p & 15), row0 = p >> 4;
@@ -559,7 +572,7 @@ __global__ void __launch_bounds__(kQkThreads, 1) tree_qk(const __grid_constant__
       uint4 x[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        x[i] = *reinterpret_cast<const uint4*>(row + pb * kTrPlanes + 16 * ((4 * grp + i) ^ (key & 7)));
+        x[i] = *reinterpret_cast<const uint4*>(row + pb * kTrSlot + 16 * ((4 * grp + i) ^ (key & 7)));
       uint32_t o[4][4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) ta_bytes(x[i].x, x[i].y, x[i].z, x[i].w, o[i]);
@@ -649,7 +662,11 @@ __global__ void __launch_bounds__(kQkThreads, 1) tree_qk(const __grid_constant__
 // (three planes of 64 bytes per 64 keys, at every 256 bytes of the row).  A
 // term is held as u32: the one value of 2^32 (a score equal to the maximum) is
 // coded 2^32 - 1, which no other score gives (the next lower score's term is
-// below 2^32 - 2^15).
+// below 2^32 - 2^15).  Bound by the instructions of the exp terms where there
+// are many rows (16.8 million scores in 83 us, 2.7 instructions a cycle and SM),
+// by its chain of loads, barriers and sums where there are few.  One CTA for
+// 128 rows of 4112 keys each took 8 us longer than clusters of five, weights
+// made in the value kernel, once per 128 dims, 14 us more at 64 nodes.
 // ---------------------------------------------------------------------------
 constexpr int kExThreads = 256;
 constexpr int kExMostKeys = 32768;  // of a CTA: 128 KB of terms
@@ -767,9 +784,11 @@ __global__ void __launch_bounds__(kExThreads) tree_softmax(const __grid_constant
 // A stage is 64 keys of the 128 dims, 32 KB as they are in a ring of slots; the
 // value bytes go to the MMAs through TMEM like the key bytes above (a thread
 // holds one dim of 16 keys); the weights' digits, operand B, lie behind them.
+// Bound by shared memory: a stage of 64 rows takes some 1230 cycles, its
+// traffic 1000 of them, its MMAs 768.
 constexpr int kPvStages = 6;
 template <int NR>
-__host__ __device__ constexpr int pv_slot() { return kTrPlanes + 3 * NR * 64; }
+__host__ __device__ constexpr int pv_slot() { return kTrSlot + 3 * NR * 64; }
 template <int NR>
 __host__ __device__ constexpr int pv_stages() { return NR == 16 ? kPvStages : 5; }
 template <int NR>
@@ -843,7 +862,7 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
   // p / 4, p / 4 + 32, .. (rows past the block are zero)
   auto load_w = [&](int u, int b) {
     const int c = lp & 3;
-    const uint32_t dst = su32(slots) + b * kSlot + kTrPlanes;
+    const uint32_t dst = su32(slots) + b * kSlot + kTrSlot;
 #pragma unroll
     for (int i = 0; i < (NR + 31) / 32; ++i) {
       const int r = (lp >> 2) + 32 * i;
@@ -936,7 +955,7 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
   } else if (warp == kTrConvWarps) {
     const bool leader = ta_elect();
     const uint32_t full = ta_idesc(3 * NR), low = ta_idesc(2 * NR), one = ta_idesc(NR);
-    const uint64_t wdesc = smem_desc_sw64(su32(slots) + kTrPlanes);
+    const uint64_t wdesc = smem_desc_sw64(su32(slots) + kTrSlot);
     int pb = 0;
     for (int u = 0; u < total; ++u) {
 #pragma unroll
