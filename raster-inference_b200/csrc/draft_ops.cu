@@ -33,8 +33,9 @@ __device__ __forceinline__ void do_go() { asm volatile("griddepcontrol.launch_de
 //             then the marked tokens' values replace what the stream wrote.
 // Bound by memory: a row streams once.  64 rows of 262144 logits under all rules
 // and a history of 4096, written out (130 MB): 41 us, 3.2 TB/s, of which the
-// stream takes 24; gathering and computing, some 30000 cycles on every CTA at
-// once, leave the memory idle.  (Bringing the CTA's part into L2 meanwhile: 43.)
+// stream takes 26; gathering and computing, on every CTA at once, leave the
+// memory idle.  (Bringing the CTA's part into L2 meanwhile: 43; half of the
+// warps gathering while the others stream: 44.)
 // ---------------------------------------------------------------------------
 
 __device__ __forceinline__ int32_t clamp_i32(int64_t v) {

@@ -117,6 +117,39 @@ def test_tree_attention_ragged_batch(window, own):
     assert np.array_equal(c.run(window), c.want(window))
 
 
+@pytest.mark.parametrize("ctx,nodes,heads,kv,d,window", [
+    (5000, 20, 8, 2, 16, 0),      # blocks of 64 rows, the last one short, several tiles a CTA
+    (9001, 40, 8, 2, 80, 0),      # two chunks of dims, the second short
+    (5003, 33, 4, 2, 7, 0),       # rows that are not 16-byte aligned
+    (5000, 64, 4, 2, 16, 4500),   # windows that begin inside the tiles
+    (6000, 16, 4, 1, 130, 0),     # two blocks of dims
+    (40000, 1, 2, 1, 64, 0),      # few rows, many tiles a CTA
+    (40000, 8, 4, 1, 36, 0),
+    (1500, 64, 32, 4, 8, 0)])     # more rows than softmax CTAs are resident
+@pytest.mark.parametrize("kind", ["norm", "wide", "edge"])
+def test_tree_attention_long(ctx, nodes, heads, kv, d, window, kind):
+    rng = np.random.default_rng(ctx + nodes + d)
+    c = Case(rng, [ctx], [random_tree(rng, nodes, roots=nodes % 2 == 1)], heads, kv, d, kind,
+             qscale=8 if kind == "norm" else None, own=nodes % 3 == 0)
+    assert np.array_equal(c.run(window), c.want(window))
+
+
+def test_tree_attention_ragged_batch_of_wide_blocks():
+    rng = np.random.default_rng(77)
+    ctxs = [900, 0, 2500, 64, 1300, 4001, 127, 3000]
+    trees = [random_tree(rng, n) for n in (20, 64, 17, 33, 1, 40, 16, 64)]
+    c = Case(rng, ctxs, trees, 8, 2, 32, "norm", own=True, qscale=8, cap_extra=5)
+    assert np.array_equal(c.run(0), c.want(0))
+
+
+@pytest.mark.parametrize("ctx", [200000, 300000])
+def test_tree_attention_of_the_longest_rows(ctx):
+    # rows of eight and of sixteen softmax CTAs
+    rng = np.random.default_rng(ctx)
+    c = Case(rng, [ctx], [[-1, 0]], 2, 1, 4, "norm", qscale=8)
+    assert np.array_equal(c.run(0), c.want(0))
+
+
 @pytest.mark.parametrize("shift", [0, 1, 2, 3])
 def test_tree_attention_unaligned(shift):
     # rows that start off a 16-byte boundary
@@ -324,6 +357,16 @@ def test_logit_rules_many_rows_and_trees():
     rng = np.random.default_rng(6)
     trees = [random_tree(rng, int(rng.integers(1, 65))) for _ in range(14)]
     rules_case(rng, 97, trees, 10, 2, 1, True)
+
+
+@pytest.mark.parametrize("vocab,hist,nbias,mask,write,inplace,extreme", [
+    (70004, 500, 30, 1, True, False, False), (70004, 500, 30, 1, True, True, False), (66000, 0, 0, 2, False, False, False),
+    (70001, 300, 40, 3, True, False, False), (131072, 40000, 20, 0, True, True, False), (70004, 900, 12, 2, True, False, True)])
+def test_logit_rules_wide_vocabularies(vocab, hist, nbias, mask, write, inplace, extreme):
+    # rows whose CTAs stream and compute side by side; 40000 ids are more than a table holds
+    rng = np.random.default_rng(vocab + hist)
+    rules_case(rng, vocab, [random_tree(rng, 7), random_tree(rng, 4, roots=True)], hist, nbias, mask, write, inplace=inplace,
+               extreme=extreme)
 
 
 def test_logit_rules_ties_and_lowest_value():

@@ -221,6 +221,28 @@ def test_output_under_rules_equals_stepwise_reference():
     assert len(out[3]) == 3 and len(out[0]) == 24
 
 
+@pytest.mark.parametrize("nodes", [1, 8])
+def test_one_sequence_under_rules(nodes):
+    # alone and without a draft it decodes one token at a time
+    m = rdet.Model.synthetic(mini_config(), seed=6, width=16, max_prefill=32, layer_commitments=True)
+    words = (97 + 31) // 32
+
+    def low(output):
+        bits = np.zeros(words * 32, dtype=np.uint8)
+        bits[:40 + len(output)] = 1
+        return np.packbits(bits, bitorder="little").view(np.uint32)
+
+    rules = dict(repetition=80000, presence=4000, bias={2: 1 << 14}, allow=low)
+    ids = [int(t) for t in lcg_ids(9, 97, 9)]
+    s = m.new_sequence(60)
+    s.prefill(ids)
+    stats = {}
+    out = drafted.run_output_decode(m, [s], [ids], 20, nodes=nodes, rules=[rules], stats=stats)[0]
+    ref, r = greedy_loop(m, ids, 20, rules)
+    assert out == ref and state_of(s, m.L) == state_of(r, m.L)
+    assert nodes > 1 or stats["passes"] == 20
+
+
 def test_select_without_rules_and_empty_lists():
     m = rdet.Model.synthetic(mini_config(), seed=4, width=16, max_prefill=16)
     s = m.new_sequence(20)
