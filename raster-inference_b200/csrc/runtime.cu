@@ -2426,7 +2426,7 @@ static void tree_decode(Ctx& c, const std::vector<Seq*>& seqs, const uint32_t* c
   int nodes = 0;
   for (size_t i = 0; i < seqs.size(); ++i) nodes += (int)counts[i];
   // With tensor cores, fill up to the rows from which the linears use them: 16
-  // nodes of the E4B shape at context 4096 take 7.7 ms so, 174 ms with the
+  // nodes of the E4B shape at context 4096 take 7.5 ms so, 174 ms with the
   // CUDA-core linear of fewer rows (one token by rdet_decode: 4.0 ms).
   const int B = c.tc && c.max_prefill >= (uint32_t)kTcMinRows ? std::max(nodes, kTcMinRows) : nodes;
   auto& tr = c.tree;

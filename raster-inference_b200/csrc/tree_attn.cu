@@ -44,9 +44,9 @@
 // blocks, each at most 3 * 2^14 per key, exact in s32 up to 2^15 keys.
 //
 // Measured (eight heads of two KV heads, head_dim 512; warm passes in a graph).
-// 64 nodes at context 32768, 256 query rows a KV head: 306 us, of which scores
+// 64 nodes at context 32768, 256 query rows a KV head: 304 us, of which scores
 // 119 (tensor pipe active 50%, its products alone take 62), softmax 83, values
-// 104 (58%, 46).  16 nodes at context 4096: 36 us (13.6, 8.5, 14), most of it
+// 102 (58%, 46).  16 nodes at context 4096: 35 us (13.6, 8.5, 13), most of it
 // the start and the end of three dependent kernels of one CTA an SM.
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -1006,11 +1006,13 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
   // Row r's sum v of digit products to the output: the bytes'
   // bias, and what the weights' roundings left times the first maximum's value.
   unsigned long long* const acc = reinterpret_cast<unsigned long long*>(ws + g.acc_off) + (int64_t)grow0 * d;
-  auto finish = [&](int r, uint64_t v) {
-    const int32_t wt = s_wsum[r];
+  auto first_value = [&](int r) {  // the first maximum's value
     const int key = t.lo + s_first[r];
-    const int32_t* p = key < t.ctx ? vc + (int64_t)key * d : vt + (int64_t)(key - t.ctx) * d;
-    v += (uint64_t)(kTrBias * wt) + (uint64_t)mul_wide(sub_sat(kOneAct, wt), p[dim]);
+    return (key < t.ctx ? vc + (int64_t)key * d : vt + (int64_t)(key - t.ctx) * d)[dim];
+  };
+  auto finish = [&](int r, uint64_t v, int32_t value) {
+    const int32_t wt = s_wsum[r];
+    v += (uint64_t)(kTrBias * wt) + (uint64_t)mul_wide(sub_sat(kOneAct, wt), value);
     orow(r)[dim] = requantize_flat((int64_t)v);
   };
   if (warp < kTrConvWarps && total > 0) {
@@ -1026,7 +1028,7 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
         const int64_t v = shift_sum(0, c[0][i], c[1][i], c[2][i], c[3][i], c[4][i], c[5][i], 0);
         if (r + i < nr && dim < d) {
           if (S > 1) atomicAdd(acc + (int64_t)(r + i) * d + dim, (unsigned long long)v);
-          else finish(r + i, (uint64_t)v);
+          else finish(r + i, (uint64_t)v, first_value(r + i));
         }
       }
     }
@@ -1039,8 +1041,22 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
     __syncthreads();
     if (s_last && warp < kTrConvWarps && dim < d) {
       __threadfence();
-      for (int r = quarter; r < nr; r += 4)
-        finish(r, __ldcg(acc + (int64_t)r * d + dim));
+      // a thread's rows in flight together (one after the other the sixteen of a
+      // 64-row block took the last CTA 11000 cycles)
+      constexpr int kF = NR == 16 ? 1 : 8;
+      for (int q = quarter; q < nr; q += 4 * kF) {
+        uint64_t v[kF];
+        int32_t value[kF];
+#pragma unroll
+        for (int i = 0; i < kF; ++i) {
+          const int r = min(q + 4 * i, nr - 1);
+          v[i] = __ldcg(acc + (int64_t)r * d + dim);
+          value[i] = first_value(r);
+        }
+#pragma unroll
+        for (int i = 0; i < kF; ++i)
+          if (q + 4 * i < nr) finish(q + 4 * i, v[i], value[i]);
+      }
     }
   }
   fence_before();
