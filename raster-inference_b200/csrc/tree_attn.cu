@@ -488,6 +488,7 @@ __global__ void __launch_bounds__(kQkThreads, 1) tree_qk(const __grid_constant__
     if (++ls == ns) { ls = 0; ++lt; }
     if (++lb == nst) { lb = 0; lph ^= 1; }
   };
+  __syncthreads();  // the barriers are there
   ta_wait();
   ta_go();
   // Query digits: chunk s holds dims [64 s, 64 s + 64) of rows a * NR + r; a
@@ -503,7 +504,6 @@ __global__ void __launch_bounds__(kQkThreads, 1) tree_qk(const __grid_constant__
     for (int s = 0; s < 8; ++s)
       if (s < ns) load4<VEC>(v[s], q, 64 * s + 4 * l16, d, r < nr);
   };
-  __syncthreads();  // the barriers are there
   int32_t qmax = INT32_MIN;
   if (warp > 20) {
     for (int u = 0; u < min(nst, total); ++u) load();
@@ -702,13 +702,13 @@ __global__ void __launch_bounds__(kExThreads) tree_softmax(const __grid_constant
     if (rr % g.nr == 0 && tid < (g.d + 127) / 128) reinterpret_cast<uint32_t*>(ws + g.cnt_off)[items + tid] = 0;
   }
   const int k0 = chunk * g.ex_keys, k1 = min(t.pad, k0 + g.ex_keys);  // (k0 >= k1: no keys)
+  uint4 next;
+  ld16(next, sc + k0 + 4 * tid, k0 + 4 * tid < k1);
   uint32_t top = 0;
   for (int i = lane; i < t.qk_per; i += 32) top = max(top, tmax[i]);
   const uint32_t m = __reduce_max_sync(0xffffffffu, top) ^ 0x80000000u;
   uint64_t sum = 0;
   int32_t first = INT32_MAX;  // the thread's first key at the maximum
-  uint4 next;
-  ld16(next, sc + k0 + 4 * tid, k0 + 4 * tid < k1);
   for (int j = k0 + 4 * tid; j < k1; j += 4 * kExThreads) {
     const uint4 v = next;
     ld16(next, sc + j + 4 * kExThreads, j + 4 * kExThreads < k1);
