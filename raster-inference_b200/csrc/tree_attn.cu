@@ -887,7 +887,9 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
     s_fail = 0;
   }
   if (warp == kTrConvWarps) ta_alloc<512>(&tmem_holder);
-  __syncthreads();  // the barriers are there
+  fence_before();
+  __syncthreads();  // the barriers and TMEM are there
+  fence_after();
   // The values do not depend on the terms: their first stages load before the
   // wait (this grid starts only after the score kernel has completed, and with
   // it everything before it).
@@ -895,31 +897,9 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
     for (int u = 0; u < min(kSt, total); ++u) load();
   ta_wait();
   ta_go();
-  if (warp > kTrConvWarps)
+  if (warp > kTrConvWarps) {
     for (int u = 0; u < min(kSt, total); ++u) load_w(u, u);
-  const int32_t* pw = reinterpret_cast<const int32_t*>(ws + g.sum_off) + (int64_t)grow0 * g.ex_chunks;
-  const int32_t* pidx = reinterpret_cast<const int32_t*>(ws + g.idx_off) + (int64_t)grow0 * g.ex_chunks;
-  if (tid < 8 * NR) {  // eight lanes a row
-    const int r = tid >> 3;
-    int32_t v = 0, f = INT32_MAX;
-    if (r < nr)
-      for (int i = tid & 7; i < g.ex_chunks; i += 8) {
-        v += pw[r * g.ex_chunks + i];
-        f = min(f, pidx[r * g.ex_chunks + i]);
-      }
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) {
-      v += __shfl_xor_sync(0xffffffffu, v, o);
-      f = min(f, __shfl_xor_sync(0xffffffffu, f, o));
-    }
-    if ((tid & 7) == 0) {
-      s_first[r] = f;
-      s_wsum[r] = v;
-    }
   }
-  fence_before();
-  __syncthreads();
-  fence_after();
   constexpr uint32_t tmem = 0;  // all 512 columns, as above
   if (tid == 0 && tmem_holder != 0) s_fail = 1;
   auto wait = [&](uint64_t* bar, uint32_t parity) {
@@ -992,6 +972,26 @@ __global__ void __launch_bounds__(kPvThreads, 1) tree_pv(const __grid_constant__
       const int b = lb;
       load();
       load_w(u, b);
+    }
+    // the rows' first maxima and sums of weights, wanted at the end
+    constexpr int kT = kTrLoaders / NR;  // threads a row
+    const int r = lp / kT;
+    const int64_t at = (int64_t)(grow0 + min(r, nr - 1)) * g.ex_chunks;
+    const int32_t* pw = reinterpret_cast<const int32_t*>(ws + g.sum_off) + at;
+    const int32_t* pidx = reinterpret_cast<const int32_t*>(ws + g.idx_off) + at;
+    int32_t v = 0, f = INT32_MAX;
+    for (int i = lp % kT; i < g.ex_chunks; i += kT) {
+      v += pw[i];
+      f = min(f, pidx[i]);
+    }
+#pragma unroll
+    for (int o = kT / 2; o > 0; o >>= 1) {
+      v += __shfl_xor_sync(0xffffffffu, v, o);
+      f = min(f, __shfl_xor_sync(0xffffffffu, f, o));
+    }
+    if (lp % kT == 0) {
+      s_first[r] = f;
+      s_wsum[r] = v;
     }
     cp_wait_all();
   }
