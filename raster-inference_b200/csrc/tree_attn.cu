@@ -44,9 +44,9 @@
 // blocks, each at most 3 * 2^14 per key, exact in s32 up to 2^15 keys.
 //
 // Measured (eight heads of two KV heads, head_dim 512; warm passes in a graph).
-// 64 nodes at context 32768, 256 query rows a KV head: 304 us, of which scores
+// 64 nodes at context 32768, 256 query rows a KV head: 303 us, of which scores
 // 119 (tensor pipe active 50%, its products alone take 62), softmax 83, values
-// 102 (58%, 46).  16 nodes at context 4096: 35 us (13.6, 8.5, 13), most of it
+// 101 (58%, 46).  16 nodes at context 4096: 35 us (13.6, 8.5, 13), most of it
 // the start and the end of three dependent kernels of one CTA an SM.
 #include <cuda.h>
 #include <cuda_runtime.h>
