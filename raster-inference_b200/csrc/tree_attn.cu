@@ -1192,8 +1192,9 @@ size_t tree_attn_plan(TreeGroup& g) {
   g.qk_items = qk;
   // Keys of a softmax CTA: four per thread, more where the CTAs would not be
   // resident at once (a CTA is mostly latency: 1288 rows of up to 4108 keys take
-  // 46 us in clusters of three CTAs), and so many that a row's cluster has at
-  // most eight CTAs (sixteen for the longest).
+  // 46 us in clusters of three CTAs, 25 with one CTA a row; 128 rows of 4112 keys
+  // 8.5 us in clusters of five, 17 with one), and so many that a row's cluster
+  // has at most eight CTAs (sixteen for the longest).
   g.ex_keys = 4 * kExThreads;
   while ((g.ex_keys < 32 * kExThreads && (int64_t)rows * ceil_div(maxpad, g.ex_keys) > 8 * kSms) ||
          ceil_div(maxpad, g.ex_keys) > (g.ex_keys < kExMostKeys ? 8 : 16))
