@@ -610,6 +610,14 @@ struct Ctx {
   }
   template <typename T>
   T* dalloc_n(size_t n) { return static_cast<T*>(dalloc(n * sizeof(T))); }
+  // A copy to or from host memory behind the stream's work, complete on return.
+  // (cudaMemcpy runs on the legacy default stream, which neither waits for a
+  // non-blocking stream nor is waited for by one: it read synthetic scalars
+  // before their generator had run.)
+  void copy(void* dst, const void* src, size_t bytes, cudaMemcpyKind kind) {
+    CK(cudaMemcpyAsync(dst, src, bytes, kind, stream));
+    CK(cudaStreamSynchronize(stream));
+  }
   ~Ctx() {
     cudaSetDevice(device);
     if (stream) cudaStreamSynchronize(stream);
@@ -764,7 +772,7 @@ struct Loader {
     } else if (synthetic) {
       void* p = upload_raw(n, *t);  // generated on the device, read back once
       c.weight_bytes -= t->bytes;   // held on the host like an artifact scalar
-      CK(cudaMemcpy(out, p, 4, cudaMemcpyDeviceToHost));
+      c.copy(out, p, 4, cudaMemcpyDeviceToHost);
     } else if (t->width == 16) {
       int16_t v;
       memcpy(&v, t->payload, 2);

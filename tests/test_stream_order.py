@@ -1,0 +1,14 @@
+"""Copies and memsets of the runtime are ordered with the context's stream.
+That stream is non-blocking: a copy on the legacy default stream neither
+waits for it nor is waited for by it, so the runtime makes none."""
+import os
+import re
+
+from helpers import ROOT
+
+
+def test_no_copy_reads_back_on_the_default_stream():
+    text = open(os.path.join(ROOT, "raster-inference_b200", "csrc", "runtime.cu")).read()
+    code = re.sub(r"//[^\n]*", "", text)
+    assert "cudaStreamNonBlocking" in code
+    assert not re.findall(r"cudaMemcpy\([^;]*DeviceToHost\)", code)
