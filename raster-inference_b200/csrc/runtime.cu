@@ -760,7 +760,7 @@ struct Loader {
     for (int i = 0; i < len; ++i) { int16_t v; memcpy(&v, src + i, 2); w[i] = v; }
     int32_t* p = c.dalloc_n<int32_t>(len);
     c.weight_bytes += (uint64_t)len * 4;
-    CK(cudaMemcpy(p, w.data(), (size_t)len * 4, cudaMemcpyHostToDevice));
+    c.copy(p, w.data(), (size_t)len * 4, cudaMemcpyHostToDevice);
     return p;
   }
   bool scalar(const std::string& n, int32_t* out) {
@@ -838,7 +838,7 @@ static void build_model(Ctx& c, std::map<std::string, TensorInfo>& tab, bool syn
       if (it == rope_tabs.end()) {
         std::vector<int64_t> t = rope_inv_freq(base, hd, lc.rotary);
         int64_t* dp = c.dalloc_n<int64_t>(t.size());
-        CK(cudaMemcpy(dp, t.data(), t.size() * 8, cudaMemcpyHostToDevice));
+        c.copy(dp, t.data(), t.size() * 8, cudaMemcpyHostToDevice);
         it = rope_tabs.emplace(key, dp).first;
         c.rope_list.emplace_back(dp, lc.rotary / 2);
       }
@@ -913,7 +913,7 @@ static void alloc_workspaces(Ctx& c) {
   if (c.argblocks < 1) c.argblocks = 1;
   d.argpart = c.dalloc_n<int32_t>(2 * c.argblocks);
   c.d_err = c.dalloc_n<int32_t>(1);
-  CK(cudaMemset(c.d_err, 0, 4));
+  CK(cudaMemsetAsync(c.d_err, 0, 4, c.stream));
 }
 
 constexpr size_t kTcSplitScratch = 64ull << 20;  // split-K partials for short row counts
@@ -1078,7 +1078,7 @@ static void check_err_flag(Ctx& c, const char* what) {
   CK(cudaMemcpyAsync(&e, c.d_err, 4, cudaMemcpyDeviceToHost, c.stream));
   CK(cudaStreamSynchronize(c.stream));
   if (e) {
-    CK(cudaMemset(c.d_err, 0, 4));
+    CK(cudaMemsetAsync(c.d_err, 0, 4, c.stream));
     throw Fail{RDET_E_RANGE, std::string(what) + ": token id is out of bounds for the embedding tensor"};
   }
   if (stream_error_flag(true))
@@ -1616,11 +1616,11 @@ static void seq_alloc(Ctx& c, Seq& q, int cap) {
            td_encode_cache_map(maps.data() + (size_t)l * 256 + 128, q.vc[l], rows, lc.head_dim);
     }
     q.d_maps = static_cast<unsigned char*>(q.dalloc(maps.size()));
-    CK(cudaMemcpy(q.d_maps, maps.data(), maps.size(), cudaMemcpyHostToDevice));
+    c.copy(q.d_maps, maps.data(), maps.size(), cudaMemcpyHostToDevice);
     q.maps_ok = ok;
   }
   q.d_pos = static_cast<int32_t*>(q.dalloc(16));
-  CK(cudaMemset(q.d_pos, 0, 16));
+  CK(cudaMemsetAsync(q.d_pos, 0, 16, c.stream));
   q.logits = static_cast<int32_t*>(q.dalloc((size_t)m.V * 4));
   q.d_token = static_cast<uint32_t*>(q.dalloc(16));
   q.d_step = static_cast<int32_t*>(q.dalloc(16));
@@ -3532,7 +3532,8 @@ int32_t rdet_tp_ipc_export(rdet_ctx* ctx, uint32_t max_batch, void* out, size_t 
     t.p2p_rows = (int)max_batch;
     t.recv = c.dalloc_n<int64_t>((size_t)t.world * 2 * t.p2p_rows * c.cfg.H);
     t.flags = c.dalloc_n<uint32_t>(32);
-    CK(cudaMemset(t.flags, 0, 32 * sizeof(uint32_t)));
+    CK(cudaMemsetAsync(t.flags, 0, 32 * sizeof(uint32_t), c.stream));
+    CK(cudaStreamSynchronize(c.stream));  // before a peer can raise one
     cudaIpcMemHandle_t h[2];
     CK(cudaIpcGetMemHandle(&h[0], t.recv));
     CK(cudaIpcGetMemHandle(&h[1], t.flags));

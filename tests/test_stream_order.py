@@ -12,3 +12,9 @@ def test_no_copy_reads_back_on_the_default_stream():
     code = re.sub(r"//[^\n]*", "", text)
     assert "cudaStreamNonBlocking" in code
     assert not re.findall(r"cudaMemcpy\([^;]*DeviceToHost\)", code)
+
+
+def test_no_copy_or_memset_on_the_default_stream():
+    text = open(os.path.join(ROOT, "raster-inference_b200", "csrc", "runtime.cu")).read()
+    code = re.sub(r"//[^\n]*", "", text)
+    assert not re.findall(r"cudaMemcpy\(|cudaMemset\(|cudaMemcpy2D\(|cudaMemcpyToSymbol\(", code)
