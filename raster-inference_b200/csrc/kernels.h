@@ -141,7 +141,7 @@ struct TcOut {
 // false when y64 is asked for and the scratch cannot hold the partial sums
 bool launch_tc_linear(const TcAct& a, const TcWeight& w, const TcOut& o, cudaStream_t s);
 void tc_init();  // per-device kernel attributes (called by kernels_init)
-int tc_error_flag(bool reset);  // nonzero when a tensor-core pipeline wait gave up
+int32_t* tc_error_word();  // (device) nonzero when a tensor-core pipeline wait gave up
 
 // ---- row ops -------------------------------------------------------------------
 // y[s] = rmsnorm(x[s], g)   (g == nullptr: weightless value norm)
@@ -304,7 +304,7 @@ bool launch_attn_decode_tc(const AttnDecodeArgs& a, int sms, cudaStream_t s);
 // [rows][d] i32 that launch_attn_decode_tc reads: 32 x 64 boxes, 128-byte
 // swizzle.  False when d is not a multiple of 128 or encoding fails.
 bool td_encode_cache_map(void* out, const int32_t* base, int rows, int d);
-int tc_attn_dec_error_flag(bool reset);
+int32_t* tc_attn_dec_error_word();
 void tc_attn_dec_init();
 // Whether launch_attn_decode_cluster runs the cluster kernel for this shape
 // (rotary: the fused prologue's rotary width, 0 when not fused).  When it
@@ -336,7 +336,7 @@ size_t tc_attn_ws_bytes(int S, int Hq, int Hkv, int d);
 bool tc_attn_eligible(int S, int Hq, int Hkv, int d);
 bool launch_attn_prefill_tc(const AttnPrefillArgs& a, void* ws, size_t ws_bytes, cudaStream_t s);
 void tc_attn_init();                 // per-device kernel attributes (called by kernels_init)
-int tc_attn_error_flag(bool reset);  // nonzero when one of its pipeline waits gave up
+int32_t* tc_attn_error_word();       // (device) nonzero when one of its pipeline waits gave up
 
 // ---- embedding / PLE / logits ------------------------------------------------------
 void launch_embed(const uint32_t* ids, int32_t S, const DevMat& emb, int32_t scale, int32_t* out, int32_t* err,
@@ -416,7 +416,7 @@ struct TreeGroup {
 size_t tree_attn_plan(TreeGroup& g);           // returns the workspace bytes
 void launch_tree_attn(const TreeGroup& g, cudaStream_t s);
 void tree_attn_init();                         // per-device kernel attributes (called by kernels_init)
-int tree_attn_error_flag(bool reset);          // nonzero when one of its pipeline waits gave up
+int32_t* tree_attn_error_word();               // (device) nonzero when one of its pipeline waits gave up
 
 // Rules on logits rows (rdet_det_logits_rules): rows by value.
 constexpr int kRuleRows = 192;
@@ -487,7 +487,15 @@ int sm_count();
 // one-time kernel attributes of the current device (idempotent; call outside
 // stream capture before the first launch on a device)
 void kernels_init();
-// nonzero when a bounded pipeline wait in a streamed kernel gave up (reset: clear it)
-int stream_error_flag(bool reset);
+// The kernels' error words on the current device, each nonzero when a bounded
+// pipeline wait of one file's kernels gave up.
+constexpr int kErrorWords = 5;
+struct ErrorWords {
+  int32_t* w[kErrorWords];
+};
+ErrorWords error_words();
+// out[0] = *first (0 for nullptr), out[1] = whether some error word is set, and
+// clears what was set; out: two ints that the device can write (pinned host memory).
+void launch_error_words(const ErrorWords& w, int32_t* first, int32_t* out, cudaStream_t s);
 
 }  // namespace rdet

@@ -541,6 +541,8 @@ struct Ctx {
   PrefillWs pw;
   DecodeWs dw;
   int32_t* d_err = nullptr;
+  ErrorWords err_words{};        // the kernels' error words on this device
+  int32_t* h_err = nullptr;      // pinned: d_err and whether an error word is set, as last read
   int argblocks = 0;
   // rdet_select_batch: row pointer table, chunk pairs and tokens for up to sel_rows rows
   int sel_rows = 0;
@@ -636,6 +638,7 @@ struct Ctx {
       if (e) cudaEventDestroy(e);
     if (kvs.host) cudaFreeHost(kvs.host);
     if (rules.host) cudaFreeHost(rules.host);
+    if (h_err) cudaFreeHost(h_err);
     for (void* p : tp.ipc_opened) cudaIpcCloseMemHandle(p);
     if (tp.comm) nccl_api().commDestroy(tp.comm);
     for (void* p : allocs) cudaFree(p);
@@ -914,6 +917,10 @@ static void alloc_workspaces(Ctx& c) {
   d.argpart = c.dalloc_n<int32_t>(2 * c.argblocks);
   c.d_err = c.dalloc_n<int32_t>(1);
   CK(cudaMemsetAsync(c.d_err, 0, 4, c.stream));
+  void* h = nullptr;
+  CK(cudaHostAlloc(&h, 8, cudaHostAllocDefault));
+  c.h_err = static_cast<int32_t*>(h);
+  c.err_words = error_words();
 }
 
 constexpr size_t kTcSplitScratch = 64ull << 20;  // split-K partials for short row counts
@@ -1074,15 +1081,11 @@ static bool row_norm(Ctx& c, RowNormArgs ra, int B, ActPlanes* ap) {
 }
 
 static void check_err_flag(Ctx& c, const char* what) {
-  int32_t e = 0;
-  CK(cudaMemcpyAsync(&e, c.d_err, 4, cudaMemcpyDeviceToHost, c.stream));
+  launch_error_words(c.err_words, c.d_err, c.h_err, c.stream);
+  CK(cudaGetLastError());
   CK(cudaStreamSynchronize(c.stream));
-  if (e) {
-    CK(cudaMemsetAsync(c.d_err, 0, 4, c.stream));
-    throw Fail{RDET_E_RANGE, std::string(what) + ": token id is out of bounds for the embedding tensor"};
-  }
-  if (stream_error_flag(true))
-    throw Fail{RDET_E_CUDA, std::string(what) + ": a weight-streaming pipeline wait timed out"};
+  if (c.h_err[1]) throw Fail{RDET_E_CUDA, std::string(what) + ": a weight-streaming pipeline wait timed out"};
+  if (c.h_err[0]) throw Fail{RDET_E_RANGE, std::string(what) + ": token id is out of bounds for the embedding tensor"};
 }
 
 // ---------------------------------------------------------------------------

@@ -47,7 +47,7 @@
 
 namespace rdet {
 
-// set when a bounded pipeline wait gives up (read by tc_attn_error_flag)
+// set when a bounded pipeline wait gives up (read by launch_error_words)
 __device__ int g_ta_err = 0;
 
 namespace {
@@ -663,14 +663,10 @@ bool ta_shape(TaParams& p, int S, int Hq, int Hkv, int d) {
 
 }  // namespace
 
-int tc_attn_error_flag(bool reset) {
-  int v = 0;
-  cudaMemcpyFromSymbol(&v, g_ta_err, sizeof(int));
-  if (reset && v) {
-    int z = 0;
-    cudaMemcpyToSymbol(g_ta_err, &z, sizeof(int));
-  }
-  return v;
+int32_t* tc_attn_error_word() {
+  void* p = nullptr;
+  cudaGetSymbolAddress(&p, g_ta_err);
+  return static_cast<int32_t*>(p);
 }
 
 void tc_attn_init() {

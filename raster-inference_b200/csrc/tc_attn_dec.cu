@@ -57,7 +57,7 @@
 
 namespace rdet {
 
-// set when a bounded wait gives up (read by tc_attn_dec_error_flag)
+// set when a bounded wait gives up (read by launch_error_words)
 __device__ int g_tad_err = 0;
 
 namespace {
@@ -699,14 +699,10 @@ void tc_attn_dec_init() {
   done[dev] = 1;
 }
 
-int tc_attn_dec_error_flag(bool reset) {
-  int v = 0;
-  cudaMemcpyFromSymbol(&v, g_tad_err, sizeof(int));
-  if (reset && v) {
-    int z = 0;
-    cudaMemcpyToSymbol(g_tad_err, &z, sizeof(int));
-  }
-  return v;
+int32_t* tc_attn_dec_error_word() {
+  void* p = nullptr;
+  cudaGetSymbolAddress(&p, g_tad_err);
+  return static_cast<int32_t*>(p);
 }
 
 bool td_encode_cache_map(void* out, const int32_t* base, int rows, int d) {

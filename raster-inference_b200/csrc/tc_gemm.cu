@@ -47,7 +47,7 @@
 
 namespace rdet {
 
-// set when a bounded pipeline wait gives up (read by tc_error_flag)
+// set when a bounded pipeline wait gives up (read by launch_error_words)
 __device__ int g_tc_err = 0;
 // the CTA-pair GEMM for prompts of more than 128 tokens (0: one-CTA tiles;
 // RDET_TC_PAIR=0 in the environment selects them)
@@ -1033,14 +1033,10 @@ bool encode_u8_planes(void* out, const uint8_t* base, int nplanes, int rows, int
 
 static_assert(sizeof(CUtensorMap) <= sizeof(TcAct::map), "tensor map storage");
 
-int tc_error_flag(bool reset) {
-  int v = 0;
-  cudaMemcpyFromSymbol(&v, g_tc_err, sizeof(int));
-  if (reset && v) {
-    int z = 0;
-    cudaMemcpyToSymbol(g_tc_err, &z, sizeof(int));
-  }
-  return v;
+int32_t* tc_error_word() {
+  void* p = nullptr;
+  cudaGetSymbolAddress(&p, g_tc_err);
+  return static_cast<int32_t*>(p);
 }
 
 void tc_init() {

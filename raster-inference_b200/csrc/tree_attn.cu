@@ -60,7 +60,7 @@
 
 namespace rdet {
 
-// set when a bounded wait gives up (read by tree_attn_error_flag)
+// set when a bounded wait gives up (read by launch_error_words)
 __device__ int g_tree_err = 0;
 
 namespace {
@@ -1096,14 +1096,10 @@ void tree_attn_init() {
   pv_attr<64, false>();
 }
 
-int tree_attn_error_flag(bool reset) {
-  int v = 0;
-  cudaMemcpyFromSymbol(&v, g_tree_err, sizeof(int));
-  if (reset && v) {
-    int z = 0;
-    cudaMemcpyToSymbol(g_tree_err, &z, sizeof(int));
-  }
-  return v;
+int32_t* tree_attn_error_word() {
+  void* p = nullptr;
+  cudaGetSymbolAddress(&p, g_tree_err);
+  return static_cast<int32_t*>(p);
 }
 
 size_t tree_attn_plan(TreeGroup& g) {

@@ -18,3 +18,12 @@ def test_no_copy_or_memset_on_the_default_stream():
     text = open(os.path.join(ROOT, "raster-inference_b200", "csrc", "runtime.cu")).read()
     code = re.sub(r"//[^\n]*", "", text)
     assert not re.findall(r"cudaMemcpy\(|cudaMemset\(|cudaMemcpy2D\(|cudaMemcpyToSymbol\(", code)
+
+
+def test_error_words_are_not_copied_one_by_one():
+    # a symbol copy runs on the legacy default stream and waits for itself
+    csrc = os.path.join(ROOT, "raster-inference_b200", "csrc")
+    for name in sorted(os.listdir(csrc)):
+        if name.endswith(".cu"):
+            code = re.sub(r"//[^\n]*", "", open(os.path.join(csrc, name)).read())
+            assert not re.findall(r"cudaMemcpy(?:From|To)Symbol\(", code), name
