@@ -18,14 +18,17 @@
 #include <map>
 #include <memory>
 #include <mutex>
+#include <set>
 #include <stdexcept>
 #include <string>
 #include <thread>
+#include <tuple>
 #include <vector>
 
 #include <nccl.h>  // types only: libnccl is loaded at run time
 
 #include "det_dev.cuh"
+#include "dev_buf.h"
 #include "json.h"
 #include "kernels.h"
 #include "rdet.h"
@@ -589,8 +592,7 @@ struct Ctx {
     int32_t* pos = nullptr;        // [rows] node positions, [rows] cache rows
     int32_t* dec_out = nullptr;    // [rows][L, H] per-layer outputs
     int32_t* logits = nullptr;     // [rows, V]
-    void* ws = nullptr;            // workspace of the tree attention
-    size_t ws_bytes = 0;
+    GrowBuf ws;                    // workspace of the tree attention
   } tree;
   // selection under rules: tokens (up to rows), the rules' arrays in pinned and device memory
   struct {
@@ -612,6 +614,7 @@ struct Ctx {
   }
   template <typename T>
   T* dalloc_n(size_t n) { return static_cast<T*>(dalloc(n * sizeof(T))); }
+  void* alloc(size_t bytes) { return dalloc(bytes); }  // for the growing buffers
   // A copy to or from host memory behind the stream's work, complete on return.
   // (cudaMemcpy runs on the legacy default stream, which neither waits for a
   // non-blocking stream nor is waited for by one: it read synthetic scalars
@@ -1885,18 +1888,38 @@ struct TreeBatch {
   std::vector<TreeGroup> groups;       // launch groups of the attention, without the layer's caches
   std::vector<std::vector<Seq*>> seqs; // the sequences of each group
 };
+// The shapes of layer l's attention, and the workspace of the groups at them.
+static size_t tree_plan(const Ctx& c, TreeBatch& tb, int l) {
+  const LayerCfg& lc = c.cfg.layers[l];
+  size_t need = 0;
+  for (TreeGroup& g : tb.groups) {
+    g.Hq = c.cfg.Hq;
+    g.Hkv = lc.kv_heads;
+    g.d = lc.head_dim;
+    g.window = lc.window;
+    need = std::max(need, tree_attn_plan(g));
+  }
+  return need;
+}
+// The workspace that the pass needs at most, over its layers' different shapes.
+static size_t tree_workspace(const Ctx& c, TreeBatch& tb) {
+  std::set<std::tuple<int, int, int>> seen;
+  size_t need = 0;
+  for (int l = 0; l < c.cfg.L; ++l) {
+    const LayerCfg& lc = c.cfg.layers[l];
+    if (seen.emplace(lc.kv_heads, lc.head_dim, lc.window).second) need = std::max(need, tree_plan(c, tb, l));
+  }
+  return need;
+}
 // The tree attention of layer l over `q`, the caches holding the nodes' rows
 // from each sequence's position on.
 static void tree_attention(Ctx& c, TreeBatch& tb, int l, const int32_t* q, int32_t* out) {
   const LayerCfg& lc = c.cfg.layers[l];
   const int own = lc.donor < 0 ? l : lc.donor, d = lc.head_dim;
   size_t node = 0;
+  REQUIRE(tree_plan(c, tb, l) <= c.tree.ws.bytes, RDET_E_CUDA, "tree attention: the pass's workspace is too small");
   for (size_t i = 0; i < tb.groups.size(); ++i) {
     TreeGroup& g = tb.groups[i];
-    g.Hq = c.cfg.Hq;
-    g.Hkv = lc.kv_heads;
-    g.d = d;
-    g.window = lc.window;
     for (int j = 0; j < g.nseq; ++j) {
       const Seq& s = *tb.seqs[i][j];
       TreeSeq& t = g.seq[j];
@@ -1906,14 +1929,9 @@ static void tree_attention(Ctx& c, TreeBatch& tb, int l, const int32_t* q, int32
       t.vt = t.v + (size_t)t.ctx * d;
       t.kstride = t.tstride = (int64_t)s.cap * d;
     }
-    const size_t need = tree_attn_plan(g);
-    if (c.tree.ws_bytes < need) {  // doubled, so that growing contexts replace it rarely
-      c.tree.ws_bytes = 2 * need;
-      c.tree.ws = c.dalloc(c.tree.ws_bytes);
-    }
     g.q = q + node * c.cfg.Hq * d;
     g.out = out + node * c.cfg.Hq * d;
-    g.ws = c.tree.ws;
+    g.ws = c.tree.ws.p;
     launch_tree_attn(g, c.stream);
     node += (size_t)g.nnode;
   }
@@ -2483,6 +2501,7 @@ static void tree_decode(Ctx& c, const std::vector<Seq*>& seqs, const uint32_t* c
   }
   for (int r = nodes; r < B; ++r)
     rows[r] = BatchRow{seqs[0], tr.pos + r, tr.dec_out + (size_t)r * m.L * m.H, tr.logits + (size_t)r * m.V};
+  tr.ws.reserve(c, tree_workspace(c, tb));
   tr.epoch += 1;  // earlier trees' buffers are overwritten from here on
   CK(cudaMemcpyAsync(tr.pos, host.data(), host.size() * 4, cudaMemcpyHostToDevice, c.stream));
   batch_tables(c, rows);

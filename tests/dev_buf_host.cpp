@@ -1,0 +1,60 @@
+// The growing buffers of a context over a host allocator that fails on demand.
+#include <cstdint>
+#include <map>
+#include <stdexcept>
+
+#include "dev_buf.h"
+
+namespace {
+struct FakeAlloc {
+  std::map<void*, size_t> live;
+  uintptr_t next = 4096;
+  uint64_t fail = 0;  // bit i: the i-th call from now on fails
+  int calls = 0;
+  size_t most = 0, held = 0;
+  void* alloc(size_t bytes) {
+    const bool bad = fail >> calls & 1;
+    ++calls;
+    if (bad) throw std::runtime_error("no memory");
+    void* p = reinterpret_cast<void*>(next);
+    next += (bytes + 4095) / 4096 * 4096 + 4096;
+    live[p] = bytes;
+    held += bytes;
+    if (held > most) most = held;
+    return p;
+  }
+  void arm(uint64_t f) {
+    fail = f;
+    calls = 0;
+  }
+  // the buffer lies in live memory of at least the size that it claims
+  bool holds(const void* p, size_t bytes) const {
+    const auto it = live.find(const_cast<void*>(p));
+    return bytes == 0 ? true : it != live.end() && it->second >= bytes;
+  }
+};
+}  // namespace
+
+extern "C" {
+// 0: after every request of a workspace, failed ones among them, it holds what it claims
+int workspace(uint64_t fail_first, uint64_t fail_second) {
+  FakeAlloc a;
+  rdet::GrowBuf b;
+  const size_t needs[] = {1000, 900, 5000, 5000, 5000};
+  const uint64_t fails[] = {fail_first, 0, fail_second, 3, 0};
+  for (int i = 0; i < 5; ++i) {
+    const rdet::GrowBuf before = b;
+    a.arm(fails[i]);
+    bool failed = false;
+    try {
+      b.reserve(a, needs[i]);
+    } catch (const std::exception&) {
+      failed = true;
+    }
+    if (!a.holds(b.p, b.bytes)) return 1 + i;
+    if (failed ? b.p != before.p || b.bytes != before.bytes : b.bytes < needs[i]) return 11 + i;
+    if (i == 4 && failed) return 21;
+  }
+  return 0;
+}
+}

@@ -1,0 +1,45 @@
+"""The buffers that a context replaces as its calls grow (dev_buf.h), compiled
+for the host with an allocator that fails: a request that fails leaves what
+was there, under its own size."""
+import ctypes as C
+import os
+import re
+import subprocess
+import tempfile
+
+import pytest
+
+from helpers import ROOT
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+CSRC = os.path.join(ROOT, "raster-inference_b200", "csrc")
+
+
+@pytest.fixture(scope="module")
+def host():
+    out = os.path.join(tempfile.mkdtemp(prefix="dev-buf-"), "dev_buf.so")
+    r = subprocess.run(["g++", "-O1", "-std=c++17", "-shared", "-fPIC", "-I", CSRC, os.path.join(HERE, "dev_buf_host.cpp"),
+                        "-o", out], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+    L = C.CDLL(out)
+    L.workspace.argtypes = [C.c_uint64, C.c_uint64]
+    return L
+
+
+def runtime():
+    return re.sub(r"//[^\n]*", "", open(os.path.join(CSRC, "runtime.cu")).read())
+
+
+@pytest.mark.parametrize("first", range(4))
+@pytest.mark.parametrize("second", range(4))
+def test_a_failed_workspace_keeps_its_size(host, first, second):
+    assert host.workspace(first, second) == 0
+
+
+def test_the_tree_workspace_is_reserved_before_the_pass():
+    # nothing is allocated between the layers of a pass that has begun
+    code = runtime()
+    body = code[code.index("static void tree_attention("):]
+    body = body[:body.index("\n}\n")]
+    assert "dalloc" not in body and "reserve" not in body
+    assert "tree.ws_bytes" not in code
