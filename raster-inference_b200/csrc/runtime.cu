@@ -528,6 +528,18 @@ struct KvStage {
   cudaEvent_t ev[2] = {nullptr, nullptr};
 };
 
+// Device memory.  A failure leaves no error behind: the next check of a launch
+// would take it for its own.
+static void* device_alloc(size_t bytes) {
+  void* p = nullptr;
+  const cudaError_t e = cudaMalloc(&p, bytes ? bytes : 16);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    throw Fail{RDET_E_OOM, std::string("cudaMalloc failed: ") + cudaGetErrorString(e)};
+  }
+  return p;
+}
+
 struct Ctx {
   int device = 0;
   cudaStream_t stream = nullptr;
@@ -606,11 +618,8 @@ struct Ctx {
   KvStage kvs;
 
   void* dalloc(size_t bytes) {
-    void* p = nullptr;
-    cudaError_t e = cudaMalloc(&p, bytes ? bytes : 16);
-    if (e != cudaSuccess) throw Fail{RDET_E_OOM, std::string("cudaMalloc failed: ") + cudaGetErrorString(e)};
-    allocs.push_back(p);
-    return p;
+    allocs.push_back(device_alloc(bytes));
+    return allocs.back();
   }
   template <typename T>
   T* dalloc_n(size_t n) { return static_cast<T*>(dalloc(n * sizeof(T))); }
@@ -694,11 +703,8 @@ struct Seq {
   int graph_kernels = 0;
   std::vector<void*> allocs;
   void* dalloc(size_t bytes) {
-    void* p = nullptr;
-    cudaError_t e = cudaMalloc(&p, bytes ? bytes : 16);
-    if (e != cudaSuccess) throw Fail{RDET_E_OOM, std::string("cudaMalloc failed: ") + cudaGetErrorString(e)};
-    allocs.push_back(p);
-    return p;
+    allocs.push_back(device_alloc(bytes));
+    return allocs.back();
   }
   int device = 0;
   ~Seq() {
@@ -2799,6 +2805,7 @@ static int32_t guard(F&& f) {
     f();
     return RDET_OK;
   } catch (const Fail& e) {
+    cudaGetLastError();  // the next call's checks of its launches must not find this call's error
     g_last_error = e.msg;
     return e.code;
   } catch (const std::bad_alloc&) {
