@@ -2,6 +2,7 @@
 // gives the memory: void* alloc(size_t), which throws where there is none.
 #pragma once
 #include <cstddef>
+#include <cstdint>
 
 namespace rdet {
 
@@ -26,5 +27,34 @@ struct GrowBuf {
     bytes = want;
   }
 };
+
+// Rows of one size, `extra` bytes for all of them together.
+struct GrowRows {
+  void* p = nullptr;
+  int rows = 0;
+  template <class A>
+  void reserve(A& a, int need, int least, size_t row_bytes, size_t extra) {
+    if (rows >= need) return;
+    const int want = need > least ? need : least;
+    p = a.alloc((size_t)want * row_bytes + extra);
+    rows = want;
+  }
+};
+
+// What a pass over drafted trees needs: the batch tables, a workspace, and the
+// rows that hold the trees' outputs until a path is accepted.  Those come last
+// and the epoch, which ends earlier trees, after them: a call that fails here
+// leaves every tree of an earlier one as it was.
+struct PassNeed {
+  int rows;
+  size_t table_row, table_extra, workspace, tree_row, tree_extra;
+};
+template <class A>
+void reserve_pass(A& a, const PassNeed& n, GrowRows& tables, GrowBuf& ws, GrowRows& tree, uint64_t& epoch) {
+  tables.reserve(a, n.rows, 8, n.table_row, n.table_extra);
+  ws.reserve(a, n.workspace);
+  tree.reserve(a, n.rows, 64, n.tree_row, n.tree_extra);
+  epoch += 1;
+}
 
 }  // namespace rdet

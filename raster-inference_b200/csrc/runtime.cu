@@ -583,7 +583,7 @@ struct Ctx {
   // batched decode: per-row tables (device) and the batch logits
   struct {
     int rows = 0;                  // rows the tables hold
-    void* mem = nullptr;           // one allocation for every table below
+    GrowRows mem;                  // one allocation for every table below
     uint32_t* ids = nullptr;
     int32_t** pos = nullptr;       // [rows] each sequence's device position
     int32_t* caps = nullptr;       // [rows]
@@ -599,7 +599,7 @@ struct Ctx {
   TpState tp;
   // drafted trees (rdet_tree_decode): one row per node of the last call
   struct {
-    int rows = 0;                  // rows the buffers hold
+    GrowRows mem;                  // one allocation for every buffer below
     uint64_t epoch = 0;            // tree decodes so far
     int32_t* pos = nullptr;        // [rows] node positions, [rows] cache rows
     int32_t* dec_out = nullptr;    // [rows][L, H] per-layer outputs
@@ -1833,29 +1833,26 @@ struct BatchRow {
   int32_t* dec_out;  // [L, H]
   int32_t* logits;   // [V]
 };
+// Bytes of one row of the batch tables: its pointers, id, capacity, place and logits.
+static size_t batch_row_bytes(const ModelCfg& m) { return (4 + 2 * (size_t)m.L) * 8 + 12 + (size_t)m.V * 4; }
+static void batch_reserve(Ctx& c, int B) { c.bw.mem.reserve(c, B, 8, batch_row_bytes(c.cfg), 256); }
 static void batch_tables(Ctx& c, const std::vector<BatchRow>& in) {
   const ModelCfg& m = c.cfg;
   auto& bw = c.bw;
   const int B = (int)in.size();
-  if (bw.rows < B) {
-    const int rows = std::max(B, 8);
-    const size_t ptrs = (size_t)rows * (4 + 2 * (size_t)m.L);
-    const size_t bytes = ptrs * 8 + (size_t)rows * 12 + (size_t)rows * m.V * 4 + 256;
-    bw.mem = c.dalloc(bytes);
-    auto* base = static_cast<unsigned char*>(bw.mem);
-    bw.pos = reinterpret_cast<int32_t**>(base);
-    bw.dec_out = bw.pos + rows;
-    bw.logits_dst = bw.dec_out + rows;
-    bw.kc = bw.logits_dst + rows;
-    bw.vc = bw.kc + (size_t)m.L * rows;
-    bw.maps = reinterpret_cast<const unsigned char**>(reinterpret_cast<uintptr_t>(bw.vc + (size_t)m.L * rows));
-    bw.ids = reinterpret_cast<uint32_t*>(reinterpret_cast<uintptr_t>(bw.maps + rows));
-    bw.caps = reinterpret_cast<int32_t*>(bw.ids + rows);
-    bw.order = bw.caps + rows;
-    bw.logits = reinterpret_cast<int32_t*>((reinterpret_cast<uintptr_t>(bw.order + rows) + 255) & ~(uintptr_t)255);
-    bw.rows = rows;
-  }
-  const int rows = bw.rows;
+  batch_reserve(c, B);
+  const int rows = bw.rows = bw.mem.rows;
+  auto* base = static_cast<unsigned char*>(bw.mem.p);
+  bw.pos = reinterpret_cast<int32_t**>(base);
+  bw.dec_out = bw.pos + rows;
+  bw.logits_dst = bw.dec_out + rows;
+  bw.kc = bw.logits_dst + rows;
+  bw.vc = bw.kc + (size_t)m.L * rows;
+  bw.maps = reinterpret_cast<const unsigned char**>(reinterpret_cast<uintptr_t>(bw.vc + (size_t)m.L * rows));
+  bw.ids = reinterpret_cast<uint32_t*>(reinterpret_cast<uintptr_t>(bw.maps + rows));
+  bw.caps = reinterpret_cast<int32_t*>(bw.ids + rows);
+  bw.order = bw.caps + rows;
+  bw.logits = reinterpret_cast<int32_t*>((reinterpret_cast<uintptr_t>(bw.order + rows) + 255) & ~(uintptr_t)255);
   std::vector<int32_t*> host((size_t)rows * (4 + 2 * (size_t)m.L), nullptr);
   bw.maps_ok = true;
   std::vector<int32_t> caps(2 * (size_t)rows, 0);  // [caps | row order]
@@ -2465,17 +2462,9 @@ static void tree_decode(Ctx& c, const std::vector<Seq*>& seqs, const uint32_t* c
   // CUDA-core linear of fewer rows (one token by rdet_decode: 4.0 ms).
   const int B = c.tc && c.max_prefill >= (uint32_t)kTcMinRows ? std::max(nodes, kTcMinRows) : nodes;
   auto& tr = c.tree;
-  if (tr.rows < B) {
-    const int rows = std::max(B, 64);
-    tr.pos = c.dalloc_n<int32_t>(2 * (size_t)rows);
-    tr.dec_out = c.dalloc_n<int32_t>((size_t)rows * m.L * m.H);
-    tr.logits = c.dalloc_n<int32_t>((size_t)rows * m.V);
-    tr.rows = rows;
-  }
   TreeBatch tb;
   tb.nodes = nodes;
-  tb.slots = tr.pos + tr.rows;
-  std::vector<int32_t> host(2 * (size_t)tr.rows, 0);  // [positions | cache rows]
+  std::vector<int32_t> host(2 * (size_t)B, 0);  // [positions | cache rows]
   std::vector<BatchRow> rows(B);
   std::vector<uint32_t> ids(B, 0);
   int maxcap = 0, row = 0;
@@ -2498,17 +2487,27 @@ static void tree_decode(Ctx& c, const std::vector<Seq*>& seqs, const uint32_t* c
       depth[j] = p >= 0 ? depth[p] + 1 : 0;
       g.mask[g.nnode + j] = (p >= 0 ? g.mask[g.nnode + p] : 0) | 1ull << j;
       host[row] = q.pos + depth[j];
-      host[tr.rows + row] = q.pos + j;
-      rows[row] = BatchRow{&q, tr.pos + row, tr.dec_out + (size_t)row * m.L * m.H, tr.logits + (size_t)row * m.V};
+      host[B + row] = q.pos + j;
+      rows[row].q = &q;
       ids[row] = tokens[row];
     }
     g.nnode += n;
     maxcap = std::max(maxcap, q.cap);
   }
-  for (int r = nodes; r < B; ++r)
-    rows[r] = BatchRow{seqs[0], tr.pos + r, tr.dec_out + (size_t)r * m.L * m.H, tr.logits + (size_t)r * m.V};
-  tr.ws.reserve(c, tree_workspace(c, tb));
-  tr.epoch += 1;  // earlier trees' buffers are overwritten from here on
+  reserve_pass(c, PassNeed{B, batch_row_bytes(m), 256, tree_workspace(c, tb), (2 + (size_t)m.L * m.H + m.V) * 4, 512},
+               c.bw.mem, tr.ws, tr.mem, tr.epoch);
+  // nothing below fails for want of memory; earlier trees' buffers are overwritten
+  auto up = [](void* p) { return reinterpret_cast<int32_t*>((reinterpret_cast<uintptr_t>(p) + 255) & ~(uintptr_t)255); };
+  tr.pos = static_cast<int32_t*>(tr.mem.p);
+  tr.dec_out = up(tr.pos + 2 * (size_t)tr.mem.rows);
+  tr.logits = up(tr.dec_out + (size_t)tr.mem.rows * m.L * m.H);
+  tb.slots = tr.pos + B;
+  for (int r = 0; r < B; ++r) {
+    if (r >= nodes) rows[r].q = seqs[0];
+    rows[r].pos = tr.pos + r;
+    rows[r].dec_out = tr.dec_out + (size_t)r * m.L * m.H;
+    rows[r].logits = tr.logits + (size_t)r * m.V;
+  }
   CK(cudaMemcpyAsync(tr.pos, host.data(), host.size() * 4, cudaMemcpyHostToDevice, c.stream));
   batch_tables(c, rows);
   batch_pass(c, ids.data(), B, nodes, maxcap, &tb);

@@ -57,4 +57,33 @@ int workspace(uint64_t fail_first, uint64_t fail_second) {
   }
   return 0;
 }
+
+// Passes of growing and falling row counts; in the one numbered `victim` the
+// allocations of `fail` fail.  0: a failed pass leaves the trees' rows and the
+// epoch as they were, and everything holds what it claims.
+int passes(int victim, uint64_t fail) {
+  FakeAlloc a;
+  rdet::GrowRows tables, tree;
+  rdet::GrowBuf ws;
+  uint64_t epoch = 7;
+  const int rows[] = {1, 40, 200, 30, 900, 900, 2000};
+  for (int i = 0; i < 7; ++i) {
+    const rdet::GrowRows tree0 = tree;
+    const uint64_t epoch0 = epoch;
+    const rdet::PassNeed n{rows[i], 4000, 256, (size_t)rows[i] * 3000, 9000, 768};
+    a.arm(i == victim ? fail : 0);
+    bool failed = false;
+    try {
+      rdet::reserve_pass(a, n, tables, ws, tree, epoch);
+    } catch (const std::exception&) {
+      failed = true;
+    }
+    if (failed && (i != victim || tree.p != tree0.p || tree.rows != tree0.rows || epoch != epoch0)) return 1 + i;
+    if (!failed && (epoch != epoch0 + 1 || tree.rows < rows[i] || tables.rows < rows[i] || ws.bytes < n.workspace)) return 11 + i;
+    if (!a.holds(tree.p, tree.rows ? (size_t)tree.rows * n.tree_row + n.tree_extra : 0)) return 21 + i;
+    if (!a.holds(tables.p, tables.rows ? (size_t)tables.rows * n.table_row + n.table_extra : 0)) return 31 + i;
+    if (!a.holds(ws.p, ws.bytes)) return 41 + i;
+  }
+  return 0;
+}
 }

@@ -23,6 +23,7 @@ def host():
     assert r.returncode == 0, r.stderr
     L = C.CDLL(out)
     L.workspace.argtypes = [C.c_uint64, C.c_uint64]
+    L.passes.argtypes = [C.c_int, C.c_uint64]
     return L
 
 
@@ -43,3 +44,18 @@ def test_the_tree_workspace_is_reserved_before_the_pass():
     body = body[:body.index("\n}\n")]
     assert "dalloc" not in body and "reserve" not in body
     assert "tree.ws_bytes" not in code
+
+
+@pytest.mark.parametrize("victim", range(7))
+def test_a_failed_pass_keeps_the_trees_before_it(host, victim):
+    for fail in range(64):
+        assert host.passes(victim, fail) == 0, fail
+
+
+def test_a_pass_takes_its_memory_at_once():
+    # tree_decode allocates through reserve_pass alone, which ends the trees before it last
+    code = runtime()
+    body = code[code.index("static void tree_decode("):]
+    body = body[:body.index("\n}\n")]
+    assert "dalloc" not in body and "epoch +=" not in body and body.count("reserve_pass(") == 1
+    assert not re.search(r"\btr\.(dec_out|logits|pos|rows)\s*=", body[:body.index("reserve_pass(")])

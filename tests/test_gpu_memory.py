@@ -25,3 +25,34 @@ def test_a_refused_sequence_leaves_the_context_usable():
         m.new_sequence(2_000_000_000)
     rdet.decode_batch(m, [a, b], [6, 6])
     assert a.select() == b.select()
+
+
+def test_a_refused_tree_decode_keeps_the_trees_before_it():
+    # 8192 rows of 4 million logits: the batch tables take 137 GB, and the trees'
+    # rows, as large again, are not to be had
+    cfg = mini_config(vocab_size=1 << 22, hidden_size_per_layer_input=None)
+    cfg["text_config"] = {k: v for k, v in cfg["text_config"].items() if v is not None}
+    m = rdet.Model.synthetic(cfg, seed=4, width=16, max_prefill=8192)
+    a, r = m.new_sequence(12), m.new_sequence(12)
+    for s in (a, r):
+        s.prefill([1, 2, 3])
+    rdet.tree_decode(m, [a], [[5, 6, 7]], [[-1, 0, 0]])
+    many = [m.new_sequence(68) for _ in range(128)]
+    for s in many:
+        s.prefill([1])
+    for _ in range(2):
+        with pytest.raises(rdet.RdetError) as e:
+            rdet.tree_decode(m, many, [[1] * 64] * 128, [[-1] * 64] * 128)
+        assert e.value.code == RDET_E_OOM
+    picked = rdet.tree_select(m, [a])
+    rdet.tree_accept(m, [a], [[0, 2]])
+    for t, p in ((5, picked[0][0]), (7, picked[0][2])):
+        r.decode(t)
+        assert r.select() == p
+    assert np.array_equal(a.read(rdet.BUF_LOGITS), r.read(rdet.BUF_LOGITS))
+    for l in range(m.L):
+        assert a.commitment(rdet.BUF_LAYER_OUTPUT, l) == r.commitment(rdet.BUF_LAYER_OUTPUT, l)
+    assert a.commitment(rdet.BUF_KV) == r.commitment(rdet.BUF_KV)
+    rdet.tree_decode(m, [a], [[5, 6]], [[-1, 0]])  # and the context goes on
+    assert rdet.tree_select(m, [a])[0]
+    m.close()
