@@ -1,5 +1,6 @@
 // Device memory that a context replaces as its calls need more of it.  `A`
-// gives the memory: void* alloc(size_t), which throws where there is none.
+// gives and takes the memory: void* alloc(size_t), which throws where there is
+// none, and void release(void*), which waits until nothing uses it any more.
 #pragma once
 #include <cstddef>
 #include <cstdint>
@@ -23,20 +24,33 @@ struct GrowBuf {
     } catch (...) {
       n = a.alloc(want = need);
     }
+    if (p) a.release(p);
     p = n;
     bytes = want;
   }
 };
 
-// Rows of one size, `extra` bytes for all of them together.
+// Rows of one size, `extra` bytes for all of them together: at least `least`
+// rows, and twice as many as before when they grow, but not more than `most`
+// (which every need is within) for either reason.
 struct GrowRows {
   void* p = nullptr;
   int rows = 0;
   template <class A>
-  void reserve(A& a, int need, int least, size_t row_bytes, size_t extra) {
+  void reserve(A& a, int need, int least, int most, size_t row_bytes, size_t extra) {
     if (rows >= need) return;
-    const int want = need > least ? need : least;
-    p = a.alloc((size_t)want * row_bytes + extra);
+    int want = rows > 0 ? 2 * rows : least;
+    if (want > most) want = most;
+    if (want < need) want = need;
+    void* n = nullptr;
+    try {
+      n = a.alloc((size_t)want * row_bytes + extra);
+    } catch (...) {
+      if (want == need) throw;
+      n = a.alloc((size_t)(want = need) * row_bytes + extra);
+    }
+    if (p) a.release(p);
+    p = n;
     rows = want;
   }
 };
@@ -46,14 +60,14 @@ struct GrowRows {
 // and the epoch, which ends earlier trees, after them: a call that fails here
 // leaves every tree of an earlier one as it was.
 struct PassNeed {
-  int rows;
+  int rows, most;
   size_t table_row, table_extra, workspace, tree_row, tree_extra;
 };
 template <class A>
 void reserve_pass(A& a, const PassNeed& n, GrowRows& tables, GrowBuf& ws, GrowRows& tree, uint64_t& epoch) {
-  tables.reserve(a, n.rows, 8, n.table_row, n.table_extra);
+  tables.reserve(a, n.rows, 8, n.most, n.table_row, n.table_extra);
   ws.reserve(a, n.workspace);
-  tree.reserve(a, n.rows, 64, n.tree_row, n.tree_extra);
+  tree.reserve(a, n.rows, 64, n.most, n.tree_row, n.tree_extra);
   epoch += 1;
 }
 

@@ -608,11 +608,10 @@ struct Ctx {
   } tree;
   // selection under rules: tokens (up to rows), the rules' arrays in pinned and device memory
   struct {
-    uint32_t* tok = nullptr;
-    int rows = 0;
+    GrowBuf tok;
     unsigned char* host = nullptr;
-    unsigned char* dev = nullptr;
-    size_t bytes = 0;
+    size_t host_bytes = 0;
+    GrowBuf dev;
   } rules;
   CommitPipe cp;
   KvStage kvs;
@@ -623,7 +622,13 @@ struct Ctx {
   }
   template <typename T>
   T* dalloc_n(size_t n) { return static_cast<T*>(dalloc(n * sizeof(T))); }
-  void* alloc(size_t bytes) { return dalloc(bytes); }  // for the growing buffers
+  // for the growing buffers
+  void* alloc(size_t bytes) { return dalloc(bytes); }
+  void release(void* p) {
+    CK(cudaStreamSynchronize(stream));  // every use of them is on this stream
+    allocs.erase(std::find(allocs.begin(), allocs.end(), p));
+    CK(cudaFree(p));
+  }
   // A copy to or from host memory behind the stream's work, complete on return.
   // (cudaMemcpy runs on the legacy default stream, which neither waits for a
   // non-blocking stream nor is waited for by one: it read synthetic scalars
@@ -1835,7 +1840,7 @@ struct BatchRow {
 };
 // Bytes of one row of the batch tables: its pointers, id, capacity, place and logits.
 static size_t batch_row_bytes(const ModelCfg& m) { return (4 + 2 * (size_t)m.L) * 8 + 12 + (size_t)m.V * 4; }
-static void batch_reserve(Ctx& c, int B) { c.bw.mem.reserve(c, B, 8, batch_row_bytes(c.cfg), 256); }
+static void batch_reserve(Ctx& c, int B) { c.bw.mem.reserve(c, B, 8, (int)c.max_prefill, batch_row_bytes(c.cfg), 256); }
 static void batch_tables(Ctx& c, const std::vector<BatchRow>& in) {
   const ModelCfg& m = c.cfg;
   auto& bw = c.bw;
@@ -2494,7 +2499,8 @@ static void tree_decode(Ctx& c, const std::vector<Seq*>& seqs, const uint32_t* c
     g.nnode += n;
     maxcap = std::max(maxcap, q.cap);
   }
-  reserve_pass(c, PassNeed{B, batch_row_bytes(m), 256, tree_workspace(c, tb), (2 + (size_t)m.L * m.H + m.V) * 4, 512},
+  reserve_pass(c, PassNeed{B, (int)c.max_prefill, batch_row_bytes(m), 256, tree_workspace(c, tb),
+                           (2 + (size_t)m.L * m.H + m.V) * 4, 512},
                c.bw.mem, tr.ws, tr.mem, tr.epoch);
   // nothing below fails for want of memory; earlier trees' buffers are overwritten
   auto up = [](void* p) { return reinterpret_cast<int32_t*>((reinterpret_cast<uintptr_t>(p) + 255) & ~(uintptr_t)255); };
@@ -2547,22 +2553,19 @@ static std::vector<rdet_rules> stage_rules(Ctx& c, const rdet_rules* rules, size
     bytes += ((r.allow ? masks[i] * words : 0) + r.history_len + 2 * (size_t)r.n_bias) * 4;
   }
   auto& rs = c.rules;
-  if (rs.bytes < bytes) {
-    if (rs.host) CK(cudaFreeHost(rs.host));
-    rs.host = nullptr;
-    rs.bytes = 0;
-    const size_t grown = 2 * bytes;  // histories grow by a token a step
+  rs.dev.reserve(c, bytes);  // doubled: histories grow by a token a step
+  if (rs.host_bytes < bytes) {
     void* h = nullptr;
-    CK(cudaHostAlloc(&h, grown, cudaHostAllocDefault));
+    CK(cudaHostAlloc(&h, rs.dev.bytes, cudaHostAllocDefault));
+    if (rs.host) cudaFreeHost(rs.host);
     rs.host = static_cast<unsigned char*>(h);
-    rs.dev = static_cast<unsigned char*>(c.dalloc(grown));
-    rs.bytes = grown;
+    rs.host_bytes = rs.dev.bytes;
   }
   size_t at = 0;
   auto put = [&](const void* src, size_t count) -> const void* {
     if (!src || count == 0) return nullptr;
     memcpy(rs.host + at, src, count * 4);
-    const void* dst = rs.dev + at;
+    const void* dst = static_cast<unsigned char*>(rs.dev.p) + at;
     at += count * 4;
     return dst;
   };
@@ -2574,7 +2577,7 @@ static std::vector<rdet_rules> stage_rules(Ctx& c, const rdet_rules* rules, size
     r.bias_values = static_cast<const int32_t*>(put(r.bias_values, r.n_bias));
     out.push_back(r);
   }
-  if (at) CK(cudaMemcpyAsync(rs.dev, rs.host, at, cudaMemcpyHostToDevice, c.stream));
+  if (at) CK(cudaMemcpyAsync(rs.dev.p, rs.host, at, cudaMemcpyHostToDevice, c.stream));
   return out;
 }
 // One logit row under staged rules r (nullptr: none), whose mask is r's mask-th.
@@ -2600,17 +2603,14 @@ static rdet_logit_row rules_row(const Ctx& c, const rdet_rules* r, const int32_t
 static void select_under_rules(Ctx& c, const std::vector<rdet_logit_row>& rows, uint32_t* tokens_out) {
   const int n = (int)rows.size();
   if (n == 0) return;
-  if (c.rules.rows < n) {
-    const int cap = std::max(n, 64);
-    c.rules.tok = c.dalloc_n<uint32_t>((size_t)cap);
-    c.rules.rows = cap;
-  }
-  const int32_t rc = rdet_det_logits_rules(rows.data(), (uint32_t)n, (uint32_t)c.cfg.V, c.rules.tok, c.stream);
+  c.rules.tok.reserve(c, std::max(n, 64) * sizeof(uint32_t));
+  uint32_t* const tok = static_cast<uint32_t*>(c.rules.tok.p);
+  const int32_t rc = rdet_det_logits_rules(rows.data(), (uint32_t)n, (uint32_t)c.cfg.V, tok, c.stream);
   if (rc != RDET_OK) {
     CK(cudaStreamSynchronize(c.stream));  // the staged rules may still be copied from
     throw Fail{rc, g_last_error};
   }
-  CK(cudaMemcpyAsync(tokens_out, c.rules.tok, (size_t)n * 4, cudaMemcpyDeviceToHost, c.stream));
+  CK(cudaMemcpyAsync(tokens_out, tok, (size_t)n * 4, cudaMemcpyDeviceToHost, c.stream));
   CK(cudaStreamSynchronize(c.stream));
 }
 

@@ -23,6 +23,10 @@ struct FakeAlloc {
     if (held > most) most = held;
     return p;
   }
+  void release(void* p) {
+    held -= live.at(p);
+    live.erase(p);
+  }
   void arm(uint64_t f) {
     fail = f;
     calls = 0;
@@ -70,7 +74,7 @@ int passes(int victim, uint64_t fail) {
   for (int i = 0; i < 7; ++i) {
     const rdet::GrowRows tree0 = tree;
     const uint64_t epoch0 = epoch;
-    const rdet::PassNeed n{rows[i], 4000, 256, (size_t)rows[i] * 3000, 9000, 768};
+    const rdet::PassNeed n{rows[i], 4096, 4000, 256, (size_t)rows[i] * 3000, 9000, 768};
     a.arm(i == victim ? fail : 0);
     bool failed = false;
     try {
@@ -83,7 +87,28 @@ int passes(int victim, uint64_t fail) {
     if (!a.holds(tree.p, tree.rows ? (size_t)tree.rows * n.tree_row + n.tree_extra : 0)) return 21 + i;
     if (!a.holds(tables.p, tables.rows ? (size_t)tables.rows * n.table_row + n.table_extra : 0)) return 31 + i;
     if (!a.holds(ws.p, ws.bytes)) return 41 + i;
+    if (a.live.size() > 3) return 51 + i;  // nothing superseded stays
   }
   return 0;
+}
+
+// Passes that need one row more each time: allocations in all (their number
+// grows with the logarithm), or -1 where more than the buffers in use and one
+// beside them was ever held.
+int growing(int passes, int most) {
+  FakeAlloc a;
+  rdet::GrowRows tables, tree;
+  rdet::GrowBuf ws;
+  uint64_t epoch = 0;
+  int calls = 0;
+  for (int i = 1; i <= passes; ++i) {
+    const rdet::PassNeed n{i, most, 4000, 256, (size_t)i * 3000, 9000, 768};
+    a.arm(0);
+    rdet::reserve_pass(a, n, tables, ws, tree, epoch);
+    calls += a.calls;
+    if (tree.rows > most || tables.rows > most || a.live.size() != 3) return -1;
+  }
+  const size_t last = (size_t)tree.rows * 9000 + 768 + (size_t)tables.rows * 4000 + 256 + ws.bytes;
+  return a.held == last && a.most <= 2 * last ? calls : -1;
 }
 }

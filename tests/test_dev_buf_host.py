@@ -24,6 +24,7 @@ def host():
     L = C.CDLL(out)
     L.workspace.argtypes = [C.c_uint64, C.c_uint64]
     L.passes.argtypes = [C.c_int, C.c_uint64]
+    L.growing.argtypes = [C.c_int, C.c_int]
     return L
 
 
@@ -59,3 +60,8 @@ def test_a_pass_takes_its_memory_at_once():
     body = body[:body.index("\n}\n")]
     assert "dalloc" not in body and "epoch +=" not in body and body.count("reserve_pass(") == 1
     assert not re.search(r"\btr\.(dec_out|logits|pos|rows)\s*=", body[:body.index("reserve_pass(")])
+
+
+def test_growing_passes_replace_their_buffers_rarely_and_keep_none(host):
+    assert 0 < host.growing(4000, 4096) <= 3 * 12
+    assert 0 < host.growing(40, 40) <= 3 * 6

@@ -5,6 +5,7 @@ import pytest
 
 from helpers import mini_config, rdet
 
+torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 RDET_E_OOM = -7
@@ -55,4 +56,35 @@ def test_a_refused_tree_decode_keeps_the_trees_before_it():
     assert a.commitment(rdet.BUF_KV) == r.commitment(rdet.BUF_KV)
     rdet.tree_decode(m, [a], [[5, 6]], [[-1, 0]])  # and the context goes on
     assert rdet.tree_select(m, [a])[0]
+    m.close()
+
+
+def test_growing_trees_and_rules_keep_no_superseded_buffers():
+    # every call needs more rows than any before it; a row of a million logits is
+    # 4 MB in the batch tables and 4 MB among the trees' outputs
+    vocab, nseq = 1 << 20, 8
+    cfg = mini_config(vocab_size=vocab, hidden_size_per_layer_input=None)
+    cfg["text_config"] = {k: v for k, v in cfg["text_config"].items() if v is not None}
+    m = rdet.Model.synthetic(cfg, seed=4, width=16, max_prefill=512)
+    seqs = [m.new_sequence(600) for _ in range(nseq)]
+    ref = m.new_sequence(600)
+    for s in (*seqs, ref):
+        s.prefill([1, 2, 3])
+    rdet.tree_decode(m, seqs, [[1]] * nseq, [[-1]] * nseq)  # loads the kernels
+    rdet.tree_select(m, seqs, [dict(history=[1])] * nseq)
+    torch.cuda.synchronize()
+    before, rows, at = torch.cuda.mem_get_info()[0], 0, 3
+    for n in range(9, 26):
+        rdet.tree_decode(m, seqs, [[(7 * n + j) % vocab for j in range(n)]] * nseq, [list(range(-1, n - 1))] * nseq)
+        picked = rdet.tree_select(m, seqs, [dict(history=list(range(40 * n)))] * nseq)
+        assert all(p == picked[0] for p in picked)
+        rdet.tree_accept(m, seqs, [[0, 1]] * nseq)
+        for j in range(2):
+            ref.decode((7 * n + j) % vocab)
+        rows = n * nseq
+    used = before - torch.cuda.mem_get_info()[0]
+    assert used <= 2 * rows * 2 * (vocab + 4096) * 4 + (256 << 20), used
+    for s in seqs:
+        assert np.array_equal(s.read(rdet.BUF_LOGITS), ref.read(rdet.BUF_LOGITS))
+        assert s.commitment(rdet.BUF_KV) == ref.commitment(rdet.BUF_KV)
     m.close()
