@@ -280,7 +280,8 @@ int32_t rdet_det_attention_decode_noalloc(const int32_t* q, const int32_t* k_cac
  * context + depth(i).  The operators below take caller-owned memory, launch on
  * `stream` (a cudaStream_t or NULL), allocate nothing and keep nothing from one
  * call for the next, so calls on different streams may overlap as long as
- * their outputs and workspaces do not.  Their descriptor arrays are host
+ * their outputs and workspaces do not.  rdet_det_status tells whether the
+ * kernels of a stream ended as they should.  Their descriptor arrays are host
  * memory that is read before the call returns.  No counterpart in the
  * reference, which decodes one token at a time; the arithmetic is det_num v1's. */
 typedef struct rdet_tree_seq {
@@ -354,6 +355,14 @@ typedef struct rdet_tree_move {
 } rdet_tree_move;
 int32_t rdet_det_tree_commit(const rdet_tree_move* moves, uint32_t n_moves, const uint32_t* nodes,
                              const uint32_t* path_off, uint32_t n_paths, void* stream);
+
+/* The kernel-level entry points return before their kernels run.  A kernel
+ * whose pipeline wait gives up (after about a second) ends with wrong rows and
+ * sets an error word of the device.  This call waits for `stream` and returns
+ * RDET_E_CUDA when one is set on the current device, by whichever launch since
+ * they were last read, and clears them; RDET_OK otherwise.  (A context's own
+ * calls read them as well, and return RDET_E_CUDA.)  Not during stream capture. */
+int32_t rdet_det_status(void* stream);
 
 /* Tensor-parallel batched decode (no counterpart in the reference, which runs
  * one process on the CPU).  Every rank

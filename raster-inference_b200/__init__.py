@@ -40,7 +40,7 @@ SYMBOLS = [
     "rdet_tree_accept", "rdet_read", "rdet_commitment", "rdet_kv_prefix_commitments",
     "rdet_det_gemv", "rdet_det_linear",
     "rdet_det_attention_decode", "rdet_det_attention_decode_noalloc", "rdet_det_attention_prefill", "rdet_convert_to_wgt",
-    "rdet_det_attention_tree_workspace", "rdet_det_attention_tree", "rdet_det_logits_rules", "rdet_det_tree_commit",
+    "rdet_det_attention_tree_workspace", "rdet_det_attention_tree", "rdet_det_logits_rules", "rdet_det_tree_commit", "rdet_det_status",
     "rdet_get_stream", "rdet_tensor_core_prefill", "rdet_nccl_unique_id", "rdet_tp_init", "rdet_tp_world", "rdet_tp_shard_logits", "rdet_tp_ipc_export", "rdet_tp_ipc_connect", "rdet_seq_kernels_per_step", "rdet_last_error",
     "rdet_version",
 ]
@@ -142,6 +142,7 @@ def lib() -> C.CDLL:
         "rdet_det_attention_tree": [p, u32, p, u32, u32, u32, u32, p, p, sz, p],
         "rdet_det_logits_rules": [p, u32, u32, p, p],
         "rdet_det_tree_commit": [p, u32, p, p, u32, p],
+        "rdet_det_status": [p],
         "rdet_get_stream": [p, p],
         "rdet_tensor_core_prefill": [p],
         "rdet_nccl_unique_id": [p, sz],
@@ -632,3 +633,9 @@ def tree_moves(moves, paths) -> Descriptors:
 def det_tree_commit(moves: Descriptors, stream: int = 0):
     """The drafted K/V rows of accepted paths into the caches (rdet_det_tree_commit)."""
     _check(lib().rdet_det_tree_commit(moves.array, moves.n, moves.nodes, moves.path_off, moves.n_paths, stream))
+
+
+def det_status(stream: int = 0):
+    """Waits for the stream and raises when a kernel on the current device gave
+    up on a pipeline wait since this was last asked (rdet_det_status)."""
+    _check(lib().rdet_det_status(stream))

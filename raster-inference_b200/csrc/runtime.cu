@@ -1094,11 +1094,13 @@ static bool row_norm(Ctx& c, RowNormArgs ra, int B, ActPlanes* ap) {
   return true;
 }
 
+constexpr char kPipelineError[] =
+    "a pipeline wait gave up in a kernel on this device since the error words were last read";
 static void check_err_flag(Ctx& c, const char* what) {
   launch_error_words(c.err_words, c.d_err, c.h_err, c.stream);
   CK(cudaGetLastError());
   CK(cudaStreamSynchronize(c.stream));
-  if (c.h_err[1]) throw Fail{RDET_E_CUDA, std::string(what) + ": a weight-streaming pipeline wait timed out"};
+  if (c.h_err[1]) throw Fail{RDET_E_CUDA, std::string(what) + ": " + kPipelineError};
   if (c.h_err[0]) throw Fail{RDET_E_RANGE, std::string(what) + ": token id is out of bounds for the embedding tensor"};
 }
 
@@ -3972,6 +3974,25 @@ int32_t rdet_det_tree_commit(const rdet_tree_move* moves, uint32_t n_moves, cons
     for (const auto& part : parts)
       launch_tree_commit(part->m, (int)part->moves, (int)part->paths, static_cast<cudaStream_t>(stream));
     CK(cudaGetLastError());
+  });
+}
+
+int32_t rdet_det_status(void* stream) {
+  return guard([&] {
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const ErrorWords words = error_words();
+    int32_t set[kErrorWords] = {};
+    CK(cudaGetLastError());
+    for (int i = 0; i < kErrorWords; ++i) CK(cudaMemcpyAsync(&set[i], words.w[i], 4, cudaMemcpyDeviceToHost, s));
+    CK(cudaStreamSynchronize(s));
+    bool any = false;
+    for (int i = 0; i < kErrorWords; ++i)
+      if (set[i]) {
+        any = true;
+        CK(cudaMemsetAsync(words.w[i], 0, 4, s));
+      }
+    if (any) CK(cudaStreamSynchronize(s));
+    REQUIRE(!any, RDET_E_CUDA, kPipelineError);
   });
 }
 
