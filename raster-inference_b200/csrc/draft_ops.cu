@@ -63,7 +63,9 @@ struct RuleSmem {
   uint16_t list[kRuleSlots];            // the slots in use, in any order
 };
 
-// loads and stores of rows that are touched once
+// Loads of rows that are touched once, and of the words of rules.  None is .nc:
+// this grid may be resident already while the grid before it writes what it
+// reads, so only coherent loads behind the wait see it.
 __device__ __forceinline__ void ld_stream(int4& v, const int32_t* p, bool on) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %5, 0;\n @p ld.global.L1::no_allocate.v4.s32 {%0, %1, %2, %3}, [%4];\n}"
@@ -97,7 +99,11 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) logit_rules_kernel(co
   do_go();
   const bool any = hlen > 0 || nbias > 0 || rs.row[row].has_path;
   const bool wide = ((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-  auto allowed = [&](uint32_t w) { return allow ? __ldg(allow + w) : 0xffffffffu; };
+  auto allowed = [&](uint32_t w) {
+    uint32_t v = 0xffffffffu;
+    ld_word(v, allow + w, allow != nullptr);
+    return v;
+  };
   uint64_t b = 0;
   // the thread's first maximum of unmarked tokens (they come in ascending
   // order), and the first of them where all are at the lowest value

@@ -27,3 +27,13 @@ def test_error_words_are_not_copied_one_by_one():
         if name.endswith(".cu"):
             code = re.sub(r"//[^\n]*", "", open(os.path.join(csrc, name)).read())
             assert not re.findall(r"cudaMemcpy(?:From|To)Symbol\(", code), name
+
+
+def test_overlapping_grids_load_coherently():
+    # kernels that may be resident while the grid before them writes their inputs:
+    # the non-coherent path wants data that nobody writes while the kernel lives
+    csrc = os.path.join(ROOT, "raster-inference_b200", "csrc")
+    for name in ("draft_ops.cu", "tree_attn.cu"):
+        code = re.sub(r"//[^\n]*", "", open(os.path.join(csrc, name)).read())
+        assert "griddepcontrol.wait" in code
+        assert not re.findall(r"__ldg\(|ld\.global\.nc|__restrict__", code), name
