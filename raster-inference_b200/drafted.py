@@ -90,9 +90,11 @@ def run_output_decode(model, seqs, prompts, max_new_tokens: int, nodes: int = 16
     prompts[i] are the tokens behind sequence i's cache.  rules[i] (or None for
     all): bias, repetition, frequency and presence as rdet.select_rules takes
     them, the prompt and the output being the history, and allow, a function
-    from the output so far to the mask of the next token.  A sequence ends
-    early where its mask allows no token.  stats, a dict, receives the number
-    of passes over the weights."""
+    from the output so far to the mask of the next token.  It is asked about
+    outputs shorter than max_new_tokens whose every token its own masks allow,
+    and about no others, as in a loop of one token a step: drafted nodes that a
+    mask forbids are dropped.  A sequence ends early where its mask allows no
+    token.  stats, a dict, receives the number of passes over the weights."""
     if not 1 <= nodes <= rdet.MAX_TREE_NODES:
         raise ValueError(f"nodes: 1 to {rdet.MAX_TREE_NODES}")
     if len(prompts) != len(seqs) or (rules is not None and len(rules) != len(seqs)):
@@ -116,6 +118,10 @@ def run_output_decode(model, seqs, prompts, max_new_tokens: int, nodes: int = 16
             s = [seqs[i] for i in part]
             trees = [drafts[i].tree(nxt[i], min(nodes if len(out[i]) + 1 < max_new_tokens else 1, model.max_prefill,
                                                 seqs[i].max_ctx - seqs[i].position)) for i in part]
+            masks = [None] * len(part)
+            for k, i in enumerate(part):
+                if allow[i]:
+                    trees[k], masks[k] = _admissible(allow[i], out[i], max_new_tokens, model.V, *trees[k])
             if stats is not None:
                 stats["passes"] = stats.get("passes", 0) + 1
             if len(part) == 1 and len(trees[0][0]) == 1:
@@ -126,14 +132,12 @@ def run_output_decode(model, seqs, prompts, max_new_tokens: int, nodes: int = 16
                 for t in (out[i], text[i]):
                     t.append(nxt[i])
                 drafts[i].extend([nxt[i]])
-                nxt[i] = seqs[i].select() if rules is None else rdet.select_rules(
-                    model, s, [_rules_of(rules[i], text[i], allow[i] and [allow[i](out[i])])])[0]
+                if len(out[i]) < max_new_tokens:
+                    nxt[i] = seqs[i].select() if rules is None else rdet.select_rules(
+                        model, s, [_rules_of(rules[i], text[i], masks[0])])[0]
                 continue
             rdet.tree_decode(model, s, [t for t, _ in trees], [p for _, p in trees])
-            lists = None
-            if rules is not None:
-                lists = [_rules_of(rules[i], text[i], allow[i] and _masks(allow[i], out[i], *t))
-                         for i, t in zip(part, trees)]
+            lists = None if rules is None else [_rules_of(rules[i], text[i], m) for i, m in zip(part, masks)]
             picked = rdet.tree_select(model, s, lists)
             paths = [accepted_path(*t, sel, max_new_tokens - len(out[i])) for i, t, sel in zip(part, trees, picked)]
             rdet.tree_accept(model, s, paths)
@@ -145,9 +149,27 @@ def run_output_decode(model, seqs, prompts, max_new_tokens: int, nodes: int = 16
                 nxt[i] = sel[path[-1]]
 
 
-def _masks(allow, output, tokens, parents):
-    """The mask after every node: its path is the output so far, its ancestors and itself."""
-    paths: list[list[int]] = []
-    for t, p in zip(tokens, parents):
-        paths.append((list(output) if p < 0 else paths[p]) + [t])
-    return [allow(p) for p in paths]
+def _admissible(allow, output, limit, vocab, tokens, parents):
+    """The nodes of a drafted tree that the masks allow behind `output`, as
+    (tokens, parents), and the mask after each.  Node 0 is the token that was
+    selected, so it is allowed.  An output of `limit` tokens is complete: no
+    node follows it, and its mask, which nothing selects under, allows all."""
+    kept: list[int] = []   # old numbers
+    new: dict[int, int] = {}
+    masks, paths, words = [], [], (vocab + 31) // 32
+    for j, (t, p) in enumerate(zip(tokens, parents)):
+        if j:
+            if p not in new or t >= vocab or len(paths[new[p]]) >= limit:
+                continue
+            if not int(masks[new[p]][t >> 5]) >> (t & 31) & 1:
+                continue
+        new[j] = len(kept)
+        kept.append(j)
+        paths.append((list(output) if j == 0 else paths[new[p]]) + [t])
+        mask = np.full(words, 0xFFFFFFFF, dtype=np.uint32)
+        if len(paths[-1]) < limit:
+            mask = np.ascontiguousarray(allow(paths[-1]), dtype=np.uint32)
+            if mask.shape != (words,):
+                raise ValueError(f"allow: a mask of {words} words")
+        masks.append(mask)
+    return ([tokens[j] for j in kept], [new[parents[j]] if j else -1 for j in kept]), masks
