@@ -3231,6 +3231,12 @@ int32_t rdet_generate(rdet_ctx* ctx, rdet_seq* seq, uint32_t n_tokens, uint32_t*
       q.d_hist = static_cast<uint32_t*>(q.dalloc((size_t)std::max<uint32_t>(n_tokens, 1) * 4));
       q.hist_cap = (int)n_tokens;
     }
+    if (n_tokens) {
+      // The steps advance the position on the device and overwrite rows behind
+      // the committed ones: a failed call leaves a sequence to be prefilled again.
+      q.prefilled = false;
+      q.tree_parents.clear();
+    }
     for (uint32_t i = 0; i < n_tokens; ++i) {
       select_launch(c, q);
       CK(cudaMemcpyAsync(q.d_hist + i, q.d_token, 4, cudaMemcpyDeviceToDevice, c.stream));
@@ -3239,6 +3245,7 @@ int32_t rdet_generate(rdet_ctx* ctx, rdet_seq* seq, uint32_t n_tokens, uint32_t*
     if (n_tokens) CK(cudaMemcpyAsync(tokens_out, q.d_hist, (size_t)n_tokens * 4, cudaMemcpyDeviceToHost, c.stream));
     CK(cudaStreamSynchronize(c.stream));
     check_err_flag(c, "generate");
+    q.prefilled = true;
     q.pos += (int)n_tokens;
     q.last_was_prefill = false;
   });
