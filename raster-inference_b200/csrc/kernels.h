@@ -380,7 +380,10 @@ void launch_tp_signal(const TpPeerFlags& peers, int32_t world, int32_t rank, uin
 // One launch group of the tree attention: sequences and the nodes of their
 // trees by value (kernel parameters), so a call copies nothing to the device.
 constexpr int kTreeNodes = 64;        // nodes of one tree at most (ancestor masks are 64 bits)
-constexpr int kTreeMaxKeys = 16 * 32704;  // attended rows of one sequence: at most 32 value CTAs' s32 accumulators
+// Attended rows of one sequence: the sixteen CTAs of a row's softmax cluster hold
+// 32768 keys each.  (A value CTA's s32 sums hold 32704; its plan takes as many
+// CTAs as it likes.)
+constexpr int kTreeMaxKeys = 16 * 32704;
 constexpr int kTreeGroupSeqs = 32, kTreeGroupNodes = 512;
 struct TreeSeq {
   const int32_t *k = nullptr, *v = nullptr;    // [Hkv, cap, d]

@@ -85,7 +85,10 @@ def run_output_decode(model, seqs, prompts, max_new_tokens: int, nodes: int = 16
                       stats=None) -> list[list[int]]:
     """The greedy tokens of every prefilled sequence, as
     rdet.run_output_decode gives them one sequence at a time, with up to
-    `nodes` drafted tokens per sequence and step.
+    `nodes` drafted tokens per sequence and step.  It drafts whenever the draft
+    offers a tree and does not measure what is accepted: drafts that are never
+    right cost a lone sequence up to twice the time of one token a step (E4B
+    shape, 128 tokens: 0.96 s against 0.48; without a draft to offer 0.49).
 
     prompts[i] are the tokens behind sequence i's cache.  rules[i] (or None for
     all): bias, repetition, frequency and presence as rdet.select_rules takes
