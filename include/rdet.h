@@ -125,7 +125,8 @@ int32_t rdet_decode_finalize(rdet_ctx* ctx, rdet_seq* seq);
 /* Greedy generation on the device (native.rs:265-450 loop: select ->
  * decode_transition, n_tokens times), each decode_transition replayed as the
  * sequence's CUDA graph.  Writes the n_tokens selected ids; logits of the
- * last decode stay resident. */
+ * last decode stay resident.  A call that
+ * fails once its steps run leaves the sequence to be prefilled again. */
 int32_t rdet_generate(rdet_ctx* ctx, rdet_seq* seq, uint32_t n_tokens, uint32_t* tokens_out);
 
 /* ---- drafted decoding -------------------------------------------------------

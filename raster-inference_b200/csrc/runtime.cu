@@ -3224,7 +3224,7 @@ int32_t rdet_generate(rdet_ctx* ctx, rdet_seq* seq, uint32_t n_tokens, uint32_t*
     CK(cudaSetDevice(c.device));
     check_decode_ready(c, q);
     REQUIRE(c.decode_owner == nullptr, RDET_E_STATE, "a routine-granular decode is in flight on this context");
-    REQUIRE(q.pos + (int)n_tokens <= q.cap, RDET_E_RANGE, "generation would overflow the sequence KV cache");
+    REQUIRE(n_tokens <= (uint32_t)(q.cap - q.pos), RDET_E_RANGE, "generation would overflow the sequence KV cache");
     require_logits(q);
     ensure_decode_graph(c, q);
     if (q.hist_cap < (int)n_tokens) {

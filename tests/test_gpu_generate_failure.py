@@ -35,3 +35,14 @@ def test_a_failed_generation_asks_for_a_new_prefill():
             x.decode(2)
     assert np.array_equal(s.read(rdet.BUF_LOGITS), r.read(rdet.BUF_LOGITS))
     assert s.commitment(rdet.BUF_KV) == r.commitment(rdet.BUF_KV)
+
+
+def test_counts_past_the_cache_are_refused():
+    # counts of 2^31 and more are negative as an int, so they must not be compared as one
+    m = rdet.Model.synthetic(mini_config(), seed=4, width=16, max_prefill=16)
+    s = m.new_sequence(10)
+    s.prefill([1, 2, 3])
+    out = np.zeros(16, dtype=np.uint32)
+    for n in (8, 1 << 31, (1 << 32) - 4, (1 << 32) - 1):
+        assert rdet.lib().rdet_generate(m._h, s._h, n, out.ctypes.data) == -6
+    assert s.position == 3 and len(s.generate(7)) == 7
